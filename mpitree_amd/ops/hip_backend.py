@@ -823,7 +823,7 @@ class HipBackend:
                            tab.data_ptr())
         kw = dict(tab=tab.data_ptr(), n_tab=S, me=me, emit_prefix=me == 0)
         slot = pool.take_next()  # (agreed last fit: emit before the host wait)
-        if slot is not None:
+        if slot is not None and slot.dev:
             emit(slot.dev + HEADER, (slot.nbytes - HEADER) // bpn, **kw)
         gv = gall.view(Pn, W)
         h = _pinned_copy(torch.cat([total, gv[:, 1], gv[:, 2]]), "shm.total")
@@ -837,8 +837,15 @@ class HipBackend:
             slot = pool.choose(masks, nbytes, shm_free=free)
             if slot is None:
                 return None
-            emit(slot.dev + HEADER, 0, **kw)
+            if slot.dev:
+                emit(slot.dev + HEADER, 0, **kw)
+                torch.cuda.current_stream(self.device).synchronize()
+        if not slot.dev:  # (not registered: through this rank's own pinned memory)
+            stage, dptr = _zc_out(nbytes)
+            stage[nbytes - 4 * N : nbytes].view(np.int32)[:] = -1
+            emit(dptr, 0, **kw)
             torch.cuda.current_stream(self.device).synchronize()
+            slot.copy_nodes(stage[:nbytes], N)
         pool.barrier(slot)
         pool.plan_next(masks, slot, nbytes, shm_free=free)
         self.pos_rec = self.pos_st = None

@@ -9,17 +9,19 @@ the whole tree to host memory over its own PCIe link (2.2 ms at ~55 GB/s) -- a
 cost that does not shrink with P.
 
 When every rank of the group runs on one node, the ranks instead share one host
-buffer per fit (a ``/dev/shm`` mapping registered with the HIP runtime, so a
-kernel can store into it over PCIe):
+buffer per fit (a ``/dev/shm`` mapping):
 
 1. each rank ranks its own position space (replicated prefix + its own
    segments; ``assemble.hip`` asm_rank) and counts the nodes of each of its
    segments (``shm_seg_count``); one all-gather of those counts (a few KB, RCCL);
 2. every rank sorts the segments and derives each of its nodes' final id =
    local rank + nodes of other ranks' segments before it (``shm_seg_prefix``);
-3. each rank's emit kernel writes its own nodes (rank 0 also the prefix) straight
-   into the shared buffer (zero-copy), so each rank moves 1 / P of the tree over
-   PCIe and no node crosses xGMI;
+3. each rank's emit kernel writes its own nodes (rank 0 also the prefix) into pinned
+   host memory of the rank, and the rank copies them into the shared buffer, so each
+   rank moves 1 / P of the tree over PCIe and no node crosses xGMI. With
+   ``MPITREE_SHM_REGISTER=1`` the mapping is registered with the HIP runtime instead and
+   the kernel stores straight into it; not every system lets a process register memory
+   that it did not allocate through HIP, so that is not the default;
 4. a flag barrier in the buffer's header; every rank returns numpy views of the
    same finished tree.
 
@@ -78,7 +80,8 @@ def shm_free_bytes() -> int:
 
 
 class _Slot:
-    """One shared buffer: a /dev/shm mapping, pinned and mapped for the device."""
+    """One shared buffer: a /dev/shm mapping. ``dev``: its device address where it is
+    registered (``MPITREE_SHM_REGISTER=1``), else 0 (nodes are copied into it)."""
 
     def __init__(self, hip, name: str, nbytes: int):
         import _posixshmem
@@ -92,11 +95,40 @@ class _Slot:
         self.name, self.nbytes, self.hip = name, nbytes, hip
         self.nd = np.frombuffer(self.mm, dtype=np.uint8)
         self.host = int(self.nd.ctypes.data)
-        self.dev = int(hip.host_register(self.host, nbytes))
+        registered = os.environ.get("MPITREE_SHM_REGISTER", "0") == "1"
+        self.dev = int(hip.host_register(self.host, nbytes)) if registered else 0
         self.linked = True
 
     def flags(self) -> np.ndarray:
         return self.nd[:HEADER].view(np.int64)
+
+    def copy_nodes(self, stage: np.ndarray, n_nodes: int) -> None:
+        """Copy the nodes that ``stage`` holds into this buffer. ``stage``: the packed
+        columns of a tree of ``n_nodes`` nodes (``TreeArrays.from_packed``), of which only
+        some are written; the last column, the depth, is -1 for the others."""
+        held = stage[-4 * n_nodes :].view(np.int32) >= 0
+        edge = np.flatnonzero(np.diff(held, prepend=False, append=False))
+        runs = list(zip(edge[::2].tolist(), edge[1::2].tolist()))
+        few = len(runs) <= 256  # (ranks own whole subtrees: a few runs of ids, rank 0
+        out = self.nd[HEADER : HEADER + stage.size]  # also the prefix's scattered ones)
+        # 8-byte columns, class counts, 4-byte columns: bytes a node from the total
+        at, width = 0, stage.size // n_nodes
+        for w in self.column_widths(width):
+            src = stage[at : at + n_nodes * w].reshape(n_nodes, w)
+            dst = out[at : at + n_nodes * w].reshape(n_nodes, w)
+            if few:
+                for a, b in runs:
+                    dst[a:b] = src[a:b]
+            else:
+                dst[held] = src[held]
+            at += n_nodes * w
+
+    @staticmethod
+    def column_widths(node_bytes: int) -> list[int]:
+        """Bytes a node takes in each packed column: three of 8 bytes and (classification)
+        the counts, then five of 4."""
+        rest = node_bytes - 3 * 8 - 5 * 4
+        return [8, 8, 8] + ([rest] if rest else []) + [4] * 5
 
     def free(self) -> bool:
         # references: self.nd and getrefcount's argument (tree views add theirs)
@@ -114,10 +146,11 @@ class _Slot:
 
     def close(self):
         self.unlink()
-        try:
-            self.hip.host_unregister(self.host)
-        except Exception:  # pragma: no cover - (teardown)
-            pass
+        if self.dev:
+            try:
+                self.hip.host_unregister(self.host)
+            except Exception:  # pragma: no cover - (teardown)
+                pass
         self.nd = None
         try:
             self.mm.close()

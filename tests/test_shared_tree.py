@@ -139,3 +139,29 @@ def test_exact_own_positions_group_jobs_by_owner():
         want[int(own[j])] += list(range(int(fj[j, 0]), int(fj[j, 0] + fj[j, 1])))
     assert sizes == [len(want[0]), len(want[1])]
     assert pos.tolist() == want[0] + want[1]
+
+
+@pytest.mark.parametrize("C", [0, 2, 7])
+@pytest.mark.parametrize("scattered", [False, True])
+def test_two_ranks_nodes_make_one_tree(C, scattered):
+    """Each rank copies the nodes its staging buffer holds (depth >= 0), whole runs of ids or
+    scattered ones, and nothing else; together they are the tree."""
+    N, width = 3000, 3 * 8 + 4 * C + 5 * 4
+    assert sum(st._Slot.column_widths(width)) == width
+    rng = np.random.default_rng(C)
+    tree = rng.integers(0, 100, size=N * width, dtype=np.uint8)
+    tree[-4 * N :].view(np.int32)[:] = rng.integers(0, 50, size=N)  # depths
+    pool = _pool(uid=0x5EED00 + C + 100 * scattered)
+    slot = pool.choose([0, 0], N * width)
+    mine = rng.random(N) < 0.5 if scattered else (np.arange(N) // 700) % 2 == 0
+    for own in (mine, ~mine):
+        stage = rng.integers(0, 255, size=N * width, dtype=np.uint8)
+        at = 0
+        for w in st._Slot.column_widths(width):
+            col = stage[at : at + N * w].reshape(N, w)
+            col[own] = tree[at : at + N * w].reshape(N, w)[own]
+            at += N * w
+        stage[-4 * N :].view(np.int32)[~own] = -1
+        slot.copy_nodes(stage, N)
+    assert np.array_equal(slot.nd[st.HEADER : st.HEADER + N * width], tree)
+    slot.close()
