@@ -6,6 +6,8 @@ Public API (also importable as ``mpitree.tree``):
 * :class:`ParallelDecisionTreeClassifier`, :class:`ParallelDecisionTreeRegressor`
 * :class:`Node`, :class:`BranchType` -- the linked tree view
 * :class:`TreeArrays` -- the flat fitted-tree format
+* :func:`leaf_embedding`, :func:`leaf_linear`, :func:`leaf_route` -- operators over a tree's
+  leaves: learned vectors and linear models per leaf, with their gradients
 
 Importing has no side effects: no process group, no GPU initialisation.
 """
@@ -18,6 +20,7 @@ from .models.decision_tree import (
 )
 from .models.node import BranchType, Node
 from .models.tree_arrays import TreeArrays
+from .ops.leaf_ops import LeafRoute, leaf_embedding, leaf_linear, leaf_route
 
 __version__ = "0.1.0"
 
@@ -29,4 +32,8 @@ __all__ = [
     "Node",
     "BranchType",
     "TreeArrays",
+    "LeafRoute",
+    "leaf_embedding",
+    "leaf_linear",
+    "leaf_route",
 ]

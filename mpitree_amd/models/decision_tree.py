@@ -33,6 +33,7 @@ from sklearn.utils.validation import check_is_fitted
 
 from ..core.criterion import parse_criterion
 from ..core.fit import fit_tree
+from ..ops.leaf_ops import LeafRoute, leaf_embedding, leaf_linear, leaf_route
 from .tree_arrays import TreeArrays
 from ..utils.level_checkpoint import CheckpointInterrupt
 
@@ -172,6 +173,53 @@ class _BaseTree(BaseEstimator):
 
             return predict_leaves(self, X)
         return self._arrays.apply(_as_numpy_X(X))
+
+    # ----------------------------------------------- learned leaf parameters
+    def _leaf_numbers(self, X):
+        check_is_fitted(self, "n_features_")
+        X = self._check_X_predict(X)
+        if isinstance(X, torch.Tensor) and X.is_cuda:
+            from ..ops.hip_predict import leaf_numbers
+
+            return leaf_numbers(self, X)
+        return torch.from_numpy(self._arrays.leaf_numbers()[self._arrays.apply(_as_numpy_X(X))])
+
+    def _leaves_for(self, X, what, params):
+        """Leaf numbers (or the route) of ``X`` on the parameters' device."""
+        check_is_fitted(self, "n_features_")
+        if not isinstance(params, torch.Tensor) or params.dim() < 1:
+            raise TypeError(f"{what} must be a tensor with one entry per leaf")
+        if params.shape[0] != self.get_n_leaves():
+            raise ValueError(f"{what} has {params.shape[0]} entries, the tree "
+                             f"{self.get_n_leaves()} leaves")
+        if isinstance(X, LeafRoute):
+            return X
+        return self._leaf_numbers(X).to(params.device)
+
+    def leaf_route(self, X) -> LeafRoute:
+        """The rows of ``X`` sorted by the leaf they reach. The leaf operators below take it in
+        place of ``X``: a fitted tree's rows do not change leaves, so a training loop over the
+        leaves' parameters walks and sorts them once."""
+        return leaf_route(self._leaf_numbers(X), self.get_n_leaves())
+
+    def leaf_embedding(self, X, table, *, scale: float = 1.0):
+        """``scale * table[leaf]`` for the leaf of each row: ``table`` is a float tensor
+        [n_leaves, D], leaves numbered in pre-order; differentiable in ``table``
+        (:func:`mpitree_amd.leaf_embedding`). ``X``: rows, or their :meth:`leaf_route`."""
+        return leaf_embedding(self._leaves_for(X, "table", table), table, scale=scale)
+
+    def leaf_linear(self, X, weight, bias=None, *, inputs=None):
+        """A linear model per leaf: ``inputs[i] @ weight[leaf].T + bias[leaf]``, with ``weight``
+        [n_leaves, N, K] and ``bias`` [n_leaves, N]; differentiable in all three
+        (:func:`mpitree_amd.leaf_linear`). ``inputs`` (n, K) defaults to the rows ``X`` themselves,
+        in the weight's type. ``X``: rows, or their :meth:`leaf_route` (then give ``inputs``)."""
+        leaves = self._leaves_for(X, "weight", weight)
+        if inputs is None:
+            if isinstance(X, LeafRoute):
+                raise ValueError("a LeafRoute holds no features: pass inputs")
+            rows = X if isinstance(X, torch.Tensor) else torch.from_numpy(_as_numpy_X(X))
+            inputs = rows.to(device=weight.device, dtype=weight.dtype)
+        return leaf_linear(inputs, leaves, weight, bias)
 
     # --------------------------------------------------------------- export
     def export_text(self, *, feature_names=None, class_names=None, precision=2) -> str:

@@ -119,6 +119,11 @@ class TreeArrays:
         """argmax of per-class counts, ties to the lowest class (reference :125)."""
         return np.argmax(self.count, axis=1)
 
+    def leaf_numbers(self) -> np.ndarray:
+        """int32 [N]: each leaf's number 0..n_leaves-1 in pre-order, -1 for internal nodes."""
+        leaf = self.feature < 0
+        return np.where(leaf, np.cumsum(leaf) - 1, -1).astype(np.int32)
+
     # -------------------------------------------------------------- ordering
     @staticmethod
     def from_unordered(

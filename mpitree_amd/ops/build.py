@@ -32,12 +32,14 @@ ARCH = os.environ.get("MPITREE_OFFLOAD_ARCH", "gfx950")
 HIP_SOURCES = ["hist.hip", "split_scan.hip", "partition.hip", "predict.hip", "misc.hip",
                "finish.hip", "finish_reg.hip", "assemble.hip", "binning.hip", "grow.hip",
                "exact2.hip", "exact_setup.hip", "small_fit.hip", "dp_route.hip", "bindings.cpp",
-               "exact2_bind.cpp", "grow_bind.cpp"]
+               "exact2_bind.cpp", "grow_bind.cpp", "leaf_route.hip", "leaf_embed.hip",
+               "leaf_linear.hip", "leaf_bind.cpp"]
 # device code without the packed f32 instructions, some of whose forms have given wrong
 # results on gfx950 (the host pass warns that it does not know the feature)
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 CPU_SOURCES = ["cpu_builder.cpp"]
-HEADERS = ["common.h", "criterion.h", "cpu_builder_core.h", "grow.h", "tiny_sort.h", "exact2.h"]
+HEADERS = ["common.h", "criterion.h", "cpu_builder_core.h", "grow.h", "tiny_sort.h", "exact2.h",
+           "leaf.h"]
 
 
 def _pybind_includes() -> list[str]:

@@ -37,7 +37,7 @@ void launch_seg_stats(hipStream_t, const uint32_t*, const void*, int, bool, cons
                       void*, int);
 void launch_init_idx(hipStream_t, uint32_t*, const int32_t*, int, int64_t);
 void launch_predict(hipStream_t, const void*, bool, int64_t, int, const void*, const double*,
-                    int32_t*);
+                    int32_t*, bool);
 void launch_bin(hipStream_t, const void*, bool, int64_t, int, const void*, int, int,
                 const int32_t*, const uint8_t*, void*, int, void*, int, int32_t*, int);
 void launch_xlog2x(hipStream_t, double*, int64_t);
@@ -60,6 +60,7 @@ void exact_setup_sort(hipStream_t, const float*, int64_t, int, uint32_t*, uint32
                       uint32_t*, void*, size_t, int32_t*, int32_t*, int, int, const int32_t*);
 void bind_exact2(pybind11::module_& m);
 void bind_grow(pybind11::module_& m);
+void bind_leaf(pybind11::module_& m);
 int exact_setup_chunk();
 void launch_fp_combine(hipStream_t, const int64_t*, int, int, int, const int32_t*, int64_t*);
 void launch_grow_dp_fixup(hipStream_t, const PlanArgs&);
@@ -177,9 +178,9 @@ PYBIND11_MODULE(_hip, m) {
     mt::launch_init_idx(S(s), P<uint32_t>(idx), P<int32_t>(y), lab_shift, n);
   });
   m.def("predict", [](uintptr_t s, uintptr_t X, bool x64, int64_t n, int F, uintptr_t nodes,
-                      uintptr_t thr, uintptr_t leaf) {
+                      uintptr_t thr, uintptr_t leaf, bool number) {
     mt::launch_predict(S(s), P<void>(X), x64, n, F, P<void>(nodes), P<double>(thr),
-                       P<int32_t>(leaf));
+                       P<int32_t>(leaf), number);
   });
   m.def(
       "bin",
@@ -487,6 +488,7 @@ PYBIND11_MODULE(_hip, m) {
   });
   mt::bind_exact2(m);
   mt::bind_grow(m);
+  mt::bind_leaf(m);
   m.def("xlog2x_device", [](uintptr_t s, uintptr_t out, int64_t n) {
     mt::launch_xlog2x(S(s), P<double>(out), n);
   });

@@ -14,10 +14,11 @@ struct NodeRec {
   int32_t feature;  // -1 leaf
   int32_t left;
   int32_t right;
-  int32_t pad;
+  int32_t number;  // of a leaf, among the leaves
 };
 
-template <typename XT>
+// kNumber: writes the leaf's number among the leaves instead of its node index
+template <typename XT, bool kNumber>
 __global__ __launch_bounds__(256) void predict_kernel(const XT* __restrict__ X, int64_t n, int F,
                                                       const NodeRec* __restrict__ nodes,
                                                       const double* __restrict__ thr,
@@ -31,20 +32,24 @@ __global__ __launch_bounds__(256) void predict_kernel(const XT* __restrict__ X, 
     node = ((double)x[r.feature] <= thr[node]) ? r.left : r.right;
     r = nodes[node];
   }
-  leaf[i] = node;
+  leaf[i] = kNumber ? r.number : node;
 }
 
 void launch_predict(hipStream_t stream, const void* X, bool x64, int64_t n, int F,
-                    const void* nodes, const double* thr, int32_t* leaf) {
+                    const void* nodes, const double* thr, int32_t* leaf, bool number) {
   if (n <= 0) return;
   dim3 grid((unsigned)((n + 255) / 256));
+  auto go = [&](auto kern, auto* x) {
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, x, n, F, (const NodeRec*)nodes, thr,
+                       leaf);
+    MT_HIP_CHECK(hipGetLastError());
+  };
   if (x64)
-    hipLaunchKernelGGL(predict_kernel<double>, grid, dim3(256), 0, stream, (const double*)X, n, F,
-                       (const NodeRec*)nodes, thr, leaf);
+    number ? go(predict_kernel<double, true>, (const double*)X)
+           : go(predict_kernel<double, false>, (const double*)X);
   else
-    hipLaunchKernelGGL(predict_kernel<float>, grid, dim3(256), 0, stream, (const float*)X, n, F,
-                       (const NodeRec*)nodes, thr, leaf);
-  MT_HIP_CHECK(hipGetLastError());
+    number ? go(predict_kernel<float, true>, (const float*)X)
+           : go(predict_kernel<float, false>, (const float*)X);
 }
 
 }  // namespace mt

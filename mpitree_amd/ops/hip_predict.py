@@ -20,6 +20,7 @@ def device_tree(est, device):
     rec[:, 0] = ta.feature
     rec[:, 1] = ta.left
     rec[:, 2] = ta.right
+    rec[:, 3] = ta.leaf_numbers()
     thr = np.where(ta.feature >= 0, ta.threshold, 0.0).astype(np.float64)
     nodes = torch.from_numpy(rec).to(device)
     thr_d = torch.from_numpy(thr).to(device)
@@ -29,14 +30,24 @@ def device_tree(est, device):
 
 def predict_leaves(est, X: torch.Tensor) -> torch.Tensor:
     """Leaf index per row of a device feature matrix (int64 tensor on X's device)."""
+    return _walk(est, X, False).long()
+
+
+def leaf_numbers(est, X: torch.Tensor) -> torch.Tensor:
+    """Number of each row's leaf among the leaves (int32 tensor on X's device)."""
+    return _walk(est, X, True)
+
+
+def _walk(est, X: torch.Tensor, number: bool) -> torch.Tensor:
     hip = native.hip()
     if X.dtype not in (torch.float32, torch.float64):
         X = X.double()
     X = X.contiguous()
-    nodes, thr = device_tree(est, X.device)
     n, F = X.shape
-    leaf = torch.empty(n, dtype=torch.int32, device=X.device)
-    hip.predict(torch.cuda.current_stream(X.device).cuda_stream, X.data_ptr(),
-                X.dtype == torch.float64, n, F, nodes.data_ptr(), thr.data_ptr(),
-                leaf.data_ptr())
-    return leaf.long()
+    with torch.cuda.device(X.device):
+        nodes, thr = device_tree(est, X.device)
+        leaf = torch.empty(n, dtype=torch.int32, device=X.device)
+        hip.predict(torch.cuda.current_stream(X.device).cuda_stream, X.data_ptr(),
+                    X.dtype == torch.float64, n, F, nodes.data_ptr(), thr.data_ptr(),
+                    leaf.data_ptr(), number)
+    return leaf

@@ -1,0 +1,540 @@
+"""Operators over a tree's leaves against plain 64-bit implementations.
+
+Bounds: a sum of terms t held in 32 bits is off by at most (terms + 2) 2^-23 sum |t| (a rounding of
+at most 2^-24 for each product and each addition), and rounding the result to the output's type by
+eps / 2 of it (eps of the type: 2^-23, 2^-10, 2^-7), or half the type's smallest step near zero."""
+
+import numpy as np
+import pytest
+import torch
+
+from mpitree_amd import (DecisionTreeClassifier, DecisionTreeRegressor, LeafRoute, leaf_embedding,
+                         leaf_linear, leaf_route)
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def check(got, want, mass, terms, what):
+    """got (any type) against want (float64), a sum of `terms` terms with absolute sum `mass`."""
+    fi = torch.finfo(got.dtype)
+    got = got.detach().double().cpu()
+    bound = (want.abs() * fi.eps / 2 + fi.smallest_normal * fi.eps / 2) * (1 + 2.0 ** -8)
+    bound = bound + (terms + 2) * 2.0 ** -23 * mass * (1 + fi.eps)
+    off = (got - want).abs() - bound
+    assert torch.isfinite(got).all(), what
+    assert (off <= 0).all(), (what, float(off.max()), int(off.argmax()))
+
+
+def draw_leaves(g, n, G, skew=0.0, none=0.0, dtype=torch.int64):
+    p = (torch.arange(G, dtype=torch.float64) + 1) ** -skew
+    ids = torch.searchsorted(torch.cumsum(p / p.sum(), 0),
+                             torch.rand(n, generator=g, dtype=torch.float64)).clamp(max=G - 1)
+    ids = torch.randperm(G, generator=g)[ids]
+    out = torch.rand(n, generator=g) < none
+    ids[out] = torch.where(torch.rand(int(out.sum()), generator=g) < 0.5, -1, G)
+    return ids.to(dtype)
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ------------------------------------------------------------------------------- route
+def check_route(ids, G, device):
+    r = leaf_route(ids.to(device), G)
+    key = np.where((ids.numpy() >= 0) & (ids.numpy() < G), ids.numpy(), G).astype(np.int64)
+    order = np.argsort(key, kind="stable")
+    assert np.array_equal(r.order.cpu().numpy(), order)
+    assert np.array_equal(r.keys.cpu().numpy(), key[order])
+    want = np.searchsorted(key[order], np.arange(G + 1))
+    assert np.array_equal(r.offsets.cpu().numpy(), np.append(want, len(key)))
+    assert np.array_equal(r.counts.cpu().numpy(), np.bincount(key, minlength=G + 1)[:G])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("G", [1, 2, 255, 256, 4097, 65535, 65536, 200_001])
+@pytest.mark.parametrize("n", [0, 1, 64, 65, 4095, 4096, 4097, 50_001])
+def test_route_is_the_stable_sort(device, n, G):
+    dtype = torch.int32 if n % 2 else torch.int64
+    check_route(draw_leaves(gen(n + G), n, G, skew=0.7, none=0.1, dtype=dtype), G, device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", ["last", "none", "ends", "huge"])
+@pytest.mark.parametrize("n", [100, 10_000])
+def test_route_of_extreme_leaves(device, n, kind):
+    G = 70_000
+    ids = {"last": torch.full((n,), G - 1), "none": torch.full((n,), -1),
+           "ends": torch.arange(n) % 2 * (G - 1),
+           "huge": torch.arange(n) % 5 + 2 ** 40 * (torch.arange(n) % 3 == 0)}[kind]
+    check_route(ids, G, device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("G", [3, 1000])
+def test_route_of_many_tiles(G):
+    check_route(draw_leaves(gen(3), 2_200_003, G, skew=0.5, none=0.01), G, "cuda")
+
+
+# --------------------------------------------------------------------------- embedding
+def embed_case(device, n, G, D, dtype, scale, skew, none, ids_dtype=torch.int64, as_route=False):
+    g = gen(n * 7 + G * 3 + D)
+    ids = draw_leaves(g, n, G, skew, none, ids_dtype)
+    table = torch.randn(G, D, generator=g).to(dtype)
+    dy = torch.randn(n, D, generator=g).to(dtype)
+    has = (ids >= 0) & (ids < G)
+    t64, d64 = table.double(), dy.double()
+    want = torch.where(has[:, None], t64[torch.where(has, ids, 0).long()] * scale, 0.0)
+    dwant, dmass = torch.zeros(2, G, D, dtype=torch.float64)
+    dwant.index_add_(0, ids[has].long(), d64[has] * scale)
+    dmass.index_add_(0, ids[has].long(), d64[has].abs() * abs(scale))
+    terms = int(torch.bincount(ids[has].long(), minlength=1).max()) if n else 0
+
+    leaves = leaf_route(ids.to(device), G) if as_route else ids.to(device)
+    p = table.to(device).requires_grad_()
+    y = leaf_embedding(leaves, p, scale=scale)
+    check(y, want, 0 * want, 0, "forward")
+    (dt,) = torch.autograd.grad(y, p, dy.to(device))
+    check(dt, dwant, dmass, terms, "gradient")
+    assert torch.equal(leaf_embedding(leaves, p.detach(), scale=scale), y.detach())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [1, 2, 7, 16, 63, 64, 258, 1024, 2056])
+@pytest.mark.parametrize("n,G", [(1, 1), (1, 5000), (63, 7), (500, 300), (700, 1), (9000, 6)])
+def test_embedding(device, dtype, D, n, G):
+    embed_case(device, n, G, D, dtype, 0.25 if D % 2 else 3.5, 0.8, 0.1 if n > 1 else 0.0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embedding_of_a_route_and_int32(device, dtype):
+    embed_case(device, 5000, 40, 24, dtype, 1.0, 1.5, 0.2, torch.int32, as_route=True)
+    embed_case(device, 5000, 40, 24, dtype, -2.0, 1.5, 0.2, torch.int32)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_embedding_runs_at_the_cut(device):
+    # leaves of exactly 63, 64, 65, 128 and 129 rows side by side, at every offset of the cuts
+    sizes = [63, 1, 64, 65, 0, 128, 129, 64, 3, 200]
+    ids = torch.repeat_interleave(torch.arange(len(sizes)), torch.tensor(sizes))
+    for first in (0, 1, 17, 63):
+        lv = torch.cat([torch.full((first,), 10), ids + 11])
+        d = torch.randn(len(lv), 5, generator=gen(first), dtype=torch.float32)
+        t = torch.zeros(30, 5, device=device, requires_grad=True)
+        (dt,) = torch.autograd.grad(leaf_embedding(lv.to(device), t), t, d.to(device))
+        want = torch.zeros(30, 5, dtype=torch.float64).index_add_(0, lv, d.double())
+        mass = torch.zeros(30, 5, dtype=torch.float64).index_add_(0, lv, d.double().abs())
+        check(dt, want, mass, 200, first)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_embedding_strided_operands(device):
+    g = gen(5)
+    base = torch.randn(50, 40, generator=g)
+    ids = torch.randint(0, 50, (6, 20), generator=g)
+    cuts = [lambda b: b[:, 3:20], lambda b: b[:, ::2], lambda b: b.t()[:20].t(), lambda b: b[:, :1]]
+    for cut in cuts:  # views of the device's copy, not copies of views
+        tab, t = cut(base), cut(base.to(device))
+        y = leaf_embedding(ids.to(device).t(), t, scale=2.0)
+        assert y.shape == (20, 6, tab.shape[1])
+        assert torch.equal(y.cpu(), tab[ids.t()] * 2.0)
+    # a broadcast incoming gradient (y.sum()) and one with strided columns
+    t = base.to(device).requires_grad_()
+    (dt,) = torch.autograd.grad(leaf_embedding(ids.to(device), t).sum(), t)
+    want = torch.bincount(ids.flatten(), minlength=50)[:, None].expand(50, 40).float()
+    assert torch.equal(dt.cpu(), want)
+    up = torch.randn(40, 6, 20, generator=g)
+    (dt,) = torch.autograd.grad(leaf_embedding(ids.to(device), t), t,
+                                up.to(device).permute(1, 2, 0))
+    want = torch.zeros(50, 40, dtype=torch.float64)
+    want.index_add_(0, ids.flatten(), up.permute(1, 2, 0).reshape(-1, 40).double())
+    check(dt, want, want.abs() + 30, 30, "strided")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_embedding_keeps_what_the_table_holds(device):
+    # infinities and NaN come back from their own rows only; an unused NaN row reaches nothing
+    t = torch.ones(4, 3)
+    t[1], t[2] = float("inf"), float("nan")
+    y = leaf_embedding(torch.tensor([0, 1, -1, 3, 9], device=device), t.to(device)).cpu()
+    assert torch.equal(y, torch.tensor([[1.0] * 3, [float("inf")] * 3, [0.0] * 3, [1.0] * 3,
+                                        [0.0] * 3]))
+    # rows without a leaf bring NaN to no gradient
+    dy = torch.ones(3, 2)
+    dy[1] = float("nan")
+    p = torch.zeros(2, 2, device=device, requires_grad=True)
+    y = leaf_embedding(torch.tensor([0, 7, 0], device=device), p)
+    (dt,) = torch.autograd.grad(y, p, dy.to(device))
+    assert torch.equal(dt.cpu(), torch.tensor([[2.0, 2.0], [0.0, 0.0]]))
+
+
+# ------------------------------------------------------------------------------ linear
+def linear_case(device, n, G, K, N, dtype, bias, skew=0.5, none=0.1, seed=0, as_route=False):
+    g = gen(seed + n + 3 * G + 5 * K + 7 * N)
+    ids = draw_leaves(g, n, G, skew, none if n > 1 else 0.0)
+    x = torch.randn(n, K, generator=g).to(dtype)
+    w = (torch.randn(G, N, K, generator=g) * K ** -0.5).to(dtype)
+    b = torch.randn(G, N, generator=g).to(dtype) if bias else None
+    dy = torch.randn(n, N, generator=g).to(dtype)
+    f = dict(dtype=torch.float64)
+    y, ym = torch.zeros(n, N, **f), torch.zeros(n, N, **f)
+    dx, dxm = torch.zeros(n, K, **f), torch.zeros(n, K, **f)
+    dw, dwm = torch.zeros(G, N, K, **f), torch.zeros(G, N, K, **f)
+    db, dbm = torch.zeros(G, N, **f), torch.zeros(G, N, **f)
+    longest = 0
+    for q in range(G):
+        r = torch.nonzero(ids == q).flatten()
+        longest = max(longest, len(r))
+        X, W, D = x[r].double(), w[q].double(), dy[r].double()
+        y[r], ym[r] = X @ W.t(), X.abs() @ W.abs().t()
+        if bias:
+            y[r] += b[q].double()
+            ym[r] += b[q].double().abs()
+        dx[r], dxm[r] = D @ W, D.abs() @ W.abs()
+        dw[q], dwm[q] = D.t() @ X, D.abs().t() @ X.abs()
+        db[q], dbm[q] = D.sum(0), D.abs().sum(0)
+
+    px, pw = x.to(device).requires_grad_(), w.to(device).requires_grad_()
+    pb = b.to(device).requires_grad_() if bias else None
+    leaves = leaf_route(ids.to(device), G) if as_route else ids.to(device)
+    out = leaf_linear(px, leaves, pw, pb)
+    check(out, y, ym, K + 1, "y")
+    grads = torch.autograd.grad(out, [px, pw] + ([pb] if bias else []), dy.to(device))
+    check(grads[0], dx, dxm, N, "dx")
+    check(grads[1], dw, dwm, longest, "dw")
+    if bias:
+        check(grads[2], db, dbm, longest, "db")
+    with torch.no_grad():
+        assert torch.equal(leaf_linear(px, leaves, pw, pb), out)
+
+
+# widths around the tiles' and chunks' edges; rows below and above the route-free form's 64
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K,N", [(1, 1), (8, 16), (32, 1), (33, 17), (64, 64), (100, 130), (7, 200),
+                                 (136, 40), (264, 264), (96, 15)])
+@pytest.mark.parametrize("n,G", [(1, 1), (17, 3), (64, 5), (65, 2), (300, 40), (1000, 3)])
+def test_linear(device, dtype, K, N, n, G):
+    linear_case(device, n, G, K, N, dtype, bias=(K + n) % 2 == 0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,G,K,N", [(64, 1, 40, 24), (50, 2, 513, 33), (3000, 1, 72, 200),
+                                     (3000, 700, 24, 24), (900, 2, 400, 300)])
+def test_linear_leaf_sizes(device, dtype, n, G, K, N):
+    linear_case(device, n, G, K, N, dtype, bias=True, skew=0.0, none=0.0, as_route=True)
+    linear_case(device, n, G, K, N, dtype, bias=False, skew=2.0, none=0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("skew", [0.0, 2.5])
+def test_linear_long_leaves(dtype, skew):
+    # leaves longer than the weight gradient's run, so partial matrices are joined
+    linear_case("cuda", 40_000, 9, 24, 20, dtype, bias=True, skew=skew, none=0.05)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_linear_all_rows_without_a_leaf(device):
+    for n in (5, 500):
+        x = torch.full((n, 8), float("nan"), device=device, requires_grad=True)
+        w = torch.ones(3, 4, 8, device=device, requires_grad=True)
+        b = torch.ones(3, 4, device=device, requires_grad=True)
+        y = leaf_linear(x, torch.full((n,), -1, device=device), w, b)
+        assert torch.equal(y.cpu(), torch.zeros(n, 4))
+        for grad in torch.autograd.grad(y, (x, w, b), torch.full_like(y, float("nan"))):
+            assert torch.equal(grad.cpu(), torch.zeros(grad.shape))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [40, 400])
+def test_linear_nan_stays_in_its_rows(device, n):
+    # a NaN in one row's features reaches that row's output and its leaf's gradients alone, for
+    # widths that end inside a tile
+    x = torch.ones(n, 20)
+    x[7] = float("nan")
+    ids = torch.arange(n) % 4
+    px = x.to(device).requires_grad_()
+    w = torch.ones(4, 18, 20, device=device, requires_grad=True)
+    y = leaf_linear(px, ids.to(device), w)
+    bad = torch.isnan(y).any(1).cpu()
+    assert bad[7] and bad.sum() == 1
+    dx, dw = torch.autograd.grad(y, (px, w), torch.ones_like(y))
+    assert torch.equal(dx.cpu(), torch.full((n, 20), 18.0))
+    assert torch.isnan(dw[3]).all() and torch.equal(dw[:3].cpu(), torch.full((3, 18, 20), n / 4.0))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_strided_operands(device, dtype):
+    g = gen(11)
+    for n in (24, 240):
+        big = torch.randn(n, 60, generator=g).to(dtype)
+        ids = torch.randint(0, 5, (n,), generator=g)
+        wt = (torch.randn(5, 16, 24, generator=g) / 5).to(dtype)
+        for cut in (slice(0, 24), slice(3, 27), slice(8, 32)):
+            x, w = big.to(device)[:, cut], wt.to(device).transpose(1, 2).contiguous()
+            y = leaf_linear(x, ids.to(device), w.transpose(1, 2))
+            assert torch.equal(y, leaf_linear(x.contiguous(), ids.to(device), wt.to(device)))
+        # broadcast incoming gradient, leading dimensions, one row of features for all
+        x = big[:1, :24].to(device).expand(n, 24).reshape(4, n // 4, 24).requires_grad_()
+        y = leaf_linear(x, ids.to(device).reshape(4, -1), wt.to(device))
+        assert y.shape == (4, n // 4, 16)
+        (dx,) = torch.autograd.grad(y.sum(), x)
+        want = wt.double().sum(1)[ids].reshape(4, n // 4, 24)
+        check(dx, want, wt.double().abs().sum(1)[ids].reshape(want.shape), 16, "dx")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_empty_batches(device):
+    t = torch.zeros(4, 8, device=device, requires_grad=True)
+    w = torch.zeros(4, 3, 8, device=device, requires_grad=True)
+    none = torch.zeros((0,), dtype=torch.int64, device=device)
+    y = leaf_embedding(none, t)
+    assert y.shape == (0, 8)
+    assert torch.equal(torch.autograd.grad(y.sum(), t)[0].cpu(), torch.zeros(4, 8))
+    x = torch.zeros(0, 8, device=device, requires_grad=True)
+    y = leaf_linear(x, none, w)
+    assert y.shape == (0, 3)
+    dx, dw = torch.autograd.grad(y.sum(), (x, w))
+    assert dx.shape == (0, 8) and torch.equal(dw.cpu(), torch.zeros(4, 3, 8))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradients_against_differences(device):
+    # f32 analytic gradients against central differences of a 64-bit evaluation of the loss
+    g = gen(21)
+    n, G, K, N = 90, 4, 6, 5
+    ids = draw_leaves(g, n, G, none=0.1)
+    x, w = torch.randn(n, K, generator=g), torch.randn(G, N, K, generator=g)
+    b, t = torch.randn(G, N, generator=g), torch.randn(G, N, generator=g)
+    c = torch.randn(n, N, generator=g)
+
+    def loss64(x, w, b, t):
+        has = (ids >= 0) & (ids < G)
+        q = torch.where(has, ids, 0)
+        y = (torch.einsum("nk,nmk->nm", x, w[q]) + b[q]) * (2.0 * t[q])
+        return float((torch.where(has[:, None], y, 0.0) * c.double()).sum().detach())
+
+    leaf = [p.to(device).requires_grad_() for p in (x, w, b, t)]
+    px, pw, pb, pt = leaf
+    lv = ids.to(device)
+    loss = (leaf_linear(px, lv, pw, pb) * leaf_embedding(lv, pt, scale=2.0) * c.to(device)).sum()
+    grads = torch.autograd.grad(loss, leaf)
+    base = [p.double() for p in (x, w, b, t)]
+    for k, (p, grad) in enumerate(zip(base, grads)):
+        for j in torch.randint(0, p.numel(), (12,), generator=g).tolist():
+            h = 1e-3
+            d = torch.zeros_like(p).view(-1)
+            d[j] = h
+            hi = [q + d.view(p.shape) if i == k else q for i, q in enumerate(base)]
+            lo = [q - d.view(p.shape) if i == k else q for i, q in enumerate(base)]
+            diff = (loss64(*hi) - loss64(*lo)) / (2 * h)
+            # the loss is linear in each operand; 32-bit terms of order 100 in sums of about 100
+            assert abs(diff - float(grad.flatten()[j])) < 1e-3 * (1 + abs(diff)), (k, j)
+
+
+# ---------------------------------------------------------------------------- refusals
+def test_refusals():
+    ids = torch.zeros(4, dtype=torch.int64)
+    t, w, x = torch.zeros(3, 5), torch.zeros(3, 2, 5), torch.zeros(4, 5)
+    r = leaf_route(ids, 3)
+    with pytest.raises(TypeError, match="int32 or int64"):
+        leaf_route(ids.float(), 3)
+    with pytest.raises(TypeError, match="LeafRoute"):
+        leaf_embedding([0, 1], t)
+    with pytest.raises(ValueError, match="n_leaves"):
+        leaf_route(ids, 0)
+    with pytest.raises(ValueError, match="n_leaves"):
+        leaf_embedding(ids, t[:0])
+    with pytest.raises(TypeError, match="float32, float16 or bfloat16"):
+        leaf_embedding(ids, t.double())
+    with pytest.raises(ValueError, match="dimensions"):
+        leaf_embedding(ids, t[0])
+    with pytest.raises(ValueError, match="width"):
+        leaf_embedding(ids, t[:, :0])
+    with pytest.raises(ValueError, match="finite"):
+        leaf_embedding(ids, t, scale=float("inf"))
+    with pytest.raises(ValueError, match="route"):
+        leaf_embedding(r, torch.zeros(4, 5))
+    with pytest.raises(ValueError, match="route"):
+        leaf_linear(x, r, torch.zeros(4, 2, 5))
+    with pytest.raises(TypeError, match="as the other operands"):
+        leaf_linear(x.half(), ids, w)
+    with pytest.raises(ValueError, match="inputs have shape"):
+        leaf_linear(x[:3], ids, w)
+    with pytest.raises(ValueError, match="inputs have shape"):
+        leaf_linear(torch.zeros(4, 6), ids, w)
+    with pytest.raises(ValueError, match="bias has shape"):
+        leaf_linear(x, ids, w, torch.zeros(3, 3))
+    with pytest.raises(ValueError, match="weight's columns"):
+        leaf_linear(torch.zeros(4, 0), ids, torch.zeros(3, 2, 0))
+    with pytest.raises(ValueError, match="different devices"):
+        leaf_embedding(ids, torch.zeros(3, 5, device="meta"))
+    p = t.clone().requires_grad_()
+    (grad,) = torch.autograd.grad(leaf_embedding(ids, p).square().sum(), p, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):  # first derivatives only
+        grad.sum().backward()
+
+
+def test_changed_leaves_are_noticed():
+    # leaf numbers rewritten between forward and backward would sum to the wrong leaves
+    ids, p = torch.zeros(4, dtype=torch.int64), torch.zeros(3, 5, requires_grad=True)
+    y = leaf_embedding(ids, p)
+    ids += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+# ---------------------------------------------------------------- through the estimators
+def fitted(seed=0, regression=False, depth=5, n=600):
+    rng = np.random.default_rng(seed)
+    X = rng.normal(size=(n, 6)).astype(np.float32)
+    y = X[:, 0] * 2 + X[:, 1] if regression else (X[:, 0] + X[:, 1] > 0).astype(int)
+    cls = DecisionTreeRegressor if regression else DecisionTreeClassifier
+    return cls(max_depth=depth, device="cpu").fit(X, y), X, y
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_estimator_leaf_numbers_follow_apply(device):
+    est, X, _ = fitted()
+    nodes = est.apply(X)
+    leaf_nodes = np.nonzero(est.tree_arrays_.feature < 0)[0]
+    want = np.searchsorted(leaf_nodes, nodes)
+    Xt = torch.from_numpy(X).to(device)
+    route = est.leaf_route(Xt)
+    assert isinstance(route, LeafRoute) and route.n_leaves == est.get_n_leaves()
+    assert np.array_equal(route.leaves.cpu().numpy(), want)
+    # the table of the leaves' class counts gives predict_proba back
+    counts = torch.from_numpy(est.tree_arrays_.count[leaf_nodes].astype(np.float32)).to(device)
+    assert np.array_equal(est.leaf_embedding(Xt, counts).cpu().numpy(), est.predict_proba(X))
+    assert np.array_equal(est.leaf_embedding(route, counts).cpu().numpy(), est.predict_proba(X))
+    if device == "cuda":  # host rows, device parameters
+        assert np.array_equal(est.leaf_embedding(X, counts).cpu().numpy(), est.predict_proba(X))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_estimator_leaf_model_trains(device):
+    # walk, look up, multiply and train as a leaf model does: its gradients are the formulas'
+    est, X, y = fitted(regression=True)
+    L, (n, F) = est.get_n_leaves(), X.shape
+    Xt = torch.from_numpy(X).to(device)
+    g = gen(9)
+    w0, b0, t0 = (torch.randn(L, 3, F, generator=g), torch.randn(L, 3, generator=g),
+                  torch.randn(L, 3, generator=g))
+    w, b, t = (p.to(device).requires_grad_() for p in (w0, b0, t0))
+    target = torch.from_numpy(y)
+    route = est.leaf_route(Xt)
+    out = (est.leaf_linear(route, w, b, inputs=Xt) * est.leaf_embedding(route, t, scale=0.5)).sum(1)
+    assert torch.equal(est.leaf_linear(Xt, w, b), est.leaf_linear(route, w, b, inputs=Xt))
+    loss = ((out - target.to(device)) ** 2).mean()
+    dw, db, dt = torch.autograd.grad(loss, (w, b, t))
+    q = route.leaves.cpu().long()
+    W, B, T = (p.double().requires_grad_() for p in (w0, b0, t0))
+    X64 = torch.from_numpy(X).double()
+    ref = (((W[q] * X64[:, None, :]).sum(2) + B[q]) * T[q] * 0.5).sum(1)
+    rloss = ((ref - target.double()) ** 2).mean()
+    assert abs(float(loss) - float(rloss)) < 1e-5 * (1 + float(rloss))
+    for got, want in zip((dw, db, dt), torch.autograd.grad(rloss, (W, B, T))):
+        # each gradient sums at most n terms of order 1 that are themselves 32-bit results
+        scale = float(want.abs().max())
+        assert float((got.cpu().double() - want).abs().max()) < 2e-5 * scale
+
+
+def test_estimator_refusals():
+    est, X, _ = fitted()
+    L = est.get_n_leaves()
+    with pytest.raises(ValueError, match="leaves"):
+        est.leaf_embedding(X, torch.zeros(L + 1, 2))
+    with pytest.raises(TypeError, match="tensor"):
+        est.leaf_linear(X, np.zeros((L, 2, 6)))
+    with pytest.raises(ValueError, match="features"):
+        est.leaf_embedding(X[:, :3], torch.zeros(L, 2))
+    with pytest.raises(ValueError, match="pass inputs"):
+        est.leaf_linear(est.leaf_route(X), torch.zeros(L, 2, 6))
+    with pytest.raises(Exception, match="not fitted"):
+        DecisionTreeClassifier().leaf_route(X)
+
+
+# ------------------------------------------------------------------- streams and graphs
+@pytest.mark.gpu
+def test_results_repeat_bit_for_bit():
+    g = gen(31)
+    n, G, D = 30_000, 11, 40
+    ids = draw_leaves(g, n, G, skew=1.0, none=0.05).cuda()
+    x, dy = torch.randn(n, D, generator=g).cuda().bfloat16(), torch.randn(n, 24, generator=g).cuda()
+    w = torch.randn(G, 24, D, generator=g).cuda().bfloat16().requires_grad_()
+    b = torch.randn(G, 24, generator=g).cuda().bfloat16().requires_grad_()
+    px = x.requires_grad_()
+    first = None
+    for _ in range(3):
+        y = leaf_linear(px, ids, w, b)
+        got = (y, *torch.autograd.grad(y, (px, w, b), dy.bfloat16()))
+        if first is None:
+            first = got
+        for a, c in zip(first, got):
+            assert torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_on_another_stream():
+    g = gen(41)
+    ids = draw_leaves(g, 20_000, 50).cuda()
+    t = torch.randn(50, 64, generator=g).cuda().requires_grad_()
+    w = torch.randn(50, 32, 64, generator=g).cuda().requires_grad_()
+    want = leaf_linear(leaf_embedding(ids, t), ids, w)
+    grads = torch.autograd.grad(want.sum(), (t, w))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = leaf_linear(leaf_embedding(ids, t), ids, w)
+        more = torch.autograd.grad(got.sum(), (t, w))
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip((want, *grads), (got, *more)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [48, 9000])
+def test_captured_and_replayed(n):
+    # two captured graphs and eager work between replays, each replay against the eager result
+    G, K, N = 12, 40, 24
+
+    def step(ids, x, w, b, t):
+        y = leaf_linear(x, ids, w, b) + leaf_embedding(ids, t, scale=0.5)
+        return (y.detach(), *torch.autograd.grad(y, (x, w, b, t), torch.ones_like(y)))
+
+    def make(seed):
+        h = gen(seed)
+        return [draw_leaves(h, n, G, none=0.1).cuda(),
+                *(p.cuda().requires_grad_() for p in (
+                    torch.randn(n, K, generator=h), torch.randn(G, N, K, generator=h),
+                    torch.randn(G, N, generator=h), torch.randn(G, N, generator=h)))]
+
+    graphs = []
+    for seed in (1, 2):
+        static = make(seed)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*static)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*static)
+        graphs.append((graph, static, out))
+    for k in range(4):
+        for q, (graph, static, out) in enumerate(graphs):
+            fresh = make(100 + 10 * k + q)
+            with torch.no_grad():
+                for a, b in zip(static, fresh):
+                    a.copy_(b)
+            graph.replay()
+            want = step(*fresh)
+            torch.cuda.synchronize()
+            for a, b in zip(out, want):
+                assert torch.equal(a, b), (k, q)
