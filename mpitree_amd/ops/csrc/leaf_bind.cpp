@@ -22,8 +22,9 @@ void launch_leaf_linear_small(hipStream_t, int, const void*, int64_t, const void
                               const void*, const void*, int, int, void*);
 void launch_leaf_linear_tile(hipStream_t, int, bool, const void*, int64_t, const int32_t*,
                              const int32_t*, int64_t, int, const void*, const void*, int, int,
-                             void*);
-int64_t leaf_linear_grad_bytes(int64_t, int, int);
+                             void*, void*);
+int64_t leaf_linear_tile_bytes(int64_t, int);
+int64_t leaf_linear_grad_bytes(int, int64_t, int, int, int);
 void launch_leaf_linear_grad(hipStream_t, int, const void*, int64_t, const void*, int64_t,
                              const int32_t*, const uint32_t*, const int32_t*, int64_t, int, int,
                              int, void*, void*);
@@ -64,10 +65,12 @@ void bind_leaf(py::module_& m) {
   });
   m.def("leaf_linear_tile", [](uintptr_t s, int type, bool dx, uintptr_t src, int64_t src_stride,
                                uintptr_t order, uintptr_t off, int64_t n, int G, uintptr_t w,
-                               uintptr_t bias, int K, int N, uintptr_t out) {
+                               uintptr_t bias, int K, int N, uintptr_t out, uintptr_t work) {
     launch_leaf_linear_tile(S(s), type, dx, P<void>(src), src_stride, P<int32_t>(order),
-                            P<int32_t>(off), n, G, P<void>(w), P<void>(bias), K, N, P<void>(out));
+                            P<int32_t>(off), n, G, P<void>(w), P<void>(bias), K, N, P<void>(out),
+                            P<void>(work));
   });
+  m.def("leaf_linear_tile_bytes", &leaf_linear_tile_bytes);
   m.def("leaf_linear_grad_bytes", &leaf_linear_grad_bytes);
   m.def("leaf_linear_grad", [](uintptr_t s, int type, uintptr_t x, int64_t x_stride, uintptr_t dy,
                                int64_t dy_stride, uintptr_t order, uintptr_t keys, uintptr_t off,

@@ -16,6 +16,7 @@ namespace mt {
 constexpr int kLlThreads = 256;
 constexpr int kLlWaves = kLlThreads / kWave;
 constexpr int kLlSmallRows = 64;
+constexpr int kLlBigRows = 512;  // rows a leaf on average from which on 256-row tiles are taken
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -91,60 +92,124 @@ __device__ __forceinline__ int ll_turn_chunk(int k, int c) {  // chunk c of row 
   return k * kRow + ll_turn_slab<T, COLS>(k, c / kPer) * kPer + c % kPer;
 }
 
+// What a lane adds to a fragment's address, once for all fragments: the swizzles depend on the lane
+// alone, so the rest of an address is an immediate (turned tiles: and the slab).
+template <typename T>
+struct LlLane {
+  int flat[2];  // chunk index inside 16 rows of a flat tile, by step
+  int turn_k;   // first depth row of a turned tile
+  int turn_c;   // element inside the slab
+  int turn_f;   // the slab's swizzle
+  __device__ __forceinline__ LlLane() {
+    const int l = lane_id();
+    flat[0] = ll_flat_chunk<T>(l & 15, l >> 4);
+    flat[1] = ll_flat_chunk<T>(l & 15, 4 + (l >> 4));
+    if constexpr (sizeof(T) == 4) {
+      turn_k = 4 * (l >> 4), turn_c = l & 15;
+    } else {
+      turn_k = 8 * (l >> 4) + ((l & 15) >> 2), turn_c = (l & 3) * 4;
+    }
+    turn_f = ll_turn_slab<T, 1024>(turn_k, 0);
+  }
+};
+
 // fragment (row r0 + l % 16, chunk 4 * step + l / 16) of a flat tile
 template <typename T>
-__device__ __forceinline__ uint4 ll_frag_flat(const uint4* s, int r0, int step) {
-  const int l = lane_id();
-  return s[ll_flat_chunk<T>(r0 + (l & 15), 4 * step + (l >> 4))];
+__device__ __forceinline__ uint4 ll_frag_flat(const uint4* s, const LlLane<T>& ln, int r0,
+                                              int step) {
+  return s[r0 * 8 + ln.flat[step]];
 }
 
-// the same fragment of a turned tile: column c0 + l % 16, depth (4 * step + l / 16) * kEpc on
+// the same fragment of a turned tile: column 16 slab + l % 16, depth (4 * step + l / 16) * kEpc on
 template <typename T, int COLS>
-__device__ __forceinline__ uint4 ll_frag_turn(const uint4* s, int c0, int step) {
-  const int l = lane_id();
+__device__ __forceinline__ uint4 ll_frag_turn(const uint4* s, const LlLane<T>& ln, int slab,
+                                              int step) {
+  const int at = ln.turn_k * COLS + ln.turn_c + (slab ^ (ln.turn_f & (COLS / 16 - 1))) * 16;
+  uint4 v;
   if constexpr (sizeof(T) == 4) {
-    const float* f = (const float*)s;
-    uint4 v;
+    const float* f = (const float*)s + at + 16 * step * COLS;
     uint32_t* e = (uint32_t*)&v;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int k = 16 * step + 4 * (l >> 4) + u;
-      e[u] = __float_as_uint(f[k * COLS + ll_turn_slab<T, COLS>(k, c0 >> 4) * 16 + (l & 15)]);
-    }
-    return v;
+    for (int u = 0; u < 4; ++u) e[u] = __float_as_uint(f[u * COLS]);
   } else {
     // ds_read_b64_tr_b16: 16 lanes read 4 rows of 16 columns, 8 bytes each, and lane i of them
     // gets column i of the 4 rows
-    const uint16_t* h = (const uint16_t*)s;
+    const uint16_t* h = (const uint16_t*)s + at + 32 * step * COLS;
     s16x4 part[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int k = 32 * step + 8 * (l >> 4) + 4 * u + ((l & 15) >> 2);
-      const uint16_t* p =
-          h + k * COLS + ll_turn_slab<T, COLS>(k, c0 >> 4) * 16 + (l & 3) * 4;
+    for (int u = 0; u < 2; ++u)
       part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4*)p);
-    }
-    uint4 v;
+          (__attribute__((address_space(3))) s16x4*)(h + 4 * u * COLS));
     __builtin_memcpy(&v, &part[0], 8);
     __builtin_memcpy((char*)&v + 8, &part[1], 8);
-    return v;
   }
+  return v;
 }
 
-// four neighbouring columns of one output row
-template <typename T>
-__device__ __forceinline__ void ll_store4(T* p, f32x4 v, int left, bool vec) {
-  if (vec && left >= 4) {
+// four neighbouring columns of one output row, `left` of them inside. kVec: rows are so aligned
+// that all four are inside, or none, and one store takes them.
+template <bool kVec, typename T>
+__device__ __forceinline__ void ll_store4(T* p, f32x4 v, int left) {
+  if constexpr (kVec) {
     LeafVec<T, 4> o;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o.v[e] = leaf_from<T>(v[e]);
-    *(LeafVec<T, 4>*)p = o;
+    if (left > 0) *(LeafVec<T, 4>*)p = o;
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (e < left) p[e] = leaf_from<T>(v[e]);
   }
+}
+
+// 16 bytes a lane from memory straight into LDS: lane l's chunk lands at lds[l] (lds: one address
+// for the wave).
+__device__ __forceinline__ void ll_dma(const void* g, void* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+// The same through a buffer descriptor, address = base + lane_off + off. In assembly, because the
+// compiler orders every later LDS read behind the builtin's writes: ll_dma_wait orders them.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i32x4 ll_rsrc(const void* base) {
+  const uint64_t p = (uint64_t)base;
+  return i32x4{(int)(uint32_t)p, (int)(uint32_t)(p >> 32), -1, 0x00027000};
+}
+__device__ __forceinline__ void ll_dma_buffer(i32x4 rsrc, uint32_t lane_off, uint32_t off,
+                                              const void* lds) {
+  const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+      :
+      : "s"(to), "v"(lane_off), "s"(rsrc), "s"(off)
+      : "memory", "m0");
+}
+// ... from any address of a lane
+__device__ __forceinline__ void ll_dma_at(const void* g, const void* lds) {
+  const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(to), "v"(g)
+               : "memory", "m0");
+}
+// every fetch of this wave has landed, and every wave has come here
+__device__ __forceinline__ void ll_dma_wait() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+// what the chunks behind the end of the depth are read from
+__device__ const uint4 kLlZeros[1] = {};
+
+// Blocks go to the 8 XCDs in turn, and each XCD has its own L2: runs of kLlXcdRun tiles stay on one
+// XCD, so that neighbours share the panels they read; runs go round, so that a stretch of tiles
+// without rows does not leave an XCD idle.
+constexpr int kLlXcds = 8, kLlXcdRun = 32;
+__device__ __forceinline__ int64_t ll_xcd_order(int64_t blk) {
+  const int64_t i = blk / kLlXcds;
+  return ((i / kLlXcdRun) * kLlXcds + blk % kLlXcds) * kLlXcdRun + i % kLlXcdRun;
+}
+static int64_t ll_xcd_blocks(int64_t tiles) {  // blocks that ll_xcd_order maps onto all tiles
+  constexpr int64_t kRound = kLlXcds * kLlXcdRun;
+  return (tiles + kRound - 1) / kRound * kRound;
 }
 
 struct LlTile {
@@ -157,138 +222,428 @@ struct LlTile {
   int64_t src_stride, w_stride;  // elements between src rows; between leaves' matrices
   int G, depth, cols, w_row;     // w_row: elements of a row of W (K)
   int col_tiles, bj_shift;
-  int64_t tiles;
+  int64_t tiles;              // a bound
+  const int2* plan;           // the tiles' leaves and positions, or null: found through off
+  const int32_t* plan_count;  // how many there are
 };
 
-// One tile of BJ rows of one leaf by BI output columns. Forward: A = W's rows, flat; kDx: A = W
-// with its rows as depth, turned. B = gathered rows of src, flat.
-template <typename T, bool kDx, int BJ, int BI, int WJ, bool kAligned>
-__global__ __launch_bounds__(kLlThreads) void ll_tile_kernel(LlTile a) {
-  constexpr int E = Ll<T>::kEpc, KD = Ll<T>::kDepth;
-  constexpr int WI = kLlWaves / WJ;
-  constexpr int SJ = BJ / WJ / 16, SI = BI / WI / 16;
-  constexpr int QJ = (BJ * 8 + kLlThreads - 1) / kLlThreads;
-  constexpr int QI = (BI * 8 + kLlThreads - 1) / kLlThreads;
-  static_assert(SJ >= 1 && SI >= 1, "a wave needs a subtile");
-  __shared__ uint4 s_j[BJ * 8], s_i[BI * 8];
-  const int64_t blk = leaf_block();
-  if (blk >= a.tiles) return;
-  const int tid = threadIdx.x, l = lane_id(), w = tid / kWave;
-  const int wj = w / WI * (SJ * 16), wi = w % WI * (SI * 16);
-  const int64_t slot = blk / a.col_tiles;
-  const int i0 = (int)(blk % a.col_tiles) * BI;
-  const int g = leaf_find_group(a.off, a.G + 1, a.bj_shift, slot);
-  const int64_t m0 = a.off[g] + ((slot - ((a.off[g] >> a.bj_shift) + (int64_t)g)) << a.bj_shift);
-  const int64_t m1 = a.off[g + 1];
-  if (m0 >= m1) return;
-  const int rows = (int)min<int64_t>(BJ, m1 - m0);
-  T* const out = (T*)a.out;
-  const bool vec = a.cols % 4 == 0 && (uintptr_t)a.out % (4 * sizeof(T)) == 0;
-
-  int32_t out_row[SJ];
-#pragma unroll
-  for (int j = 0; j < SJ; ++j) {
-    const int r = wj + j * 16 + (l & 15);
-    out_row[j] = r < rows ? a.order[m0 + r] : -1;
+// The tiles of kBig rows in order of their leaves, {leaf, first sorted position}, and how many there
+// are: with many column tiles, tiles without rows between them would keep neighbours from
+// sharing what they read. One workgroup; a leaf has at least 512 rows on average here.
+constexpr int kLlPlanThreads = 1024;
+__global__ __launch_bounds__(kLlPlanThreads) void ll_plan_kernel(const int32_t* __restrict__ off,
+                                                                 int G, int bj_shift,
+                                                                 int2* __restrict__ plan,
+                                                                 int32_t* __restrict__ count) {
+  __shared__ uint32_t s_w[kLlPlanThreads / kWave];
+  const int w = threadIdx.x / kWave, lane = lane_id();
+  uint32_t before = 0;
+  for (int g0 = 0; g0 <= G; g0 += kLlPlanThreads) {
+    const int g = g0 + threadIdx.x;
+    const int a = g <= G ? off[g] : 0, b = g <= G ? off[g + 1] : 0;
+    const uint32_t mine = (uint32_t)(((int64_t)b - a + (1 << bj_shift) - 1) >> bj_shift);
+    const uint32_t incl = wave_incl_scan_u32(mine);
+    if (lane == kWave - 1) s_w[w] = incl;
+    __syncthreads();
+    uint32_t at = before, all = 0;
+    for (int q = 0; q < kLlPlanThreads / kWave; ++q) {
+      at += q < w ? s_w[q] : 0u;
+      all += s_w[q];
+    }
+    at += incl - mine;
+    for (uint32_t k = 0; k < mine; ++k) plan[at + k] = make_int2(g, a + (int)(k << bj_shift));
+    before += all;
+    __syncthreads();
   }
+  if (threadIdx.x == 0) *count = (int32_t)before;
+}
+
+// which rows and columns a tile is
+struct LlPlace {
+  int g, i0, rows;  // leaf (G: the rows without one), first column, rows (<= 0: no such tile)
+  int64_t m0;       // first sorted position
+};
+__device__ __forceinline__ LlPlace ll_place(const LlTile& a, int64_t blk, int bi) {
+  // bands of 8 column tiles: neighbours share rows of src and panels of W alike
+  LlPlace at;
+  at.rows = 0;
+  const int64_t slots = a.plan != nullptr ? *a.plan_count : a.tiles / a.col_tiles;
+  const int band = (int)(blk / (slots * 8));
+  const int wide = min(8, a.col_tiles - band * 8);
+  if (wide <= 0) return at;
+  const int64_t in_band = blk - (int64_t)band * slots * 8;
+  const int64_t slot = in_band / wide;
+  at.i0 = (band * 8 + (int)(in_band % wide)) * bi;
+  if (a.plan != nullptr) {
+    const int2 p = a.plan[slot];
+    at.g = p.x, at.m0 = p.y;
+  } else {
+    at.g = leaf_find_group(a.off, a.G + 1, a.bj_shift, slot);
+    const int64_t first = a.off[at.g];
+    at.m0 = first + ((slot - ((first >> a.bj_shift) + (int64_t)at.g)) << a.bj_shift);
+  }
+  at.rows = (int)max<int64_t>(-1, min<int64_t>(1 << a.bj_shift, a.off[at.g + 1] - at.m0));
+  return at;
+}
+
+// acc[j][i] holds row kStep j + l % 16 and columns 16 i + 4 (l / 16) .. + 3 of the wave's part
+template <typename T, int SJ, int SI>
+__device__ __forceinline__ void ll_add_bias(f32x4 (&acc)[SJ][SI], const LlTile& a, int g, int c0) {
+  if (a.bias == nullptr) return;
+  const T* const bg = (const T*)a.bias + (int64_t)g * a.cols;
+#pragma unroll
+  for (int i = 0; i < SI; ++i) {
+    const int c = c0 + i * 16 + 4 * (lane_id() >> 4);
+    f32x4 b = {};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < a.cols) b[e] = leaf_f32(bg[c + e]);
+#pragma unroll
+    for (int j = 0; j < SJ; ++j) acc[j][i] += b;
+  }
+}
+
+template <typename T, int kStep, int SJ, int SI>
+__device__ __forceinline__ void ll_store_rows(const f32x4 (&acc)[SJ][SI], const LlTile& a,
+                                              const LlPlace& at, int wj, int wi) {
+  const int l = lane_id();
+  auto store = [&](auto kvec) {
+#pragma unroll
+    for (int j = 0; j < SJ; ++j) {
+      const int r = wj + j * kStep + (l & 15);
+      if (r >= at.rows) continue;
+      T* const o = (T*)a.out + (int64_t)a.order[at.m0 + r] * a.cols;
+#pragma unroll
+      for (int i = 0; i < SI; ++i) {
+        const int c = at.i0 + wi + i * 16 + 4 * (l >> 4);
+        ll_store4<kvec()>(o + c, acc[j][i], a.cols - c);
+      }
+    }
+  };
+  const bool vec = a.cols % 4 == 0 && (uintptr_t)a.out % (4 * sizeof(T)) == 0;
+  vec ? store(std::true_type{}) : store(std::false_type{});
+}
+
+// One tile of BJ rows of one leaf by BI output columns, NW waves, WJ of them along the rows.
+// Forward: A = W's rows, flat; kDx: A = W with its rows as depth, turned. B = gathered rows of src,
+// flat. Rows past the leaf's last and columns past the last repeat the last one: their products
+// are not stored. Depth past the end is zeros in both operands.
+//
+// kAligned: the next tile of depth goes from memory straight into the LDS buffer that is not read;
+// one barrier a tile. Otherwise chunks go through registers, whose loads wait until the tile's
+// products are issued.
+template <typename T, bool kDx, int BJ, int BI, int WJ, int NW, bool kAligned>
+__global__ __launch_bounds__(NW* kWave) void ll_tile_kernel(LlTile a) {
+  constexpr int E = Ll<T>::kEpc, KD = Ll<T>::kDepth, NT = NW * kWave;
+  constexpr int WI = NW / WJ;
+  constexpr int SJ = BJ / WJ / 16, SI = BI / WI / 16;
+  constexpr int QJ = (BJ * 8 + NT - 1) / NT;
+  constexpr int QI = (BI * 8 + NT - 1) / NT;
+  static_assert(SJ >= 1 && SI >= 1, "a wave needs a subtile");
+  __shared__ uint4 s_j0[BJ * 8], s_i0[BI * 8];
+  __shared__ uint4 s_j1[kAligned ? BJ * 8 : 1], s_i1[kAligned ? BI * 8 : 1];
+  const int64_t blk = ll_xcd_order(leaf_block());
+  if (blk >= a.tiles) return;
+  const int tid = threadIdx.x, l = lane_id(), w = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int wj = w / WI * (SJ * 16), wi = w % WI * (SI * 16);
+  const LlPlace at = ll_place(a, blk, BI);
+  if (at.rows <= 0) return;
+  const int rows = at.rows, i0 = at.i0, g = at.g;
   f32x4 acc[SJ][SI] = {};
+  const LlLane<T> ln;
   if (g < a.G) {
     const T* const src = (const T*)a.src;
     const T* const wg = (const T*)a.w + (int64_t)g * a.w_stride;
     const T* jp[QJ];
 #pragma unroll
     for (int q = 0; q < QJ; ++q) {
-      const int r = (q * kLlThreads + tid) >> 3;
-      jp[q] = r < rows ? src + (int64_t)a.order[m0 + r] * a.src_stride : nullptr;
+      const int r = (q * NT + tid) >> 3;
+      jp[q] = src + (int64_t)a.order[at.m0 + min(r, rows - 1)] * a.src_stride;
     }
-    uint4 vj[QJ], vi[QI];
-    auto load = [&](int k0) {
-#pragma unroll
-      for (int q = 0; q < QJ; ++q) {
-        const int id = q * kLlThreads + tid, r = id >> 3;
-        const int k = k0 + ((id & 7) ^ (r & 7)) * E;
-        vj[q] = ll_chunk<T, kAligned>(jp[q] + k, jp[q] != nullptr ? a.depth - k : 0);
-      }
-#pragma unroll
-      for (int q = 0; q < QI; ++q) {
-        const int id = q * kLlThreads + tid;
-        if constexpr (!kDx) {
-          const int r = id >> 3;
-          const int k = k0 + ((id & 7) ^ (r & 7)) * E;
-          const bool in = BI * 8 % kLlThreads == 0 || r < BI;
-          vi[q] = ll_chunk<T, kAligned>(wg + (int64_t)(i0 + r) * a.w_row + k,
-                                        in && i0 + r < a.cols ? a.depth - k : 0);
-        } else {
-          constexpr int kRow = BI / E;
-          const int k = id / kRow, c = id % kRow;
-          const bool in = BI * 8 % kLlThreads == 0 || k < KD;
-          vi[q] = ll_chunk<T, kAligned>(wg + (int64_t)(k0 + k) * a.w_row + i0 + c * E,
-                                        in && k0 + k < a.depth ? a.cols - i0 - c * E : 0);
-        }
-      }
-    };
-    load(0);
-    for (int k0 = 0; k0 < a.depth; k0 += KD) {
-#pragma unroll
-      for (int q = 0; q < QJ; ++q) {
-        const int id = q * kLlThreads + tid;
-        if (BJ * 8 % kLlThreads == 0 || id < BJ * 8) s_j[id] = vj[q];
-      }
-#pragma unroll
-      for (int q = 0; q < QI; ++q) {
-        const int id = q * kLlThreads + tid;
-        if (BI * 8 % kLlThreads == 0 || id < BI * 8) {
-          if constexpr (!kDx)
-            s_i[id] = vi[q];
-          else
-            s_i[ll_turn_chunk<T, BI>(id / (BI / E), id % (BI / E))] = vi[q];
-        }
-      }
-      __syncthreads();
-      if (k0 + KD < a.depth) load(k0 + KD);
+    auto products = [&](const uint4* sj, const uint4* si) {
+      if (wj >= rows) return;
 #pragma unroll
       for (int step = 0; step < 2; ++step) {
         uint4 fj[SJ], fi[SI];
 #pragma unroll
-        for (int j = 0; j < SJ; ++j) fj[j] = ll_frag_flat<T>(s_j, wj + j * 16, step);
+        for (int j = 0; j < SJ; ++j) fj[j] = ll_frag_flat<T>(sj, ln, wj + j * 16, step);
 #pragma unroll
         for (int i = 0; i < SI; ++i) {
           if constexpr (!kDx)
-            fi[i] = ll_frag_flat<T>(s_i, wi + i * 16, step);
+            fi[i] = ll_frag_flat<T>(si, ln, wi + i * 16, step);
           else
-            fi[i] = ll_frag_turn<T, BI>(s_i, wi + i * 16, step);
+            fi[i] = ll_frag_turn<T, BI>(si, ln, wi / 16 + i, step);
         }
 #pragma unroll
         for (int j = 0; j < SJ; ++j)
 #pragma unroll
           for (int i = 0; i < SI; ++i) acc[j][i] = ll_mma<T>(fi[i], fj[j], acc[j][i]);
       }
-      __syncthreads();
-    }
-    if (a.bias != nullptr) {
-      const T* const bg = (const T*)a.bias + (int64_t)g * a.cols;
+    };
+    if constexpr (kAligned) {
+      auto load = [&](uint4* sj, uint4* si, int k0) {
 #pragma unroll
-      for (int i = 0; i < SI; ++i) {
-        const int c = i0 + wi + i * 16 + 4 * (l >> 4);
-        f32x4 b = {};
+        for (int q = 0; q < QJ; ++q) {
+          const int id = q * NT + tid, r = id >> 3;
+          if (BJ * 8 % NT != 0 && q * NT + w * kWave >= BJ * 8) break;
+          const int k = k0 + ((id & 7) ^ (r & 7)) * E;
+          const void* p = jp[q] + k;
+          if (k >= a.depth) p = kLlZeros;
+          ll_dma(p, sj + q * NT + w * kWave);
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (c + e < a.cols) b[e] = leaf_f32(bg[c + e]);
+        for (int q = 0; q < QI; ++q) {
+          const int id = q * NT + tid;
+          if (BI * 8 % NT != 0 && q * NT + w * kWave >= BI * 8) break;
+          const void* p;
+          if constexpr (!kDx) {
+            const int r = id >> 3;
+            const int k = k0 + ((id & 7) ^ (r & 7)) * E;
+            p = wg + (int64_t)min(i0 + r, a.cols - 1) * a.w_row + k;
+            if (k >= a.depth) p = kLlZeros;
+          } else {
+            constexpr int kRow = BI / E;
+            const int k = id / kRow;
+            const int c = ll_turn_chunk<T, BI>(k, id % kRow) - k * kRow;
+            p = wg + (int64_t)(k0 + k) * a.w_row + min(i0 + c * E, a.cols - E);
+            if (k0 + k >= a.depth) p = kLlZeros;
+          }
+          ll_dma(p, si + q * NT + w * kWave);
+        }
+      };
+      load(s_j0, s_i0, 0);
+      for (int k0 = 0; k0 < a.depth; k0 += 2 * KD) {
+        __syncthreads();
+        if (k0 + KD < a.depth) load(s_j1, s_i1, k0 + KD);
+        products(s_j0, s_i0);
+        if (k0 + KD >= a.depth) break;
+        __syncthreads();
+        if (k0 + 2 * KD < a.depth) load(s_j0, s_i0, k0 + 2 * KD);
+        products(s_j1, s_i1);
+      }
+    } else {
+      uint4 vj[QJ], vi[QI];
+      auto load = [&](int k0) {
 #pragma unroll
-        for (int j = 0; j < SJ; ++j) acc[j][i] += b;
+        for (int q = 0; q < QJ; ++q) {
+          const int id = q * NT + tid, r = id >> 3;
+          const int k = k0 + ((id & 7) ^ (r & 7)) * E;
+          vj[q] = ll_chunk<T, false>(jp[q] + k, a.depth - k);
+        }
+#pragma unroll
+        for (int q = 0; q < QI; ++q) {
+          const int id = q * NT + tid;
+          if constexpr (!kDx) {
+            const int r = id >> 3;
+            const int k = k0 + ((id & 7) ^ (r & 7)) * E;
+            vi[q] = ll_chunk<T, false>(wg + (int64_t)min(i0 + r, a.cols - 1) * a.w_row + k,
+                                       a.depth - k);
+          } else {
+            constexpr int kRow = BI / E;
+            const int k = id / kRow, c = id % kRow;
+            const bool in = BI * 8 % NT == 0 || k < KD;
+            vi[q] = ll_chunk<T, false>(wg + (int64_t)(k0 + k) * a.w_row + i0 + c * E,
+                                       in && k0 + k < a.depth ? a.cols - i0 - c * E : 0);
+          }
+        }
+      };
+      load(0);
+      for (int k0 = 0; k0 < a.depth; k0 += KD) {
+#pragma unroll
+        for (int q = 0; q < QJ; ++q) {
+          const int id = q * NT + tid;
+          if (BJ * 8 % NT == 0 || id < BJ * 8) s_j0[id] = vj[q];
+        }
+#pragma unroll
+        for (int q = 0; q < QI; ++q) {
+          const int id = q * NT + tid;
+          if (BI * 8 % NT == 0 || id < BI * 8) {
+            if constexpr (!kDx)
+              s_i0[id] = vi[q];
+            else
+              s_i0[ll_turn_chunk<T, BI>(id / (BI / E), id % (BI / E))] = vi[q];
+          }
+        }
+        __syncthreads();
+        if (k0 + KD < a.depth) load(k0 + KD);
+        products(s_j0, s_i0);
+        __syncthreads();
       }
     }
+    ll_add_bias<T, SJ, SI>(acc, a, g, i0 + wi);
   }
+  ll_store_rows<T, 16, SJ, SI>(acc, a, at, wj, wi);
+}
+
+// ---- 256 x 256 tiles of 16-bit types, where rows and columns fill them: 8 waves of 128 x 64.
+//
+// A tile of depth is multiplied in two halves. While one half is multiplied, the other's
+// fragments are read -- past the barrier, those of the next tile -- each row fragment into the
+// registers that the products have just left. The tile after next is fetched into the buffer that
+// has been read: it has one tile's products to arrive. Operands are fetched through buffer
+// descriptors: a lane's 32-bit offset is fixed and the depth is a scalar, so a fetch costs no
+// vector arithmetic; an operand has to lie within 4 GiB for that.
+// (Behind the last tile the same happens with zeros, which nothing uses.)
+//
+// A turned operand's depth rows lie in pairs, kPair bytes apart: 512 bytes a row and 32 to spare,
+// and the odd row's slabs lie at s ^ 2. So the four rows that 16 lanes read at once, and those of the
+// next 16 lanes, are in different banks, and a fragment's address is one of two lane constants
+// plus an immediate.
+constexpr int kBig = 256, kBigWaves = 8, kBigThreads = kBigWaves * kWave;
+constexpr int kBigPair = 2 * 512 + 32;
+constexpr int kBigFlatBytes = kBig * 128, kBigTurnBytes = 32 * kBigPair;
+constexpr int kBigQ = kBig * 8 / kBigThreads;  // fetches of a thread per operand and tile
+
+struct LlBigLane {
+  int e[2];  // by the slab's bit 1
+  __device__ __forceinline__ LlBigLane() {
+    const int l = lane_id(), k = 8 * (l >> 4) + ((l & 15) >> 2), odd = k & 1;
+    const int at = (k >> 1) * kBigPair + odd * 512 + (l & 3) * 8;
+    e[0] = at + odd * 64, e[1] = at - odd * 64;
+  }
+};
+// slab0: a multiple of 4, the same for the wave
+__device__ __forceinline__ uint4 ll_big_turn(const char* s, const LlBigLane& ln, int slab0, int i,
+                                             int step) {
+  s16x4 part[2];
 #pragma unroll
-  for (int j = 0; j < SJ; ++j) {
-    if (out_row[j] < 0) continue;
-    T* const o = out + (int64_t)out_row[j] * a.cols;
+  for (int u = 0; u < 2; ++u)
+    part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(s + ln.e[(i >> 1) & 1] + slab0 * 32 + i * 32 +
+                                                   (16 * step + 2 * u) * kBigPair));
+  uint4 v;
+  __builtin_memcpy(&v, &part[0], 8);
+  __builtin_memcpy((char*)&v + 8, &part[1], 8);
+  return v;
+}
+// where fetch q of this wave lands, and which depth row (0..63) and column chunk this lane brings
+__device__ __forceinline__ int ll_big_turn_to(int w, int q) {
+  return (q * kBigWaves + w) * kBigPair;
+}
+__device__ __forceinline__ int ll_big_turn_row(int w, int q) {
+  return 2 * (q * kBigWaves + w) + (lane_id() >> 5);
+}
+__device__ __forceinline__ int ll_big_turn_col() {
+  const int l = lane_id();
+  return (l & 31) ^ ((l >> 5) * 4);
+}
+
+template <typename T, bool kDx>
+__global__ __launch_bounds__(kBigThreads, 2) void ll_big_kernel(LlTile a) {
+  constexpr int E = Ll<T>::kEpc, KD = Ll<T>::kDepth;
+  constexpr int SJ = 8, SI = 4;
+  static_assert(sizeof(T) == 2, "the buffers' layout is for 16-bit types");
+  constexpr int kBytes = kBigFlatBytes + (kDx ? kBigTurnBytes : kBigFlatBytes);
+  __shared__ alignas(16) char s0[kBytes], s1[kBytes];  // rows, then columns
+  const int64_t blk = ll_xcd_order(leaf_block());
+  if (blk >= a.tiles) return;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave);
+  // rows of 16 go to the two halves of the waves in turn, so that a tile with fewer rows costs less
+  const int wj = w / 4 * 16, wi = w % 4 * (SI * 16);
+  const LlPlace at = ll_place(a, blk, kBig);
+  if (at.rows <= 0) return;
+  const int rows = at.rows, i0 = at.i0;
+  f32x4 acc[SJ][SI] = {};
+  if (at.g < a.G) {
+    const LlLane<T> ln;
+    const LlBigLane lt;
+    const T* const src = (const T*)a.src;
+    const T* const wg = (const T*)a.w + (int64_t)at.g * a.w_stride;
+    const i32x4 src_rsrc = ll_rsrc(src), w_rsrc = ll_rsrc(wg);
+    const int kc = ((tid & 7) ^ ((tid >> 3) & 7)) * E;  // a flat chunk's place in the depth
+    uint32_t jo[kBigQ], wo[kBigQ];
 #pragma unroll
-    for (int i = 0; i < SI; ++i) {
-      const int c = i0 + wi + i * 16 + 4 * (l >> 4);
-      ll_store4<T>(o + c, acc[j][i], a.cols - c, vec);
+    for (int q = 0; q < kBigQ; ++q) {
+      const int r = (q * kBigThreads + tid) >> 3;
+      jo[q] = (uint32_t)(a.order[at.m0 + min(r, rows - 1)] * a.src_stride + kc) * sizeof(T);
+      if constexpr (!kDx)
+        wo[q] = ((uint32_t)min(i0 + r, a.cols - 1) * a.w_row + kc) * sizeof(T);
+      else
+        wo[q] = ((uint32_t)ll_big_turn_row(w, q) * a.w_row +
+                 min(i0 + ll_big_turn_col() * E, a.cols - E)) * sizeof(T);
     }
+    // tail: the tile may reach past the depth
+    auto load = [&](auto tail, char* s, int k0) {
+      const uint32_t ko = (uint32_t)k0 * sizeof(T);
+      const uint32_t kw = kDx ? ko * a.w_row : ko;
+#pragma unroll
+      for (int q = 0; q < kBigQ; ++q) {
+        char* const to = s + (q * kBigThreads + w * kWave) * 16;
+        if constexpr (!tail())
+          ll_dma_buffer(src_rsrc, jo[q], ko, to);
+        else
+          ll_dma_at(k0 + kc < a.depth ? (const char*)src + jo[q] + ko : (const char*)kLlZeros, to);
+      }
+#pragma unroll
+      for (int q = 0; q < kBigQ; ++q) {
+        char* const to = s + kBigFlatBytes +
+                         (kDx ? ll_big_turn_to(w, q) : (q * kBigThreads + w * kWave) * 16);
+        const int k = kDx ? ll_big_turn_row(w, q) : kc;
+        if constexpr (!tail())
+          ll_dma_buffer(w_rsrc, wo[q], kw, to);
+        else
+          ll_dma_at(k0 + k < a.depth ? (const char*)wg + wo[q] + kw : (const char*)kLlZeros, to);
+      }
+    };
+    uint4 fj[SJ], fi0[SI], fi1[SI];
+    auto read_j = [&](const char* s, int j, int step) {
+      return ll_frag_flat<T>((const uint4*)s, ln, wj + j * 32, step);
+    };
+    auto read_i = [&](uint4 (&fi)[SI], const char* s, int step) {
+#pragma unroll
+      for (int i = 0; i < SI; ++i) {
+        if constexpr (!kDx)
+          fi[i] = ll_frag_flat<T>((const uint4*)(s + kBigFlatBytes), ln, wi + i * 16, step);
+        else
+          fi[i] = ll_big_turn(s + kBigFlatBytes, lt, wi / 16, i, step);
+      }
+    };
+    const int nj = (rows - wj + 31) / 32;  // subtiles of this wave that hold rows (<= 0: none)
+    // all: nj == SJ
+    auto half = [&](auto all, const uint4 (&fi)[SI], uint4 (&fn)[SI], const char* next, int step) {
+      read_i(fn, next, step);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < SJ; ++j) {
+        if (all() || j < nj) {
+          __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+          for (int i = 0; i < SI; ++i) acc[j][i] = ll_mma<T>(fi[i], fj[j], acc[j][i]);
+          __builtin_amdgcn_s_setprio(0);
+          fj[j] = read_j(next, j, step);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto pair = [&](auto all, auto tail, int k0) {
+      half(all, fi0, fi1, s0, 1);
+      ll_dma_wait();
+      load(tail, s0, k0 + 2 * KD);
+      half(all, fi1, fi0, s1, 0);
+      half(all, fi0, fi1, s1, 1);
+      ll_dma_wait();
+      load(tail, s1, k0 + 3 * KD);
+      half(all, fi1, fi0, s0, 0);
+    };
+    constexpr std::true_type kYes{};
+    constexpr std::false_type kNo{};
+    load(kYes, s0, 0);
+    ll_dma_wait();
+    load(kYes, s1, KD);
+#pragma unroll
+    for (int j = 0; j < SJ; ++j) fj[j] = read_j(s0, j, 0);
+    read_i(fi0, s0, 0);
+    int k0 = 0;
+    if (nj == SJ) {
+      for (; k0 + 4 * KD <= a.depth; k0 += 2 * KD) pair(kYes, kNo, k0);
+    } else {
+      for (; k0 + 4 * KD <= a.depth; k0 += 2 * KD) pair(kNo, kNo, k0);
+    }
+    for (; k0 < a.depth; k0 += 2 * KD) pair(kNo, kYes, k0);
+    ll_dma_wait();  // (the fetches behind the last tile, before the workgroup's LDS goes)
+    ll_add_bias<T, SJ, SI>(acc, a, at.g, i0 + wi);
   }
+  ll_store_rows<T, 32, SJ, SI>(acc, a, at, wj, wi);
 }
 
 // ---- dW. A unit is a leaf with at most `run` rows (units below G), or a leaf's piece of a chunk of
@@ -305,6 +660,53 @@ struct LlGrad {
   int G, N, K, k_tiles, n_tiles;
   int64_t run, units;
 };
+
+// sorted positions [pa, pb) of a unit; false: there is no such unit
+__device__ __forceinline__ bool ll_grad_rows(const LlGrad& a, int64_t unit, int64_t& pa,
+                                             int64_t& pb) {
+  if (unit < a.G) {
+    pa = a.off[unit], pb = a.off[unit + 1];
+    return pb - pa <= a.run;
+  }
+  const int64_t c = (unit - a.G) >> 1, m = a.off[a.G];
+  const int64_t ca = c * a.run, cb = min<int64_t>(ca + a.run, m);
+  if (ca >= m) return false;
+  const int64_t k0 = a.keys[ca], k1 = a.keys[cb - 1];
+  if (((unit - a.G) & 1) == 0) {
+    pa = ca, pb = min<int64_t>(cb, a.off[k0 + 1]);
+    return a.off[k0 + 1] - a.off[k0] > a.run;
+  }
+  pa = a.off[k1], pb = cb;
+  return k1 != k0 && a.off[k1 + 1] - a.off[k1] > a.run;
+}
+
+// acc[j][i] holds row 16 j + l % 16 and columns 16 i + 4 (l / 16) .. + 3 from (r0, c0) on
+template <typename T, int SJ, int SI>
+__device__ __forceinline__ void ll_grad_store(const f32x4 (&acc)[SJ][SI], const LlGrad& a,
+                                              int64_t unit, int r0, int c0) {
+  const int l = lane_id();
+  auto store = [&](auto kvec, auto* to) {
+#pragma unroll
+    for (int j = 0; j < SJ; ++j) {
+      const int r = r0 + j * 16 + (l & 15);
+      if (r >= a.N) continue;
+#pragma unroll
+      for (int i = 0; i < SI; ++i) {
+        const int c = c0 + i * 16 + 4 * (l >> 4);
+        ll_store4<kvec()>(to + (int64_t)r * a.K + c, acc[j][i], a.K - c);
+      }
+    }
+  };
+  const bool vec = a.K % 4 == 0 && (uintptr_t)a.dw % (4 * sizeof(T)) == 0;
+  const int64_t size = (int64_t)a.N * a.K;
+  if (unit < a.G) {
+    T* const to = (T*)a.dw + unit * size;
+    vec ? store(std::true_type{}, to) : store(std::false_type{}, to);
+  } else {
+    float* const to = a.part + (unit - a.G) * size;
+    vec ? store(std::true_type{}, to) : store(std::false_type{}, to);
+  }
+}
 
 // One BJ x BI tile (rows of W, columns of W) of one unit: both operands are gathered rows with the
 // rows as depth, turned.
@@ -326,24 +728,10 @@ __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
   const int wj = w / WI * (SJ * 16), wi = w % WI * (SI * 16);
 
   int64_t pa, pb;
-  if (unit < a.G) {
-    pa = a.off[unit], pb = a.off[unit + 1];
-    if (pb - pa > a.run) return;
-  } else {
-    const int64_t c = (unit - a.G) >> 1, m = a.off[a.G];
-    const int64_t ca = c * a.run, cb = min<int64_t>(ca + a.run, m);
-    if (ca >= m) return;
-    const int64_t k0 = a.keys[ca], k1 = a.keys[cb - 1];
-    if (((unit - a.G) & 1) == 0) {
-      if (a.off[k0 + 1] - a.off[k0] <= a.run) return;
-      pa = ca, pb = min<int64_t>(cb, a.off[k0 + 1]);
-    } else {
-      if (k1 == k0 || a.off[k1 + 1] - a.off[k1] <= a.run) return;
-      pa = a.off[k1], pb = cb;
-    }
-  }
+  if (!ll_grad_rows(a, unit, pa, pb)) return;
 
   f32x4 acc[SJ][SI] = {};
+  const LlLane<T> ln;
   const T* const x = (const T*)a.x;
   const T* const dy = (const T*)a.dy;
   uint4 vj[QJ], vi[QI];
@@ -386,9 +774,9 @@ __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
     for (int step = 0; step < 2; ++step) {
       uint4 fj[SJ], fi[SI];
 #pragma unroll
-      for (int j = 0; j < SJ; ++j) fj[j] = ll_frag_turn<T, BJ>(s_j, wj + j * 16, step);
+      for (int j = 0; j < SJ; ++j) fj[j] = ll_frag_turn<T, BJ>(s_j, ln, wj / 16 + j, step);
 #pragma unroll
-      for (int i = 0; i < SI; ++i) fi[i] = ll_frag_turn<T, BI>(s_i, wi + i * 16, step);
+      for (int i = 0; i < SI; ++i) fi[i] = ll_frag_turn<T, BI>(s_i, ln, wi / 16 + i, step);
 #pragma unroll
       for (int j = 0; j < SJ; ++j)
 #pragma unroll
@@ -397,22 +785,108 @@ __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
     __syncthreads();
   }
 
-  const bool whole = unit < a.G;
-  const bool vec = a.K % 4 == 0 && (uintptr_t)a.dw % (4 * sizeof(T)) == 0;
+  ll_grad_store<T, SJ, SI>(acc, a, unit, j0 + wj, i0 + wi);
+}
+
+// The same on 256 x 256 tiles of 16-bit types (see ll_big_kernel): both operands turned.
+template <typename T>
+__global__ __launch_bounds__(kBigThreads, 2) void ll_big_grad_kernel(LlGrad a) {
+  constexpr int E = Ll<T>::kEpc, KD = Ll<T>::kDepth;
+  constexpr int SJ = 8, SI = 4;
+  static_assert(sizeof(T) == 2, "the buffers' layout is for 16-bit types");
+  __shared__ alignas(16) char s0[2 * kBigTurnBytes], s1[2 * kBigTurnBytes];  // dy, then x
+  const int64_t blk = ll_xcd_order(leaf_block());
+  const int tiles = a.n_tiles * a.k_tiles;
+  const int64_t unit = blk / tiles;
+  if (unit >= a.units) return;
+  const int t = (int)(blk % tiles);
+  const int j0 = t / a.k_tiles * kBig, i0 = t % a.k_tiles * kBig;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wj = w / 4 * (SJ * 16), wi = w % 4 * (SI * 16);
+  int64_t pa, pb;
+  if (!ll_grad_rows(a, unit, pa, pb)) return;
+  const int rows = (int)(pb - pa);
+  const int32_t* const order = a.order + pa;
+
+  f32x4 acc[SJ][SI] = {};
+  if (rows > 0) {
+    const LlBigLane lt;
+    const i32x4 dy_rsrc = ll_rsrc(a.dy), x_rsrc = ll_rsrc(a.x);
+    const uint32_t jc = (uint32_t)min(j0 + ll_big_turn_col() * E, a.N - E) * sizeof(T);
+    const uint32_t ic = (uint32_t)min(i0 + ll_big_turn_col() * E, a.K - E) * sizeof(T);
+    const uint32_t js = (uint32_t)a.dy_stride * sizeof(T), is = (uint32_t)a.x_stride * sizeof(T);
+    int32_t row[kBigQ];  // of the next tile to fetch
+    auto next_rows = [&](int p0) {
 #pragma unroll
-  for (int j = 0; j < SJ; ++j) {
-    const int r = j0 + wj + j * 16 + (l & 15);
-    if (r >= a.N) continue;
+      for (int q = 0; q < kBigQ; ++q) row[q] = order[min(p0 + ll_big_turn_row(w, q), rows - 1)];
+    };
+    // tail: the tile may reach past the rows
+    auto load = [&](auto tail, char* s, int p0) {
+      // the row numbers have arrived with the barrier; told here, the compiler waits for none of
+      // them between the fetches, where it would wait for the fetches too
+      static_assert(kBigQ == 4, "");
+      asm volatile("" : "+v"(row[0]), "+v"(row[1]), "+v"(row[2]), "+v"(row[3]));
 #pragma unroll
-    for (int i = 0; i < SI; ++i) {
-      const int c = i0 + wi + i * 16 + 4 * (l >> 4);
-      if (whole)
-        ll_store4<T>((T*)a.dw + ((int64_t)unit * a.N + r) * a.K + c, acc[j][i], a.K - c, vec);
-      else
-        ll_store4<float>(a.part + ((unit - a.G) * a.N + r) * a.K + c, acc[j][i], a.K - c,
-                         a.K % 4 == 0);
-    }
+      for (int q = 0; q < kBigQ; ++q) {
+        char* const to = s + ll_big_turn_to(w, q);
+        const uint32_t jo = (uint32_t)row[q] * js + jc, io = (uint32_t)row[q] * is + ic;
+        if constexpr (!tail()) {
+          ll_dma_buffer(dy_rsrc, jo, 0, to);
+          ll_dma_buffer(x_rsrc, io, 0, to + kBigTurnBytes);
+        } else {
+          const bool in = p0 + ll_big_turn_row(w, q) < rows;
+          ll_dma_at(in ? (const char*)a.dy + jo : (const char*)kLlZeros, to);
+          ll_dma_at(in ? (const char*)a.x + io : (const char*)kLlZeros, to + kBigTurnBytes);
+        }
+      }
+      next_rows(p0 + KD);
+    };
+    uint4 fj[SJ], fi0[SI], fi1[SI];
+    auto read_j = [&](const char* s, int j, int step) {
+      return ll_big_turn(s, lt, wj / 16, j, step);
+    };
+    auto read_i = [&](uint4 (&fi)[SI], const char* s, int step) {
+#pragma unroll
+      for (int i = 0; i < SI; ++i) fi[i] = ll_big_turn(s + kBigTurnBytes, lt, wi / 16, i, step);
+    };
+    auto half = [&](const uint4 (&fi)[SI], uint4 (&fn)[SI], const char* next, int step) {
+      read_i(fn, next, step);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < SJ; ++j) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < SI; ++i) acc[j][i] = ll_mma<T>(fi[i], fj[j], acc[j][i]);
+        __builtin_amdgcn_s_setprio(0);
+        fj[j] = read_j(next, j, step);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto pair = [&](auto tail, int p0) {
+      half(fi0, fi1, s0, 1);
+      ll_dma_wait();
+      load(tail, s0, p0 + 2 * KD);
+      half(fi1, fi0, s1, 0);
+      half(fi0, fi1, s1, 1);
+      ll_dma_wait();
+      load(tail, s1, p0 + 3 * KD);
+      half(fi1, fi0, s0, 0);
+    };
+    constexpr std::true_type kYes{};
+    constexpr std::false_type kNo{};
+    next_rows(0);
+    load(kYes, s0, 0);
+    ll_dma_wait();
+    load(kYes, s1, KD);
+#pragma unroll
+    for (int j = 0; j < SJ; ++j) fj[j] = read_j(s0, j, 0);
+    read_i(fi0, s0, 0);
+    int p0 = 0;
+    for (; p0 + 4 * KD <= rows; p0 += 2 * KD) pair(kNo, p0);
+    for (; p0 < rows; p0 += 2 * KD) pair(kYes, p0);
+    ll_dma_wait();  // (the fetches behind the last tile, before the workgroup's LDS goes)
   }
+  ll_grad_store<T, SJ, SI>(acc, a, unit, j0 + wj, i0 + wi);
 }
 
 // Adds the partial matrices of the leaves with more than `run` rows: one block per chunk in which
@@ -510,7 +984,8 @@ __global__ __launch_bounds__(kLlThreads) void ll_small_kernel(LlSmall a) {
       if (c + e < a.N) acc[e] += leaf_f32(bg[c + e]);
   }
   const bool vec = a.N % 4 == 0 && (uintptr_t)a.y % (4 * sizeof(T)) == 0;
-  ll_store4<T>(y + (int64_t)row * a.N + c, acc, a.N - c, vec);
+  T* const to = y + (int64_t)row * a.N + c;
+  vec ? ll_store4<true>(to, acc, a.N - c) : ll_store4<false>(to, acc, a.N - c);
 }
 
 // ---------------------------------------------------------------------------- launches
@@ -523,6 +998,9 @@ static bool ll_aligned(std::initializer_list<const void*> ptrs,
     if (s % Ll<T>::kEpc) return false;
   return true;
 }
+
+template <int N>
+using LlInt = std::integral_constant<int, N>;
 
 template <typename F>
 static void ll_dispatch_type(int type, F f) {
@@ -554,10 +1032,16 @@ void launch_leaf_linear_small(hipStream_t s, int type, const void* x, int64_t x_
   });
 }
 
+// scratch for the tile list
+int64_t leaf_linear_tile_bytes(int64_t n, int G) {
+  return n / G >= kLlBigRows ? 8 + 8 * ((n >> 8) + G + 1) : 0;
+}
+
 // forward (dx false: src = x, depth = K, cols = N) or dx (src = dy, depth = N, cols = K)
 void launch_leaf_linear_tile(hipStream_t s, int type, bool dx, const void* src, int64_t src_stride,
                              const int32_t* order, const int32_t* off, int64_t n, int G,
-                             const void* w, const void* bias, int K, int N, void* out) {
+                             const void* w, const void* bias, int K, int N, void* out,
+                             void* work) {
   if (n <= 0) return;
   LlTile a{};
   a.src = src, a.w = w, a.bias = bias, a.out = out, a.order = order, a.off = off;
@@ -566,57 +1050,84 @@ void launch_leaf_linear_tile(hipStream_t s, int type, bool dx, const void* src, 
   ll_dispatch_type(type, [&](auto t) {
     using T = decltype(t);
     const bool al = ll_aligned<T>({src, w}, {K, src_stride, dx ? N : K});
-    auto go = [&](auto bj, auto bi, auto wj) {
+    auto go = [&](auto bj, auto bi, auto wj, auto nw) {
       a.bj_shift = __builtin_ctz((unsigned)bj());
       a.col_tiles = (a.cols + bi() - 1) / bi();
       a.tiles = ((n >> a.bj_shift) + G + 1) * a.col_tiles;
-      const dim3 grid = leaf_grid(a.tiles);
+      const dim3 grid = leaf_grid(ll_xcd_blocks(a.tiles));
       auto run = [&](auto kern) {
-        hipLaunchKernelGGL(kern, grid, dim3(kLlThreads), 0, s, a);
+        hipLaunchKernelGGL(kern, grid, dim3(nw() * kWave), 0, s, a);
         MT_HIP_CHECK(hipGetLastError());
       };
       if (dx)
-        al ? run(ll_tile_kernel<T, true, bj(), bi(), wj(), true>)
-           : run(ll_tile_kernel<T, true, bj(), bi(), wj(), false>);
+        al ? run(ll_tile_kernel<T, true, bj(), bi(), wj(), nw(), true>)
+           : run(ll_tile_kernel<T, true, bj(), bi(), wj(), nw(), false>);
       else
-        al ? run(ll_tile_kernel<T, false, bj(), bi(), wj(), true>)
-           : run(ll_tile_kernel<T, false, bj(), bi(), wj(), false>);
+        al ? run(ll_tile_kernel<T, false, bj(), bi(), wj(), nw(), true>)
+           : run(ll_tile_kernel<T, false, bj(), bi(), wj(), nw(), false>);
     };
-    using std::integral_constant;
-    using c1 = integral_constant<int, 1>;
-    using c2 = integral_constant<int, 2>;
-    using c4 = integral_constant<int, 4>;
-    using c16 = integral_constant<int, 16>;
-    using c64 = integral_constant<int, 64>;
-    using c128 = integral_constant<int, 128>;
     const int64_t mean = n / G;
+    const bool big = sizeof(T) == 2 && al && mean >= kLlBigRows &&
+                     (n >> 8) * ((a.cols + kBig - 1) / kBig) >= 512 &&
+                     n * src_stride * (int64_t)sizeof(T) < (1ll << 32) &&
+                     a.w_stride * (int64_t)sizeof(T) < (1ll << 32);
     if (a.cols <= 16)
-      go(c64{}, c16{}, c4{});
+      go(LlInt<64>{}, LlInt<16>{}, LlInt<4>{}, LlInt<4>{});
     else if (mean < 32)
-      go(c16{}, c64{}, c1{});
+      go(LlInt<16>{}, LlInt<64>{}, LlInt<1>{}, LlInt<4>{});
     else if (mean < 128 || a.cols <= 64)
-      go(c64{}, c64{}, c2{});
-    else
-      go(c128{}, c128{}, c2{});
+      go(LlInt<64>{}, LlInt<64>{}, LlInt<2>{}, LlInt<4>{});
+    else if (!big)
+      go(LlInt<128>{}, LlInt<128>{}, LlInt<2>{}, LlInt<4>{});
+    else if constexpr (sizeof(T) == 2) {
+      a.bj_shift = 8;
+      a.col_tiles = (a.cols + kBig - 1) / kBig;
+      a.tiles = ((n >> 8) + G + 1) * a.col_tiles;
+      auto run = [&](auto kern) {
+        hipLaunchKernelGGL(kern, leaf_grid(ll_xcd_blocks(a.tiles)), dim3(kBigThreads), 0, s,
+                           a);
+        MT_HIP_CHECK(hipGetLastError());
+      };
+      int2* const plan = (int2*)((int32_t*)work + 2);
+      a.plan = plan, a.plan_count = (const int32_t*)work;
+      hipLaunchKernelGGL(ll_plan_kernel, dim3(1), dim3(kLlPlanThreads), 0, s, off, G, a.bj_shift,
+                         plan, (int32_t*)work);
+      MT_HIP_CHECK(hipGetLastError());
+      dx ? run(ll_big_kernel<T, true>) : run(ll_big_kernel<T, false>);
+    }
   });
 }
 
-// rows a dW unit may have: a power of two, small enough that about 1024 tiles run at once
-static int64_t ll_grad_run(int64_t n, int64_t tiles) {
+// Rows a dW unit may have, a power of two: so many that about 1024 to 2048 tiles run at once, and
+// where whole leaves are that many already, four times the mean leaf, so that only leaves far above
+// it are cut (a cut costs a partial matrix in 32 bits, written and read).
+static int64_t ll_grad_run(int64_t n, int G, int64_t tiles) {
   int64_t run = 256;
   while (run < (1 << 20) && n / run * tiles > 2048) run <<= 1;
+  if (G * tiles >= 1024)
+    while (run < 4 * (n / G)) run <<= 1;
   return run;
 }
-static int ll_grad_tile(int N, int K) { return N > 64 && K > 64 ? 128 : 64; }
-static int64_t ll_grad_tiles(int N, int K) {
-  const int b = ll_grad_tile(N, K);
+// tile edge of dW; direct: operands are 16-byte aligned and lie within 4 GiB
+static int ll_grad_tile(int type, bool direct, int64_t n, int G, int K, int N) {
+  const int64_t big = (int64_t)((N + kBig - 1) / kBig) * ((K + kBig - 1) / kBig);
+  if (type != kLeafF32 && direct && N > 128 && K > 128 && n / G >= 256 && big * G >= 256)
+    return kBig;
+  return N > 64 && K > 64 ? 128 : 64;
+}
+static int64_t ll_grad_tiles(int b, int K, int N) {
   return (int64_t)((N + b - 1) / b) * ((K + b - 1) / b);
 }
 
-int64_t leaf_linear_grad_bytes(int64_t n, int K, int N) {
-  const int64_t run = ll_grad_run(n, ll_grad_tiles(N, K));
-  if (n <= run) return 0;
-  return 2 * ((n + run - 1) / run) * (int64_t)N * K * 4;
+// scratch for the partial matrices, whichever tile is taken
+int64_t leaf_linear_grad_bytes(int type, int64_t n, int G, int K, int N) {
+  int64_t chunks = 0;
+  for (bool direct : {false, true}) {
+    const int b = ll_grad_tile(type, direct, n, G, K, N);
+    const int64_t run = ll_grad_run(n, G, ll_grad_tiles(b, K, N));
+    if (n > run) chunks = std::max(chunks, (n + run - 1) / run);
+  }
+  return 2 * chunks * (int64_t)N * K * 4;
 }
 
 void launch_leaf_linear_grad(hipStream_t s, int type, const void* x, int64_t x_stride,
@@ -628,26 +1139,32 @@ void launch_leaf_linear_grad(hipStream_t s, int type, const void* x, int64_t x_s
   a.order = order, a.keys = keys, a.off = off;
   a.x_stride = x_stride, a.dy_stride = dy_stride;
   a.G = G, a.N = N, a.K = K;
-  const int64_t tiles = ll_grad_tiles(N, K);
-  a.run = ll_grad_run(n, tiles);
+  const int64_t elem = type == kLeafF32 ? 4 : 2;
+  const bool al = (elem == 4 ? ll_aligned<float> : ll_aligned<f16_t>)(
+      {x, dy}, {K, N, x_stride, dy_stride});
+  const bool direct = al && n * std::max(x_stride, dy_stride) * elem < (1ll << 32);
+  const int b = ll_grad_tile(type, direct, n, G, K, N);
+  const int64_t tiles = ll_grad_tiles(b, K, N);
+  a.n_tiles = (N + b - 1) / b, a.k_tiles = (K + b - 1) / b;
+  a.run = ll_grad_run(n, G, tiles);
   const int64_t chunks = n > a.run ? (n + a.run - 1) / a.run : 0;
   a.units = G + 2 * chunks;
   ll_dispatch_type(type, [&](auto t) {
     using T = decltype(t);
-    const bool al = ll_aligned<T>({x, dy}, {K, N, x_stride, dy_stride});
-    auto go = [&](auto b) {
-      a.n_tiles = (N + b() - 1) / b(), a.k_tiles = (K + b() - 1) / b();
-      const dim3 grid = leaf_grid(a.units * tiles);
-      auto run = [&](auto kern) {
-        hipLaunchKernelGGL(kern, grid, dim3(kLlThreads), 0, s, a);
-        MT_HIP_CHECK(hipGetLastError());
-      };
-      al ? run(ll_grad_kernel<T, b(), b(), 2, true>) : run(ll_grad_kernel<T, b(), b(), 2, false>);
+    auto run = [&](auto kern, int64_t blocks, int threads) {
+      hipLaunchKernelGGL(kern, leaf_grid(blocks), dim3(threads), 0, s, a);
+      MT_HIP_CHECK(hipGetLastError());
     };
-    if (ll_grad_tile(N, K) == 128)
-      go(std::integral_constant<int, 128>{});
-    else
-      go(std::integral_constant<int, 64>{});
+    const int64_t all = a.units * tiles;
+    if (b == kBig) {
+      if constexpr (sizeof(T) == 2) run(ll_big_grad_kernel<T>, ll_xcd_blocks(all), kBigThreads);
+    } else if (b == 128) {
+      al ? run(ll_grad_kernel<T, 128, 128, 2, true>, all, kLlThreads)
+         : run(ll_grad_kernel<T, 128, 128, 2, false>, all, kLlThreads);
+    } else {
+      al ? run(ll_grad_kernel<T, 64, 64, 2, true>, all, kLlThreads)
+         : run(ll_grad_kernel<T, 64, 64, 2, false>, all, kLlThreads);
+    }
     if (chunks > 0) {
       const int64_t per = ((int64_t)N * K + kLlThreads - 1) / kLlThreads;
       hipLaunchKernelGGL(ll_join_kernel<T>, leaf_grid(chunks * per), dim3(kLlThreads), 0, s, a, per,

@@ -233,11 +233,13 @@ def _linear_plain_grad(dy, x, route, w, need_x, need_w):
 
 def _linear_tile(dx: bool, src, route, w, bias) -> torch.Tensor:
     G, N, K = w.shape
-    out = torch.empty((src.shape[0], K if dx else N), dtype=src.dtype, device=src.device)
-    native.hip().leaf_linear_tile(
+    hip, n = native.hip(), src.shape[0]
+    out = torch.empty((n, K if dx else N), dtype=src.dtype, device=src.device)
+    work = torch.empty(hip.leaf_linear_tile_bytes(n, G), dtype=torch.uint8, device=src.device)
+    hip.leaf_linear_tile(
         _stream(src), _TYPES[src.dtype], dx, src.data_ptr(), src.stride(0),
-        route.order.data_ptr(), route.offsets.data_ptr(), src.shape[0], G, w.data_ptr(),
-        0 if bias is None else bias.data_ptr(), K, N, out.data_ptr())
+        route.order.data_ptr(), route.offsets.data_ptr(), n, G, w.data_ptr(),
+        0 if bias is None else bias.data_ptr(), K, N, out.data_ptr(), work.data_ptr())
     return out
 
 
@@ -264,7 +266,8 @@ def _linear_grad_weight(dy, x, route, w) -> torch.Tensor:
     G, N, K = w.shape
     hip, n = native.hip(), x.shape[0]
     dw = torch.empty((G, N, K), dtype=x.dtype, device=x.device)
-    work = torch.empty(hip.leaf_linear_grad_bytes(n, K, N), dtype=torch.uint8, device=x.device)
+    work = torch.empty(hip.leaf_linear_grad_bytes(_TYPES[x.dtype], n, G, K, N), dtype=torch.uint8,
+                       device=x.device)
     hip.leaf_linear_grad(_stream(x), _TYPES[x.dtype], x.data_ptr(), x.stride(0), dy.data_ptr(),
                          dy.stride(0), route.order.data_ptr(), route.keys.data_ptr(),
                          route.offsets.data_ptr(), n, G, K, N, dw.data_ptr(), work.data_ptr())

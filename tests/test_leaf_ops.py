@@ -238,6 +238,40 @@ def test_linear_long_leaves(dtype, skew):
     linear_case("cuda", 40_000, 9, 24, 20, dtype, bias=True, skew=skew, none=0.05)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,G,K,N,skew", [(33_000, 21, 1032, 1048, 0.0),
+                                          (33_000, 23, 1048, 1032, 1.0),
+                                          (20_000, 300, 136, 520, 0.0), (66_000, 5, 520, 776, 0.5)])
+def test_linear_large(dtype, n, G, K, N, skew):
+    # rows and columns that fill the largest tiles, with ends inside them; the sums in 64 bits and
+    # their absolute sums are computed on the device, leaf by leaf
+    g = gen(n + G)
+    ids = draw_leaves(g, n, G, skew, 0.02).cuda()
+    x = torch.randn(n, K, generator=g).to(dtype).cuda()
+    w = (torch.randn(G, N, K, generator=g) * K ** -0.5).to(dtype).cuda()
+    b = torch.randn(G, N, generator=g).to(dtype).cuda()
+    dy = torch.randn(n, N, generator=g).to(dtype).cuda()
+    for p in (x, w, b):
+        p.requires_grad_()
+    y = leaf_linear(x, ids, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    none = (ids < 0) | (ids >= G)
+    assert not y[none].any() and not dx[none].any()
+    for q in range(G):
+        r = torch.nonzero(ids == q).flatten()
+        X, W, D = x.detach()[r].double(), w.detach()[q].double(), dy[r].double()
+        B = b.detach()[q].double()
+        Xa, Wa, Da = X.abs(), W.abs(), D.abs()
+        for got, want, mass, terms, what in (
+                (y.detach()[r], X @ W.t().contiguous() + B,
+                 Xa @ Wa.t().contiguous() + B.abs(), K + 1, "y"),
+                (dx[r], D @ W, Da @ Wa, N, "dx"),
+                (dw[q], D.t().contiguous() @ X, Da.t().contiguous() @ Xa, len(r), "dw"),
+                (db[q], D.sum(0), Da.sum(0), len(r), "db")):
+            check(got, want.cpu(), mass.cpu(), terms, (what, q))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_linear_all_rows_without_a_leaf(device):
     for n in (5, 500):
