@@ -273,6 +273,7 @@ __device__ __forceinline__ LlPlace ll_place(const LlTile& a, int64_t blk, int bi
   if (wide <= 0) return at;
   const int64_t in_band = blk - (int64_t)band * slots * 8;
   const int64_t slot = in_band / wide;
+  if (slot >= slots) return at;  // (the list may be shorter than the bound that was launched)
   at.i0 = (band * 8 + (int)(in_band % wide)) * bi;
   if (a.plan != nullptr) {
     const int2 p = a.plan[slot];
