@@ -3,6 +3,8 @@
 
 #include <pybind11/pybind11.h>
 
+#include <algorithm>
+
 #include "common.h"
 
 namespace py = pybind11;
@@ -15,7 +17,7 @@ void launch_leaf_route(hipStream_t, const void*, bool, int64_t, int, int32_t*, u
 void launch_leaf_embed(hipStream_t, int, const void*, bool, const void*, int64_t, int64_t, int64_t,
                        int, float, void*);
 int64_t leaf_embed_grad_bytes(int, int64_t, int);
-void launch_leaf_embed_grad(hipStream_t, int, const void*, const int32_t*, const uint32_t*,
+void launch_leaf_embed_grad(hipStream_t, int, const void*, int64_t, const int32_t*, const uint32_t*,
                             const int32_t*, int64_t, int64_t, int, float, void*, void*);
 int leaf_linear_small_rows();
 void launch_leaf_linear_small(hipStream_t, int, const void*, int64_t, const void*, bool, int, int,
@@ -37,24 +39,48 @@ T* P(uintptr_t p) {
 }
 }  // namespace
 
+// A route in one int32 buffer: order [n], keys [n], offsets [G + 2].
+struct Route {
+  int32_t* order;
+  uint32_t* keys;
+  int32_t* off;
+  Route(uintptr_t buf, int64_t n)
+      : order(P<int32_t>(buf)), keys(P<uint32_t>(buf) + n), off(P<int32_t>(buf) + 2 * n) {}
+};
+int64_t route_len(int64_t n, int64_t G) { return 2 * n + G + 2; }
+int64_t pad16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
 void bind_leaf(py::module_& m) {
-  m.def("leaf_route_words", &leaf_route_words);
-  m.def("leaf_route", [](uintptr_t s, uintptr_t ids, bool wide, int64_t n, int G, uintptr_t order,
-                         uintptr_t keys, uintptr_t off, uintptr_t work) {
-    launch_leaf_route(S(s), P<void>(ids), wide, n, G, P<int32_t>(order), P<uint32_t>(keys),
-                      P<int32_t>(off), P<uint32_t>(work));
+  m.def("leaf_route_len", &route_len);      // int32 words of a route
+  m.def("leaf_route_words", &leaf_route_words);  // ... of the scratch of its sort
+  m.def("leaf_route", [](uintptr_t s, uintptr_t ids, bool wide, int64_t n, int G, uintptr_t buf,
+                         uintptr_t work) {
+    const Route r(buf, n);
+    launch_leaf_route(S(s), P<void>(ids), wide, n, G, r.order, r.keys, r.off, P<uint32_t>(work));
   });
   m.def("leaf_embed", [](uintptr_t s, int type, uintptr_t ids, bool wide, uintptr_t table,
                          int64_t stride, int64_t n, int64_t V, int D, float scale, uintptr_t y) {
     launch_leaf_embed(S(s), type, P<void>(ids), wide, P<void>(table), stride, n, V, D, scale,
                       P<void>(y));
   });
-  m.def("leaf_embed_grad_bytes", &leaf_embed_grad_bytes);
-  m.def("leaf_embed_grad", [](uintptr_t s, int type, uintptr_t dy, uintptr_t order, uintptr_t keys,
-                              uintptr_t off, int64_t n, int64_t V, int D, float scale,
+  // the sums of dy by leaf; ids: they are sorted first, into `work`; else `route` holds the sort
+  m.def("leaf_embed_grad_bytes", [](int type, int64_t n, int G, int D, bool routed) {
+    return leaf_embed_grad_bytes(type, n, D) +
+           (routed ? 0 : pad16(4 * leaf_route_words(n, G)) + pad16(4 * route_len(n, G)));
+  });
+  m.def("leaf_embed_grad", [](uintptr_t s, int type, uintptr_t dy, int64_t dy_stride, uintptr_t ids,
+                              bool wide, uintptr_t route, int64_t n, int G, int D, float scale,
                               uintptr_t dtable, uintptr_t work) {
-    launch_leaf_embed_grad(S(s), type, P<void>(dy), P<int32_t>(order), P<uint32_t>(keys),
-                           P<int32_t>(off), n, V, D, scale, P<void>(dtable), P<void>(work));
+    if (route == 0) {
+      route = work + pad16(4 * leaf_route_words(n, G));
+      const Route r(route, n);
+      launch_leaf_route(S(s), P<void>(ids), wide, n, G, r.order, r.keys, r.off,
+                        P<uint32_t>(work));
+      work = route + pad16(4 * route_len(n, G));
+    }
+    const Route r(route, n);
+    launch_leaf_embed_grad(S(s), type, P<void>(dy), dy_stride, r.order, r.keys, r.off, n, G, D,
+                           scale, P<void>(dtable), P<void>(work));
   });
   m.def("leaf_linear_small_rows", &leaf_linear_small_rows);
   m.def("leaf_linear_small", [](uintptr_t s, int type, uintptr_t x, int64_t x_stride, uintptr_t ids,
@@ -63,21 +89,39 @@ void bind_leaf(py::module_& m) {
     launch_leaf_linear_small(S(s), type, P<void>(x), x_stride, P<void>(ids), wide, n, G,
                              P<void>(w), P<void>(bias), K, N, P<void>(y));
   });
-  m.def("leaf_linear_tile", [](uintptr_t s, int type, bool dx, uintptr_t src, int64_t src_stride,
-                               uintptr_t order, uintptr_t off, int64_t n, int G, uintptr_t w,
-                               uintptr_t bias, int K, int N, uintptr_t out, uintptr_t work) {
-    launch_leaf_linear_tile(S(s), type, dx, P<void>(src), src_stride, P<int32_t>(order),
-                            P<int32_t>(off), n, G, P<void>(w), P<void>(bias), K, N, P<void>(out),
-                            P<void>(work));
+  // ids != 0: the rows are sorted into `route` first; else it holds the sort
+  m.def("leaf_linear_bytes", [](int64_t n, int G) {
+    return std::max(4 * leaf_route_words(n, G), leaf_linear_tile_bytes(n, G));
   });
-  m.def("leaf_linear_tile_bytes", &leaf_linear_tile_bytes);
-  m.def("leaf_linear_grad_bytes", &leaf_linear_grad_bytes);
+  m.def("leaf_linear", [](uintptr_t s, int type, uintptr_t x, int64_t x_stride, uintptr_t ids,
+                          bool wide, uintptr_t route, int64_t n, int G, uintptr_t w, uintptr_t bias,
+                          int K, int N, uintptr_t y, uintptr_t work) {
+    const Route r(route, n);
+    if (ids != 0)
+      launch_leaf_route(S(s), P<void>(ids), wide, n, G, r.order, r.keys, r.off,
+                        P<uint32_t>(work));
+    launch_leaf_linear_tile(S(s), type, false, P<void>(x), x_stride, r.order, r.off, n, G,
+                            P<void>(w), P<void>(bias), K, N, P<void>(y), P<void>(work));
+  });
+  // dx, dw and db, each where its address is not 0; one scratch, used by one after the other
+  m.def("leaf_linear_grad_bytes", [](int type, int64_t n, int G, int K, int N) {
+    return std::max({leaf_linear_tile_bytes(n, G), leaf_linear_grad_bytes(type, n, G, K, N),
+                     leaf_embed_grad_bytes(type, n, N)});
+  });
   m.def("leaf_linear_grad", [](uintptr_t s, int type, uintptr_t x, int64_t x_stride, uintptr_t dy,
-                               int64_t dy_stride, uintptr_t order, uintptr_t keys, uintptr_t off,
-                               int64_t n, int G, int K, int N, uintptr_t dw, uintptr_t work) {
-    launch_leaf_linear_grad(S(s), type, P<void>(x), x_stride, P<void>(dy), dy_stride,
-                            P<int32_t>(order), P<uint32_t>(keys), P<int32_t>(off), n, G, K, N,
-                            P<void>(dw), P<void>(work));
+                               int64_t dy_stride, uintptr_t route, int64_t n, int G, uintptr_t w,
+                               int K, int N, uintptr_t dx, uintptr_t dw, uintptr_t db,
+                               uintptr_t work) {
+    const Route r(route, n);
+    if (dx != 0)
+      launch_leaf_linear_tile(S(s), type, true, P<void>(dy), dy_stride, r.order, r.off, n, G,
+                              P<void>(w), nullptr, K, N, P<void>(dx), P<void>(work));
+    if (dw != 0)
+      launch_leaf_linear_grad(S(s), type, P<void>(x), x_stride, P<void>(dy), dy_stride, r.order,
+                              r.keys, r.off, n, G, K, N, P<void>(dw), P<void>(work));
+    if (db != 0)
+      launch_leaf_embed_grad(S(s), type, P<void>(dy), dy_stride, r.order, r.keys, r.off, n, G, N, 1.f,
+                             P<void>(db), P<void>(work));
   });
 }
 

@@ -5,11 +5,11 @@
 //
 // Gradient: dtable[v] = scale * sum of dy over the rows of leaf v, for every v (zeros where no row
 // is). The rows are sorted by leaf first (leaf_route.hip), so a leaf's rows are a run of `order`,
-// and every sum has one fixed order: the result does not depend on the launch. A leaf with at most
-// kLeRun rows is summed by one group of lanes. A leaf with more is cut at the multiples of kLeRun
-// of the sorted positions: each piece is summed by one workgroup into a partial row, and a second
-// launch adds a leaf's partial rows. A chunk of kLeRun positions meets at most two such leaves
-// (one that reaches into it, one that reaches out of it), so two partial rows a chunk suffice.
+// and every sum has one fixed order: the result does not depend on the launch. The sorted
+// positions are cut into chunks, one for a group of lanes, which streams its chunk's rows (their
+// numbers are known at once, so a batch of rows is in flight) and writes out a sum where the leaf
+// changes. A leaf that reaches over a chunk's end leaves partial rows there, at most two a chunk,
+// and a second launch adds a leaf's partial rows. Leaves without rows are found through the offsets.
 //
 // Sums are held in 32 bits for 16-bit types and in 64 bits for f32: a leaf may hold most of a
 // million rows, and a 64-bit add costs no more than a 32-bit one here, where memory is the bound.
@@ -18,8 +18,9 @@
 namespace mt {
 
 constexpr int kLeThreads = 256;
-constexpr int kLeRun = 64;
-constexpr int kLeUnroll = 4;
+constexpr int kLeUnroll = 4;  // rows of a group in flight: forward,
+constexpr int kLeBatch = 8;   // and gradient
+constexpr int kLeEmpty = 16;  // leaves that a group looks over for missing rows
 
 template <typename T>
 struct LeAcc {
@@ -76,158 +77,138 @@ __global__ __launch_bounds__(kLeThreads) void le_forward_kernel(
   }
 }
 
-// acc += dy[order[p]] for p = a, a + step, ... below b; the columns of one lane
-template <typename T, int W, int NC, typename A>
-__device__ __forceinline__ void le_sum_rows(const T* __restrict__ dy, int D, int c0, int tpr,
-                                            const int32_t* __restrict__ order, int64_t a, int64_t b,
-                                            int step, A (&acc)[NC][W]) {
-  for (int64_t p = a; p < b; p += (int64_t)step * kLeUnroll) {
-    int32_t row[kLeUnroll];
-#pragma unroll
-    for (int u = 0; u < kLeUnroll; ++u) {
-      const int64_t pu = p + (int64_t)u * step;
-      row[u] = pu < b ? order[pu] : -1;
-    }
-#pragma unroll
-    for (int q = 0; q < NC; ++q) {
-      const int c = c0 + q * tpr * W;
-      if (c >= D) break;
-      LeafVec<T, W> v[kLeUnroll];
-#pragma unroll
-      for (int u = 0; u < kLeUnroll; ++u) {
-        v[u] = LeafVec<T, W>{};
-        if (row[u] >= 0) v[u] = *(const LeafVec<T, W>*)(dy + (int64_t)row[u] * D + c);
-      }
-#pragma unroll
-      for (int u = 0; u < kLeUnroll; ++u)
-#pragma unroll
-        for (int e = 0; e < W; ++e) acc[q][e] += (A)leaf_f32(v[u].v[e]);
-    }
-  }
-}
-
 // the sums of the block's row groups, added in their order; group 0's lanes hold the result
-template <int W, int NC, typename A>
-__device__ __forceinline__ void le_block_sum(A (&acc)[NC][W], int tpr_shift, A* s_acc) {
+template <int W, typename A>
+__device__ __forceinline__ void le_block_sum(A (&acc)[W], int tpr_shift, A* s_acc) {
   const int tpr = 1 << tpr_shift, rpb = kLeThreads >> tpr_shift;
   const int sub = threadIdx.x >> tpr_shift, lr = threadIdx.x & (tpr - 1);
   // pairwise: groups [half, 2 half) hand theirs to groups [0, half)
   for (int half = rpb >> 1; half > 0; half >>= 1) {
     if (sub >= half && sub < 2 * half) {
 #pragma unroll
-      for (int q = 0; q < NC; ++q)
-#pragma unroll
-        for (int e = 0; e < W; ++e)
-          s_acc[((q * W + e) * half + (sub - half)) * tpr + lr] = acc[q][e];
+      for (int e = 0; e < W; ++e) s_acc[(e * half + (sub - half)) * tpr + lr] = acc[e];
     }
     __syncthreads();
     if (sub < half) {
 #pragma unroll
-      for (int q = 0; q < NC; ++q)
-#pragma unroll
-        for (int e = 0; e < W; ++e) acc[q][e] += s_acc[((q * W + e) * half + sub) * tpr + lr];
+      for (int e = 0; e < W; ++e) acc[e] += s_acc[(e * half + sub) * tpr + lr];
     }
     __syncthreads();
   }
 }
 
-template <typename T, int W, int NC, typename A>
-__device__ __forceinline__ void le_store(T* __restrict__ out, int D, int c0, int tpr, float scale,
-                                         const A (&acc)[NC][W]) {
+template <typename T, int W, typename A>
+__device__ __forceinline__ void le_store(T* __restrict__ out, float scale, const A (&acc)[W]) {
+  LeafVec<T, W> v;
 #pragma unroll
-  for (int q = 0; q < NC; ++q) {
-    const int c = c0 + q * tpr * W;
-    if (c >= D) break;
-    LeafVec<T, W> v;
-#pragma unroll
-    for (int e = 0; e < W; ++e) v.v[e] = leaf_from<T>((float)(acc[q][e] * (A)scale));
-    *(LeafVec<T, W>*)(out + c) = v;
-  }
+  for (int e = 0; e < W; ++e) v.v[e] = leaf_from<T>((float)(acc[e] * (A)scale));
+  *(LeafVec<T, W>*)out = v;
 }
 
-// Blocks below `light`: the leaves with at most kLeRun rows. Blocks from there on: chunk pieces of
-// the leaves with more, into `part` ([2 * chunks][D]).
-template <typename T, int W, int NC>
+// Blocks below `chunk_blocks`: a chunk of 1 << run_shift sorted positions for each group of lanes,
+// partial rows into `part` ([2 * chunks][D]: of the leaf that reaches into the chunk, of the one
+// that starts in it and reaches out). Blocks from there on: zeros for the leaves without rows.
+template <typename T, int W>
 __global__ __launch_bounds__(kLeThreads) void le_backward_kernel(
-    const T* __restrict__ dy, const int32_t* __restrict__ order, const uint32_t* __restrict__ keys,
-    const int32_t* __restrict__ off, int64_t V, int D, float scale, LeCols lc, int64_t light,
-    T* __restrict__ dtable, typename LeAcc<T>::type* __restrict__ part) {
+    const T* __restrict__ dy, int64_t stride, const int32_t* __restrict__ order,
+    const uint32_t* __restrict__ keys, const int32_t* __restrict__ off, int64_t V, int D,
+    float scale, LeCols lc, int run_shift,
+    int64_t chunk_blocks, T* __restrict__ dtable, typename LeAcc<T>::type* __restrict__ part) {
   using A = typename LeAcc<T>::type;
-  __shared__ A s_acc[NC * W * kLeThreads / 2];
   const int tpr = 1 << lc.tpr_shift, rpb = kLeThreads >> lc.tpr_shift;
   const int sub = threadIdx.x >> lc.tpr_shift, lr = threadIdx.x & (tpr - 1);
-  int64_t blk = leaf_block();
-  const int c0 = ((int)(blk % lc.col_blocks) * NC * tpr + lr) * W;
-  blk /= lc.col_blocks;
-  if (blk < light) {
-    const int64_t v = blk * rpb + sub;
-    if (v >= V) return;
-    const int64_t a = off[v], b = off[v + 1];
-    if (b - a > kLeRun) return;
-    A acc[NC][W] = {};
-    le_sum_rows<T, W, NC, A>(dy, D, c0, tpr, order, a, b, 1, acc);
-    le_store<T, W, NC, A>(dtable + v * D, D, c0, tpr, scale, acc);
+  const int64_t blk = leaf_block();
+  if (blk >= chunk_blocks) {
+    const int64_t v0 = ((blk - chunk_blocks) * rpb + sub) * kLeEmpty;
+    uint32_t none = 0;
+#pragma unroll
+    for (int i = 0; i < kLeEmpty; ++i)
+      if (v0 + i < V && off[v0 + i] == off[v0 + i + 1]) none |= 1u << i;
+    while (none) {
+      const int i = __ffs((int)none) - 1;
+      none &= none - 1;
+      for (int c = lr * W; c < D; c += tpr * W)
+        *(LeafVec<T, W>*)(dtable + (v0 + i) * D + c) = LeafVec<T, W>{};
+    }
     return;
   }
-  const int64_t c = blk - light, m = off[V];
-  const int64_t a = c * kLeRun, b = min<int64_t>(a + kLeRun, m);
-  if (a >= m) return;
-  const int64_t k0 = keys[a], k1 = keys[b - 1];
-  const int64_t e0 = off[k0 + 1], s1 = off[k1];
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    if (which == 0 && e0 - off[k0] <= kLeRun) continue;
-    if (which == 1 && (k1 == k0 || off[k1 + 1] - s1 <= kLeRun)) continue;
-    A acc[NC][W] = {};
-    const int64_t pa = which == 0 ? a : s1, pb = which == 0 ? min<int64_t>(b, e0) : b;
-    le_sum_rows<T, W, NC, A>(dy, D, c0, tpr, order, pa + sub, pb, rpb, acc);
-    le_block_sum<W, NC, A>(acc, lc.tpr_shift, s_acc);
-    if (sub == 0) {
-      A* out = part + (2 * c + which) * D;
+  const int64_t chunk = blk / lc.col_blocks * rpb + sub, m = off[V];
+  const int c0 = ((int)(blk % lc.col_blocks) * tpr + lr) * W;
+  const int64_t a = chunk << run_shift, b = min<int64_t>(a + (1 << run_shift), m);
+  if (a >= m || c0 >= D) return;
+  const bool into = a > 0 && keys[a - 1] == keys[a];
+  const bool out_of = b < m && keys[b] == keys[b - 1];
+  A acc[W] = {};
+  uint32_t cur = keys[a];
+  bool first = true;
+  auto partial = [&](int which) {
+    A* const to = part + (2 * chunk + which) * D + c0;
 #pragma unroll
-      for (int q = 0; q < NC; ++q) {
-        const int col = c0 + q * tpr * W;
-        if (col >= D) break;
+    for (int e = 0; e < W; ++e) to[e] = acc[e];
+  };
+  for (int64_t p = a; p < b; p += kLeBatch) {
+    uint32_t key[kLeBatch];
+    LeafVec<T, W> v[kLeBatch];
 #pragma unroll
-        for (int e = 0; e < W; ++e) out[col + e] = acc[q][e];
+    for (int u = 0; u < kLeBatch; ++u) {
+      const int64_t pu = min(p + u, b - 1);
+      key[u] = keys[pu];
+      v[u] = *(const LeafVec<T, W>*)(dy + order[pu] * stride + c0);
+    }
+#pragma unroll
+    for (int u = 0; u < kLeBatch; ++u) {
+      if (p + u >= b) break;
+      if (key[u] != cur) {
+        if (first && into)
+          partial(0);
+        else
+          le_store<T, W, A>(dtable + (int64_t)cur * D + c0, scale, acc);
+        first = false;
+        cur = key[u];
+#pragma unroll
+        for (int e = 0; e < W; ++e) acc[e] = 0;
       }
+#pragma unroll
+      for (int e = 0; e < W; ++e) acc[e] += (A)leaf_f32(v[u].v[e]);
     }
   }
+  if (first && into)
+    partial(0);
+  else if (out_of)
+    partial(1);
+  else
+    le_store<T, W, A>(dtable + (int64_t)cur * D + c0, scale, acc);
 }
 
-// One block (and column block) per chunk; it works if a leaf with more than kLeRun rows starts in
-// the chunk, and adds that leaf's partial rows.
-template <typename T, int W, int NC>
+// One block (and column block) per chunk; it works if a leaf starts in the chunk and reaches out of
+// it, and adds that leaf's partial rows.
+template <typename T, int W>
 __global__ __launch_bounds__(kLeThreads) void le_join_kernel(
     const typename LeAcc<T>::type* __restrict__ part, const uint32_t* __restrict__ keys,
-    const int32_t* __restrict__ off, int64_t V, int D, float scale, LeCols lc,
+    const int32_t* __restrict__ off, int64_t V, int D, float scale, LeCols lc, int run_shift,
     T* __restrict__ dtable) {
   using A = typename LeAcc<T>::type;
-  __shared__ A s_acc[NC * W * kLeThreads / 2];
+  __shared__ A s_acc[W * kLeThreads / 2];
   const int tpr = 1 << lc.tpr_shift, rpb = kLeThreads >> lc.tpr_shift;
   const int sub = threadIdx.x >> lc.tpr_shift, lr = threadIdx.x & (tpr - 1);
-  int64_t c = leaf_block();
-  const int c0 = ((int)(c % lc.col_blocks) * NC * tpr + lr) * W;
-  c /= lc.col_blocks;
-  const int64_t m = off[V], a = c * kLeRun, b = min<int64_t>(a + kLeRun, m);
-  if (a >= m) return;
-  const int64_t k0 = keys[a], k1 = keys[b - 1];
-  const int64_t s1 = off[k1], e1 = off[k1 + 1];
-  if (s1 < a || e1 - s1 <= kLeRun) return;
-  A acc[NC][W] = {};
-  const int64_t last = (e1 - 1) / kLeRun;
-  for (int64_t p = c + sub; p <= last; p += rpb) {
-    const A* in = part + (2 * p + (p == c && k1 != k0 ? 1 : 0)) * D;
+  const int64_t blk = leaf_block(), chunk = blk / lc.col_blocks;
+  const int c0 = ((int)(blk % lc.col_blocks) * tpr + lr) * W;
+  const int64_t m = off[V], a = chunk << run_shift, b = a + (1 << run_shift);
+  if (b >= m) return;
+  const uint32_t k = keys[b - 1];
+  if (keys[b] != k || off[k] < a) return;
+  const int64_t last = (off[k + 1] - 1) >> run_shift;
+  A acc[W] = {};
+  if (c0 < D) {
+#pragma unroll 4
+    for (int64_t p = chunk + sub; p <= last; p += rpb) {
+      const A* const in = part + (2 * p + (p == chunk ? 1 : 0)) * D + c0;
 #pragma unroll
-    for (int q = 0; q < NC; ++q) {
-      const int col = c0 + q * tpr * W;
-      if (col >= D) break;
-#pragma unroll
-      for (int e = 0; e < W; ++e) acc[q][e] += in[col + e];
+      for (int e = 0; e < W; ++e) acc[e] += in[e];
     }
   }
-  le_block_sum<W, NC, A>(acc, lc.tpr_shift, s_acc);
-  if (sub == 0) le_store<T, W, NC, A>(dtable + k1 * D, D, c0, tpr, scale, acc);
+  le_block_sum<W, A>(acc, lc.tpr_shift, s_acc);
+  if (sub == 0 && c0 < D) le_store<T, W, A>(dtable + (int64_t)k * D + c0, scale, acc);
 }
 
 static LeCols le_cols(int D, int W, int NC) {
@@ -316,57 +297,61 @@ void launch_leaf_embed(hipStream_t s, int type, const void* ids, bool wide, cons
     });
 }
 
-// bytes of scratch for the partial rows
+// Sorted positions of a chunk: 16 to 256, so few that the chunks make about 4096 waves (16 on each
+// CU); longer chunks leave fewer partial rows.
+static int le_run_shift(int64_t n, const LeCols& lc) {
+  int shift = 8;
+  while (shift > 4 && ((n >> shift) * lc.col_blocks << lc.tpr_shift) / kWave < 4096) --shift;
+  return shift;
+}
+
+// bytes of scratch for the partial rows, whichever width is taken
 int64_t leaf_embed_grad_bytes(int type, int64_t n, int D) {
-  if (n <= kLeRun) return 0;
-  return 2 * ((n + kLeRun - 1) / kLeRun) * D * (type == kLeafF32 ? 8 : 4);
+  int shift = 8;
+  for (int W : {8, 4, 2, 1}) shift = std::min(shift, le_run_shift(n, le_cols(D, W, 1)));
+  return 2 * ((n >> shift) + 1) * D * (type == kLeafF32 ? 8 : 4);
 }
 
 template <typename T, int W>
-static void le_backward(hipStream_t s, const T* dy, const int32_t* order, const uint32_t* keys,
-                        const int32_t* off, int64_t n, int64_t V, int D, float scale, T* dtable,
+static void le_backward(hipStream_t s, const T* dy, int64_t stride, const int32_t* order,
+                        const uint32_t* keys, const int32_t* off, int64_t n, int64_t V, int D, float scale, T* dtable,
                         void* work) {
   using A = typename LeAcc<T>::type;
-  const bool four = D >= 4 * kWave * W;
-  const LeCols lc = le_cols(D, W, four ? 4 : 1);
-  const int rpb = kLeThreads >> lc.tpr_shift;
-  const int64_t light = (V + rpb - 1) / rpb;
-  const int64_t chunks = n > kLeRun ? (n + kLeRun - 1) / kLeRun : 0;
-  const dim3 grid = leaf_grid((light + chunks) * lc.col_blocks);
-  auto go = [&](auto kern, auto join) {
-    hipLaunchKernelGGL(kern, grid, dim3(kLeThreads), 0, s, dy, order, keys, off, V, D, scale, lc,
-                       light, dtable, (A*)work);
+  const LeCols lc = le_cols(D, W, 1);
+  const int rpb = kLeThreads >> lc.tpr_shift, shift = le_run_shift(n, lc);
+  const int64_t chunks = (n + (1 << shift) - 1) >> shift;
+  const int64_t chunk_blocks = (chunks + rpb - 1) / rpb * lc.col_blocks;
+  const int64_t empty = (V + rpb * kLeEmpty - 1) / (rpb * kLeEmpty);
+  hipLaunchKernelGGL((le_backward_kernel<T, W>), leaf_grid(chunk_blocks + empty), dim3(kLeThreads), 0,
+                     s, dy, stride, order, keys, off, V, D, scale, lc, shift, chunk_blocks, dtable,
+                     (A*)work);
+  MT_HIP_CHECK(hipGetLastError());
+  if (chunks > 1) {
+    hipLaunchKernelGGL((le_join_kernel<T, W>), leaf_grid((chunks - 1) * lc.col_blocks),
+                       dim3(kLeThreads), 0, s, (const A*)work, keys, off, V, D, scale, lc, shift,
+                       dtable);
     MT_HIP_CHECK(hipGetLastError());
-    if (chunks > 0) {
-      hipLaunchKernelGGL(join, leaf_grid(chunks * lc.col_blocks), dim3(kLeThreads), 0, s,
-                         (const A*)work, keys, off, V, D, scale, lc, dtable);
-      MT_HIP_CHECK(hipGetLastError());
-    }
-  };
-  if (four)
-    go(le_backward_kernel<T, W, 4>, le_join_kernel<T, W, 4>);
-  else
-    go(le_backward_kernel<T, W, 1>, le_join_kernel<T, W, 1>);
+  }
 }
 
-void launch_leaf_embed_grad(hipStream_t s, int type, const void* dy, const int32_t* order,
-                            const uint32_t* keys, const int32_t* off, int64_t n, int64_t V, int D,
+void launch_leaf_embed_grad(hipStream_t s, int type, const void* dy, int64_t stride,
+                            const int32_t* order, const uint32_t* keys, const int32_t* off, int64_t n, int64_t V, int D,
                             float scale, void* dtable, void* work) {
   if (D <= 0) return;
-  const int W = le_width(type == kLeafF32 ? 4 : 2, D, D, dy, dtable);
+  const int W = le_width(type == kLeafF32 ? 4 : 2, D, stride, dy, dtable);
   if (type == kLeafF32)
     le_dispatch_32(W, [&](auto w) {
-      le_backward<float, w()>(s, (const float*)dy, order, keys, off, n, V, D, scale,
+      le_backward<float, w()>(s, (const float*)dy, stride, order, keys, off, n, V, D, scale,
                               (float*)dtable, work);
     });
   else if (type == kLeafF16)
     le_dispatch_16(W, [&](auto w) {
-      le_backward<f16_t, w()>(s, (const f16_t*)dy, order, keys, off, n, V, D, scale,
+      le_backward<f16_t, w()>(s, (const f16_t*)dy, stride, order, keys, off, n, V, D, scale,
                               (f16_t*)dtable, work);
     });
   else
     le_dispatch_16(W, [&](auto w) {
-      le_backward<bf16_t, w()>(s, (const bf16_t*)dy, order, keys, off, n, V, D, scale,
+      le_backward<bf16_t, w()>(s, (const bf16_t*)dy, stride, order, keys, off, n, V, D, scale,
                                (bf16_t*)dtable, work);
     });
 }

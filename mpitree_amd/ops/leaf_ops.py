@@ -25,7 +25,7 @@ plain path of the same results.
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from contextlib import nullcontext
 
 import torch
 
@@ -38,21 +38,41 @@ _MAX_ROWS = 2 ** 31 - 1
 _MAX_WIDTH = 2 ** 20
 
 
-@dataclass(frozen=True)
 class LeafRoute:
-    """Rows sorted by leaf: ``order[offsets[g]:offsets[g + 1]]`` are leaf ``g``'s rows in their
-    order, for ``g == n_leaves`` the rows without a leaf."""
+    """Rows sorted by leaf, from :func:`leaf_route`: ``order[offsets[g]:offsets[g + 1]]`` are leaf
+    ``g``'s rows in their order, for ``g == n_leaves`` the rows without a leaf.
 
-    leaves: torch.Tensor  # the leaf numbers, as given
-    n_leaves: int
-    order: torch.Tensor  # int32 [n]
-    keys: torch.Tensor  # int32 [n], the leaf at each sorted position (n_leaves: none)
-    offsets: torch.Tensor  # int32 [n_leaves + 2]
+    ``leaves`` are the leaf numbers it was made from, ``keys`` [n] the leaf at each sorted position
+    (``n_leaves``: none), ``order`` [n] and ``offsets`` [n_leaves + 2]: int32 tensors. It stays
+    valid when ``leaves`` is changed later; the operators then still follow the route."""
+
+    __slots__ = ("leaves", "n_leaves", "_buf")
+
+    def __init__(self, leaves: torch.Tensor, n_leaves: int, buf: torch.Tensor):
+        self.leaves, self.n_leaves, self._buf = leaves, n_leaves, buf
+
+    @property
+    def order(self) -> torch.Tensor:
+        return self._buf[: self.leaves.numel()]
+
+    @property
+    def keys(self) -> torch.Tensor:
+        n = self.leaves.numel()
+        return self._buf[n : 2 * n]
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        return self._buf[2 * self.leaves.numel() :]
 
     @property
     def counts(self) -> torch.Tensor:
         """Rows of each leaf, int32 [n_leaves]."""
-        return self.offsets[1 : self.n_leaves + 1] - self.offsets[: self.n_leaves]
+        off = self.offsets
+        return off[1 : self.n_leaves + 1] - off[: self.n_leaves]
+
+    def __repr__(self):
+        return (f"LeafRoute({self.leaves.numel()} rows, {self.n_leaves} leaves, "
+                f"device={self.leaves.device})")
 
 
 def _check_leaves(leaves) -> torch.Tensor:
@@ -89,14 +109,25 @@ def _check_width(what: str, width: int):
         raise ValueError(f"{what} must be in [1, {_MAX_WIDTH}], got {width}")
 
 
-def _check_device(*tensors):
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"operands on different devices: {sorted(map(str, devices))}")
+def _check_device(first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"operands on different devices: {first.device}, {t.device}")
+
+
+def _on(device):
+    """A context with ``device`` current (launches go to the current device)."""
+    if device.index == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(device)
 
 
 def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _scratch(nbytes: int, device) -> torch.Tensor:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -117,16 +148,15 @@ def leaf_route(leaves: torch.Tensor, n_leaves: int) -> LeafRoute:
         key, order = torch.sort(key, stable=True)
         bounds = torch.arange(n_leaves + 1, dtype=torch.int64)
         offsets = torch.cat([torch.searchsorted(key, bounds), torch.tensor([n])])
-        return LeafRoute(leaves, n_leaves, order.int(), key.int(), offsets.int())
+        return LeafRoute(leaves, n_leaves, torch.cat([order, key, offsets]).int())
     hip = native.hip()
-    with torch.cuda.device(dev):
+    with _on(dev):
         ids = ids.contiguous()
-        buf = torch.empty(2 * n + n_leaves + 2, dtype=torch.int32, device=dev)
-        order, keys, offsets = buf[:n], buf[n : 2 * n], buf[2 * n :]
-        work = torch.empty(hip.leaf_route_words(n, n_leaves), dtype=torch.int32, device=dev)
+        buf = torch.empty(hip.leaf_route_len(n, n_leaves), dtype=torch.int32, device=dev)
+        work = _scratch(4 * hip.leaf_route_words(n, n_leaves), dev)
         hip.leaf_route(_stream(ids), ids.data_ptr(), ids.dtype == torch.int64, n, n_leaves,
-                       order.data_ptr(), keys.data_ptr(), offsets.data_ptr(), work.data_ptr())
-    return LeafRoute(leaves, n_leaves, order, keys, offsets)
+                       buf.data_ptr(), work.data_ptr())
+    return LeafRoute(leaves, n_leaves, buf)
 
 
 # ---------------------------------------------------------------------------- embedding
@@ -141,29 +171,35 @@ def _embed_forward(ids: torch.Tensor, table: torch.Tensor, scale: float) -> torc
     if table.stride(1) != 1 and D > 1:
         table = table.contiguous()
     ids = ids.contiguous()
-    with torch.cuda.device(ids.device):
+    with _on(ids.device):
         native.hip().leaf_embed(_stream(ids), _TYPES[table.dtype], ids.data_ptr(),
                                 ids.dtype == torch.int64, table.data_ptr(), table.stride(0),
                                 ids.numel(), table.shape[0], D, scale, y.data_ptr())
     return y
 
 
-def _sum_by_leaf(dy: torch.Tensor, route: LeafRoute, scale: float) -> torch.Tensor:
+def _sum_by_leaf_plain(dy, route: LeafRoute, scale: float) -> torch.Tensor:
+    V = route.n_leaves
+    out = torch.zeros((V + 1, dy.shape[1]), dtype=torch.float64)
+    out.index_add_(0, route.keys.long(), dy[route.order.long()].double())
+    return (out[:V] * scale).to(dy.dtype)
+
+
+def _embed_grad(dy, ids, route, n_leaves: int, scale: float) -> torch.Tensor:
     """scale * the sum of dy's rows of each leaf, [n_leaves, D]."""
-    V, D = route.n_leaves, dy.shape[-1]
-    dy = dy.reshape(-1, D)
+    D = dy.shape[-1]
     if not dy.is_cuda:
-        out = torch.zeros((V + 1, D), dtype=torch.float64)
-        out.index_add_(0, route.keys.long(), dy[route.order.long()].double())
-        return (out[:V] * scale).to(dy.dtype)
-    dy = dy.contiguous()
-    hip, n, kind = native.hip(), dy.shape[0], _TYPES[dy.dtype]
-    with torch.cuda.device(dy.device):
-        out = torch.empty((V, D), dtype=dy.dtype, device=dy.device)
-        work = torch.empty(hip.leaf_embed_grad_bytes(kind, n, D), dtype=torch.uint8,
-                           device=dy.device)
-        hip.leaf_embed_grad(_stream(dy), kind, dy.data_ptr(), route.order.data_ptr(),
-                            route.keys.data_ptr(), route.offsets.data_ptr(), n, V, D, scale,
+        route = route if route is not None else leaf_route(ids, n_leaves)
+        return _sum_by_leaf_plain(dy.reshape(-1, D), route, scale)
+    hip, kind, dev = native.hip(), _TYPES[dy.dtype], dy.device
+    with _on(dev):
+        dy, ids = _rows(dy), ids.contiguous()
+        n = dy.shape[0]
+        out = torch.empty((n_leaves, D), dtype=dy.dtype, device=dev)
+        work = _scratch(hip.leaf_embed_grad_bytes(kind, n, n_leaves, D, route is not None), dev)
+        hip.leaf_embed_grad(_stream(dy), kind, dy.data_ptr(), dy.stride(0), ids.data_ptr(),
+                            ids.dtype == torch.int64,
+                            0 if route is None else route._buf.data_ptr(), n, n_leaves, D, scale,
                             out.data_ptr(), work.data_ptr())
     return out
 
@@ -179,8 +215,7 @@ class _Embedding(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
-        route = ctx.route if ctx.route is not None else leaf_route(ids, ctx.n_leaves)
-        return _sum_by_leaf(dy, route, ctx.scale), None, None, None
+        return _embed_grad(dy, ids, ctx.route, ctx.n_leaves, ctx.scale), None, None, None
 
 
 def leaf_embedding(leaves, table: torch.Tensor, *, scale: float = 1.0) -> torch.Tensor:
@@ -231,47 +266,46 @@ def _linear_plain_grad(dy, x, route, w, need_x, need_w):
     return (dx.to(x.dtype) if need_x else None), (dw.to(w.dtype) if need_w else None)
 
 
-def _linear_tile(dx: bool, src, route, w, bias) -> torch.Tensor:
-    G, N, K = w.shape
-    hip, n = native.hip(), src.shape[0]
-    out = torch.empty((n, K if dx else N), dtype=src.dtype, device=src.device)
-    work = torch.empty(hip.leaf_linear_tile_bytes(n, G), dtype=torch.uint8, device=src.device)
-    hip.leaf_linear_tile(
-        _stream(src), _TYPES[src.dtype], dx, src.data_ptr(), src.stride(0),
-        route.order.data_ptr(), route.offsets.data_ptr(), n, G, w.data_ptr(),
-        0 if bias is None else bias.data_ptr(), K, N, out.data_ptr(), work.data_ptr())
-    return out
-
-
 def _linear_forward(x, ids, route, w, b):
-    """Returns (y, route): the route is built where the kernel needs one."""
-    if not x.is_cuda:
-        route = route if route is not None else leaf_route(ids, w.shape[0])
-        return _linear_plain(x, route, w, b), route
-    hip = native.hip()
+    """Returns (y, route): the route is made where the kernel needs one."""
     n, (G, N, K) = x.shape[0], w.shape
-    with torch.cuda.device(x.device):
-        if n <= hip.leaf_linear_small_rows():
-            y = torch.empty((n, N), dtype=x.dtype, device=x.device)
-            ids = ids.contiguous()
-            hip.leaf_linear_small(_stream(x), _TYPES[x.dtype], x.data_ptr(), x.stride(0),
-                                  ids.data_ptr(), ids.dtype == torch.int64, n, G, w.data_ptr(),
-                                  0 if b is None else b.data_ptr(), K, N, y.data_ptr())
-            return y, route
+    if not x.is_cuda:
         route = route if route is not None else leaf_route(ids, G)
-        return _linear_tile(False, x, route, w, b), route
+        return _linear_plain(x, route, w, b), route
+    hip, kind, dev = native.hip(), _TYPES[x.dtype], x.device
+    with _on(dev):
+        ids = ids.contiguous()
+        wide, bias = ids.dtype == torch.int64, 0 if b is None else b.data_ptr()
+        y = torch.empty((n, N), dtype=x.dtype, device=dev)
+        if n <= hip.leaf_linear_small_rows():
+            hip.leaf_linear_small(_stream(x), kind, x.data_ptr(), x.stride(0), ids.data_ptr(), wide,
+                                  n, G, w.data_ptr(), bias, K, N, y.data_ptr())
+            return y, route
+        work = _scratch(hip.leaf_linear_bytes(n, G), dev)
+        sort = 0
+        if route is None:
+            sort = ids.data_ptr()
+            buf = torch.empty(hip.leaf_route_len(n, G), dtype=torch.int32, device=dev)
+            route = LeafRoute(ids, G, buf)
+        hip.leaf_linear(_stream(x), kind, x.data_ptr(), x.stride(0), sort, wide,
+                        route._buf.data_ptr(), n, G, w.data_ptr(), bias, K, N, y.data_ptr(),
+                        work.data_ptr())
+    return y, route
 
 
-def _linear_grad_weight(dy, x, route, w) -> torch.Tensor:
-    G, N, K = w.shape
-    hip, n = native.hip(), x.shape[0]
-    dw = torch.empty((G, N, K), dtype=x.dtype, device=x.device)
-    work = torch.empty(hip.leaf_linear_grad_bytes(_TYPES[x.dtype], n, G, K, N), dtype=torch.uint8,
-                       device=x.device)
-    hip.leaf_linear_grad(_stream(x), _TYPES[x.dtype], x.data_ptr(), x.stride(0), dy.data_ptr(),
-                         dy.stride(0), route.order.data_ptr(), route.keys.data_ptr(),
-                         route.offsets.data_ptr(), n, G, K, N, dw.data_ptr(), work.data_ptr())
-    return dw
+def _linear_grad(dy, x, route, w, need_x, need_w, need_b):
+    n, (G, N, K) = x.shape[0], w.shape
+    hip, kind, dev = native.hip(), _TYPES[x.dtype], x.device
+    with _on(dev):
+        dy = _rows(dy)
+        dx, dw, db = (torch.empty(shape, dtype=x.dtype, device=dev) if need else None
+                      for need, shape in ((need_x, (n, K)), (need_w, (G, N, K)), (need_b, (G, N))))
+        work = _scratch(hip.leaf_linear_grad_bytes(kind, n, G, K, N), dev)
+        hip.leaf_linear_grad(_stream(x), kind, x.data_ptr(), x.stride(0), dy.data_ptr(),
+                             dy.stride(0), route._buf.data_ptr(), n, G, w.data_ptr(), K, N,
+                             *(0 if t is None else t.data_ptr() for t in (dx, dw, db)),
+                             work.data_ptr())
+    return dx, dw, db
 
 
 class _Linear(torch.autograd.Function):
@@ -287,15 +321,12 @@ class _Linear(torch.autograd.Function):
         x, w, ids = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         route = ctx.route if ctx.route is not None else leaf_route(ids, w.shape[0])
-        if not x.is_cuda:
-            dx, dw = _linear_plain_grad(dy, x, route, w, need_x, need_w)
+        if x.is_cuda:
+            grads = _linear_grad(dy, x, route, w, need_x, need_w, need_b)
         else:
-            with torch.cuda.device(x.device):
-                dy = _rows(dy)
-                dx = _linear_tile(True, dy, route, w, None) if need_x else None
-                dw = _linear_grad_weight(dy, x, route, w) if need_w else None
-        db = _sum_by_leaf(dy, route, 1.0) if need_b else None
-        return dx, dw, db, None, None
+            grads = _linear_plain_grad(dy, x, route, w, need_x, need_w)
+            grads += (_sum_by_leaf_plain(dy, route, 1.0) if need_b else None,)
+        return (*grads, None, None)
 
 
 def leaf_linear(inputs: torch.Tensor, leaves, weight: torch.Tensor, bias=None) -> torch.Tensor:
