@@ -199,6 +199,18 @@ __device__ __forceinline__ void ll_dma_wait() {
 // what the chunks behind the end of the depth are read from
 __device__ const uint4 kLlZeros[1] = {};
 
+// *p, or zeros, read either way; from the global address space, which a choice of two plain
+// pointers would leave
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <typename V>
+__device__ __forceinline__ V ll_load_or_zeros(bool there, const void* p) {
+  using U = std::conditional_t<sizeof(V) == 16, u32x4,
+                               std::conditional_t<sizeof(V) == 4, uint32_t, uint16_t>>;
+  const U u = *(const __attribute__((address_space(1))) U*)(there ? (uintptr_t)p
+                                                                  : (uintptr_t)kLlZeros);
+  return __builtin_bit_cast(V, u);
+}
+
 // Blocks go to the 8 XCDs in turn, and each XCD has its own L2: runs of kLlXcdRun tiles stay on one
 // XCD, so that neighbours share the panels they read; runs go round, so that a stretch of tiles
 // without rows does not leave an XCD idle.
@@ -476,6 +488,125 @@ __global__ __launch_bounds__(NW* kWave) void ll_tile_kernel(LlTile a) {
   ll_store_rows<T, 16, SJ, SI>(acc, a, at, wj, wi);
 }
 
+// ---- short rows: at most 256 bytes of depth, so a wave holds its columns of the leaf's matrix
+// in registers and streams the leaf's rows past them, from memory straight into fragments, without
+// LDS or barriers. A wave takes up to kRowsTile rows of one leaf and SI * 16 columns.
+constexpr int kRowsTile = 128, kRowsShift = 7;
+
+template <typename T, bool kDx, int STEPS, int SI, bool kAligned>
+__global__ __launch_bounds__(kLlThreads) void ll_rows_kernel(LlTile a) {
+  constexpr int E = Ll<T>::kEpc;
+  const int l = lane_id();
+  const int64_t tile = leaf_block() * kLlWaves +
+                       __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  if (tile >= a.tiles) return;
+  const int64_t slot = tile / a.col_tiles;
+  const int i0 = (int)(tile % a.col_tiles) * SI * 16;
+  const int g = leaf_find_group(a.off, a.G + 1, kRowsShift, slot);
+  const int64_t first = a.off[g];
+  const int64_t m0 = first + ((slot - ((first >> kRowsShift) + (int64_t)g)) << kRowsShift);
+  const int rows = (int)max<int64_t>(-1, min<int64_t>(kRowsTile, a.off[g + 1] - m0));
+  if (rows <= 0) return;
+  // 16 rows at a time; the row of this lane in the j-th 16 (past the last one: that one)
+  const int32_t ord0 = a.order[m0 + min(l, rows - 1)];
+  const int32_t ord1 = a.order[m0 + min(kWave + l, rows - 1)];
+  auto row_of = [&](int j) {
+    return __shfl(j < 4 ? ord0 : ord1, ((16 * j) & (kWave - 1)) + (l & 15), kWave);
+  };
+  const bool vec = a.cols % 4 == 0 && (uintptr_t)a.out % (4 * sizeof(T)) == 0;
+  const int c0 = i0 + 4 * (l >> 4);
+  // whole: all 16 rows and all columns are there, and aligned
+  auto store = [&](auto whole, int j, int32_t row, const f32x4 (&acc)[SI]) {
+    T* const o = (T*)a.out + (int64_t)row * a.cols;
+    if constexpr (whole()) {
+#pragma unroll
+      for (int i = 0; i < SI; ++i) ll_store4<true>(o + c0 + i * 16, acc[i], 4);
+    } else {
+      if (16 * j + (l & 15) >= rows) return;
+#pragma unroll
+      for (int i = 0; i < SI; ++i) {
+        const int c = c0 + i * 16;
+        ll_store4<false>(o + c, acc[i], a.cols - c);
+      }
+    }
+  };
+  constexpr std::true_type kYes{};
+  constexpr std::false_type kNo{};
+  if (g == a.G) {  // rows without a leaf
+    const f32x4 zero[SI] = {};
+    for (int j = 0; 16 * j < rows; ++j) store(kNo, j, row_of(j), zero);
+    return;
+  }
+  const T* const src = (const T*)a.src;
+  auto load = [&](int32_t row, uint4 (&f)[STEPS]) {
+    const T* const p = src + row * a.src_stride;
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t) {
+      const int k = (4 * t + (l >> 4)) * E;
+      if constexpr (kAligned)
+        f[t] = ll_load_or_zeros<uint4>(k < a.depth, p + k);
+      else
+        f[t] = ll_chunk<T, false>(p + k, a.depth - k);
+    }
+  };
+  uint4 f0[STEPS], f1[STEPS];
+  load(row_of(0), f0);
+  const T* const wg = (const T*)a.w + (int64_t)g * a.w_stride;
+  uint4 fw[SI][STEPS];
+#pragma unroll
+  for (int i = 0; i < SI; ++i) {
+    const int col = min(i0 + i * 16 + (l & 15), a.cols - 1);  // (past the last: not stored)
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t) {
+      const int k = (4 * t + (l >> 4)) * E;
+      if constexpr (kDx) {
+        T e[E];
+#pragma unroll
+        for (int u = 0; u < E; ++u) {
+          e[u] = ll_load_or_zeros<T>(k + u < a.depth, wg + (int64_t)(k + u) * a.w_row + col);
+        }
+        __builtin_memcpy(&fw[i][t], e, 16);
+      } else {
+        const T* const p = wg + (int64_t)col * a.w_row + k;
+        if constexpr (kAligned)
+          fw[i][t] = ll_load_or_zeros<uint4>(k < a.depth, p);
+        else
+          fw[i][t] = ll_chunk<T, false>(p, a.depth - k);
+      }
+    }
+  }
+  f32x4 bias[SI] = {};
+  if (a.bias != nullptr) {
+    const T* const bg = (const T*)a.bias + (int64_t)g * a.cols;
+#pragma unroll
+    for (int i = 0; i < SI; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bias[i][e] = leaf_f32(bg[min(c0 + i * 16 + e, a.cols - 1)]);
+  }
+  auto step = [&](auto whole, int j, const uint4 (&f)[STEPS], uint4 (&next)[STEPS]) {
+    load(row_of(j + 1), next);
+    f32x4 acc[SI];
+#pragma unroll
+    for (int i = 0; i < SI; ++i) acc[i] = bias[i];
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+      for (int i = 0; i < SI; ++i) acc[i] = ll_mma<T>(fw[i][t], f[t], acc[i]);
+    store(whole, j, row_of(j), acc);
+  };
+  int j = 0;
+  if (vec && i0 + SI * 16 <= a.cols) {
+    for (; 16 * (j + 2) <= rows; j += 2) {
+      step(kYes, j, f0, f1);
+      step(kYes, j + 1, f1, f0);
+    }
+  }
+  for (; 16 * j < rows; j += 2) {
+    step(kNo, j, f0, f1);
+    if (16 * (j + 1) < rows) step(kNo, j + 1, f1, f0);
+  }
+}
+
 // ---- 256 x 256 tiles of 16-bit types, where rows and columns fill them: 8 waves of 128 x 64.
 //
 // A tile of depth is multiplied in two halves. While one half is multiplied, the other's
@@ -653,7 +784,9 @@ struct LlGrad {
   const void* x;
   const void* dy;
   void* dw;
-  float* part;  // [2 * chunks][N][K]
+  void* db;        // null: not made here
+  float* part;     // [2 * chunks][N][K]
+  double* part_b;  // [2 * chunks][N]
   const int32_t* order;
   const uint32_t* keys;
   const int32_t* off;
@@ -709,84 +842,141 @@ __device__ __forceinline__ void ll_grad_store(const f32x4 (&acc)[SJ][SI], const 
   }
 }
 
-// One BJ x BI tile (rows of W, columns of W) of one unit: both operands are gathered rows with the
-// rows as depth, turned.
-template <typename T, int BJ, int BI, int WJ, bool kAligned>
+// column c of the sum of a unit's rows of dy
+template <typename T>
+__device__ __forceinline__ void ll_store_sum(const LlGrad& a, int64_t unit, int c, double sum) {
+  if (unit < a.G)
+    ((T*)a.db)[unit * a.N + c] = leaf_from<T>((float)sum);
+  else
+    a.part_b[(unit - a.G) * a.N + c] = sum;
+}
+
+// One B x B tile (rows of W, columns of W) of one unit: both operands are gathered rows with the
+// rows as depth, turned. The row numbers of a tile of depth are fetched a tile ahead of the rows. The
+// sums of dy (db) fall out of its fragments, in 64 bits for f32. kAligned: as in ll_tile_kernel.
+template <typename T, int B, bool kAligned>
 __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
-  constexpr int E = Ll<T>::kEpc, KD = Ll<T>::kDepth;
-  constexpr int WI = kLlWaves / WJ;
-  constexpr int SJ = BJ / WJ / 16, SI = BI / WI / 16;
-  constexpr int QJ = (BJ * 8 + kLlThreads - 1) / kLlThreads;
-  constexpr int QI = (BI * 8 + kLlThreads - 1) / kLlThreads;
-  __shared__ uint4 s_j[BJ * 8], s_i[BI * 8];
+  using A = std::conditional_t<sizeof(T) == 4, double, float>;
+  constexpr int E = Ll<T>::kEpc, KD = Ll<T>::kDepth, kRow = B / E;
+  constexpr int S = B / 2 / 16, Q = B * 8 / kLlThreads;  // 2 x 2 waves
+  __shared__ uint4 s_j0[B * 8], s_i0[B * 8];
+  __shared__ uint4 s_j1[kAligned ? B * 8 : 1], s_i1[kAligned ? B * 8 : 1];
   const int64_t blk = leaf_block();
   const int tiles = a.n_tiles * a.k_tiles;
   const int64_t unit = blk / tiles;
   if (unit >= a.units) return;
   const int t = (int)(blk % tiles);
-  const int j0 = t / a.k_tiles * BJ, i0 = t % a.k_tiles * BI;
-  const int tid = threadIdx.x, l = lane_id(), w = tid / kWave;
-  const int wj = w / WI * (SJ * 16), wi = w % WI * (SI * 16);
-
+  const int j0 = t / a.k_tiles * B, i0 = t % a.k_tiles * B;
+  const int tid = threadIdx.x, l = lane_id(), w = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int wj = w / 2 * (S * 16), wi = w % 2 * (S * 16);
   int64_t pa, pb;
   if (!ll_grad_rows(a, unit, pa, pb)) return;
+  const int rows = (int)(pb - pa);
+  const int32_t* const order = a.order + pa;
 
-  f32x4 acc[SJ][SI] = {};
+  f32x4 acc[S][S] = {};
+  A sum[S] = {};
+  const bool sums = a.db != nullptr && i0 + wi == 0;
   const LlLane<T> ln;
-  const T* const x = (const T*)a.x;
-  const T* const dy = (const T*)a.dy;
-  uint4 vj[QJ], vi[QI];
-  auto load = [&](int64_t p0) {
-#pragma unroll
-    for (int q = 0; q < QJ; ++q) {
-      constexpr int kRow = BJ / E;
-      const int id = q * kLlThreads + tid, k = id / kRow, c = id % kRow;
-      const bool in = (BJ * 8 % kLlThreads == 0 || k < KD) && p0 + k < pb;
-      const int64_t row = in ? a.order[p0 + k] : 0;
-      vj[q] = ll_chunk<T, kAligned>(dy + row * a.dy_stride + j0 + c * E,
-                                    in ? a.N - j0 - c * E : 0);
-    }
-#pragma unroll
-    for (int q = 0; q < QI; ++q) {
-      constexpr int kRow = BI / E;
-      const int id = q * kLlThreads + tid, k = id / kRow, c = id % kRow;
-      const bool in = (BI * 8 % kLlThreads == 0 || k < KD) && p0 + k < pb;
-      const int64_t row = in ? a.order[p0 + k] : 0;
-      vi[q] = ll_chunk<T, kAligned>(x + row * a.x_stride + i0 + c * E, in ? a.K - i0 - c * E : 0);
-    }
-  };
-  if (pa < pb) load(pa);
-  for (int64_t p0 = pa; p0 < pb; p0 += KD) {
-#pragma unroll
-    for (int q = 0; q < QJ; ++q) {
-      const int id = q * kLlThreads + tid;
-      if (BJ * 8 % kLlThreads == 0 || id < BJ * 8)
-        s_j[ll_turn_chunk<T, BJ>(id / (BJ / E), id % (BJ / E))] = vj[q];
-    }
-#pragma unroll
-    for (int q = 0; q < QI; ++q) {
-      const int id = q * kLlThreads + tid;
-      if (BI * 8 % kLlThreads == 0 || id < BI * 8)
-        s_i[ll_turn_chunk<T, BI>(id / (BI / E), id % (BI / E))] = vi[q];
-    }
-    __syncthreads();
-    if (p0 + KD < pb) load(p0 + KD);
+  auto products = [&](const uint4* sj, const uint4* si) {
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
-      uint4 fj[SJ], fi[SI];
+      uint4 fj[S], fi[S];
 #pragma unroll
-      for (int j = 0; j < SJ; ++j) fj[j] = ll_frag_turn<T, BJ>(s_j, ln, wj / 16 + j, step);
+      for (int j = 0; j < S; ++j) fj[j] = ll_frag_turn<T, B>(sj, ln, wj / 16 + j, step);
 #pragma unroll
-      for (int i = 0; i < SI; ++i) fi[i] = ll_frag_turn<T, BI>(s_i, ln, wi / 16 + i, step);
+      for (int i = 0; i < S; ++i) fi[i] = ll_frag_turn<T, B>(si, ln, wi / 16 + i, step);
 #pragma unroll
-      for (int j = 0; j < SJ; ++j)
+      for (int j = 0; j < S; ++j)
 #pragma unroll
-        for (int i = 0; i < SI; ++i) acc[j][i] = ll_mma<T>(fi[i], fj[j], acc[j][i]);
+        for (int i = 0; i < S; ++i) acc[j][i] = ll_mma<T>(fi[i], fj[j], acc[j][i]);
+      if (sums) {
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+          T e[E];
+          __builtin_memcpy(e, &fj[j], 16);
+          A four[2] = {};
+#pragma unroll
+          for (int u = 0; u < E; ++u) four[u & 1] += (A)leaf_f32(e[u]);
+          sum[j] += four[0] + four[1];
+        }
+      }
     }
-    __syncthreads();
+  };
+  if (rows > 0) {
+    const T* const x = (const T*)a.x;
+    const T* const dy = (const T*)a.dy;
+    int32_t row[Q];  // of the next tile to fetch
+    auto next_rows = [&](int p0) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+        row[q] = order[min(p0 + (q * kLlThreads + tid) / kRow, rows - 1)];
+    };
+    if constexpr (kAligned) {
+      auto load = [&](uint4* sj, uint4* si, int p0) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const int id = q * kLlThreads + tid, k = id / kRow;
+          const int c = ll_turn_chunk<T, B>(k, id % kRow) - k * kRow;
+          const bool in = p0 + k < rows;
+          const T* const pj = dy + row[q] * a.dy_stride + min(j0 + c * E, a.N - E);
+          const T* const pi = x + row[q] * a.x_stride + min(i0 + c * E, a.K - E);
+          ll_dma(in ? (const void*)pj : kLlZeros, sj + q * kLlThreads + w * kWave);
+          ll_dma(in ? (const void*)pi : kLlZeros, si + q * kLlThreads + w * kWave);
+        }
+        next_rows(p0 + KD);
+      };
+      next_rows(0);
+      load(s_j0, s_i0, 0);
+      for (int p0 = 0; p0 < rows; p0 += 2 * KD) {
+        __syncthreads();
+        if (p0 + KD < rows) load(s_j1, s_i1, p0 + KD);
+        products(s_j0, s_i0);
+        if (p0 + KD >= rows) break;
+        __syncthreads();
+        if (p0 + 2 * KD < rows) load(s_j0, s_i0, p0 + 2 * KD);
+        products(s_j1, s_i1);
+      }
+    } else {
+      uint4 vj[Q], vi[Q];
+      auto load = [&](int p0) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const int id = q * kLlThreads + tid, k = id / kRow, c = id % kRow;
+          const bool in = p0 + k < rows;
+          vj[q] = ll_chunk<T, false>(dy + row[q] * a.dy_stride + j0 + c * E,
+                                     in ? a.N - j0 - c * E : 0);
+          vi[q] = ll_chunk<T, false>(x + row[q] * a.x_stride + i0 + c * E,
+                                     in ? a.K - i0 - c * E : 0);
+        }
+        next_rows(p0 + KD);
+      };
+      next_rows(0);
+      load(0);
+      for (int p0 = 0; p0 < rows; p0 += KD) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const int id = q * kLlThreads + tid;
+          s_j0[ll_turn_chunk<T, B>(id / kRow, id % kRow)] = vj[q];
+          s_i0[ll_turn_chunk<T, B>(id / kRow, id % kRow)] = vi[q];
+        }
+        __syncthreads();
+        if (p0 + KD < rows) load(p0 + KD);
+        products(s_j0, s_i0);
+        __syncthreads();
+      }
+    }
   }
-
-  ll_grad_store<T, SJ, SI>(acc, a, unit, j0 + wj, i0 + wi);
+  if (sums) {
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      sum[j] += __shfl_xor(sum[j], 16, kWave);
+      sum[j] += __shfl_xor(sum[j], 32, kWave);
+      const int c = j0 + wj + j * 16 + l;
+      if (l < 16 && c < a.N) ll_store_sum<T>(a, unit, c, (double)sum[j]);
+    }
+  }
+  ll_grad_store<T, S, S>(acc, a, unit, j0 + wj, i0 + wi);
 }
 
 // The same on 256 x 256 tiles of 16-bit types (see ll_big_kernel): both operands turned.
@@ -890,8 +1080,99 @@ __global__ __launch_bounds__(kBigThreads, 2) void ll_big_grad_kernel(LlGrad a) {
   ll_grad_store<T, SJ, SI>(acc, a, unit, j0 + wj, i0 + wi);
 }
 
-// Adds the partial matrices of the leaves with more than `run` rows: one block per chunk in which
-// such a leaf starts and per kLlThreads elements, in 64 bits for f32.
+// The same for f32 and few columns on either side: the waves of a block take 16 rows in turn, from
+// memory straight into fragments, each for the whole 16 SJ x 16 SI tile, and their sums meet in LDS.
+// The sums of dy (db) fall out of its fragments, in 64 bits.
+template <int SJ, int SI>
+__global__ __launch_bounds__(kLlThreads) void ll_rows_grad_kernel(LlGrad a) {
+  __shared__ f32x4 s_acc[2][SJ * SI][kWave];
+  __shared__ double s_b[kLlWaves][SJ * 16];
+  const int64_t blk = leaf_block();
+  const int tiles = a.n_tiles * a.k_tiles;
+  const int64_t unit = blk / tiles;
+  if (unit >= a.units) return;
+  const int t = (int)(blk % tiles);
+  const int j0 = t / a.k_tiles * (SJ * 16), i0 = t % a.k_tiles * (SI * 16);
+  const int l = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  int64_t pa, pb;
+  if (!ll_grad_rows(a, unit, pa, pb)) return;
+  const int rows = (int)(pb - pa);
+  const int32_t* const order = a.order + pa;
+  const float* const x = (const float*)a.x + i0 + (l & 15);
+  const float* const dy = (const float*)a.dy + j0 + (l & 15);
+
+  f32x4 acc[SJ][SI] = {};
+  double sum[SJ] = {};
+  auto load = [&](int p, f32x4 (&fj)[SJ], f32x4 (&fi)[SI]) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int q = p + 4 * (l >> 4) + u;
+      const int64_t row = q < rows ? order[q] : -1;
+#pragma unroll
+      for (int j = 0; j < SJ; ++j)
+        fj[j][u] = row >= 0 && j0 + j * 16 + (l & 15) < a.N ? dy[row * a.dy_stride + j * 16] : 0.f;
+#pragma unroll
+      for (int i = 0; i < SI; ++i)
+        fi[i][u] = row >= 0 && i0 + i * 16 + (l & 15) < a.K ? x[row * a.x_stride + i * 16] : 0.f;
+    }
+  };
+  auto products = [&](const f32x4 (&fj)[SJ], const f32x4 (&fi)[SI]) {
+#pragma unroll
+    for (int j = 0; j < SJ; ++j) {
+#pragma unroll
+      for (int i = 0; i < SI; ++i)
+        acc[j][i] = ll_mma<float>(__builtin_bit_cast(uint4, fi[i]),
+                                  __builtin_bit_cast(uint4, fj[j]), acc[j][i]);
+      sum[j] += ((double)fj[j][0] + fj[j][1]) + ((double)fj[j][2] + fj[j][3]);
+    }
+  };
+  constexpr int kTurn = 16 * kLlWaves;
+  f32x4 fj0[SJ], fi0[SI], fj1[SJ], fi1[SI];
+  int p = 16 * w;
+  load(p, fj0, fi0);
+  for (; p < rows; p += 2 * kTurn) {
+    load(p + kTurn, fj1, fi1);
+    products(fj0, fi0);
+    load(p + 2 * kTurn, fj0, fi0);
+    products(fj1, fi1);
+  }
+  // waves 2, 3 hand theirs to 0, 1, then 1 to 0
+#pragma unroll
+  for (int half = 2; half > 0; half >>= 1) {
+    if (w >= half && w < 2 * half) {
+#pragma unroll
+      for (int j = 0; j < SJ; ++j)
+#pragma unroll
+        for (int i = 0; i < SI; ++i) s_acc[w - half][j * SI + i][l] = acc[j][i];
+    }
+    __syncthreads();
+    if (w < half) {
+#pragma unroll
+      for (int j = 0; j < SJ; ++j)
+#pragma unroll
+        for (int i = 0; i < SI; ++i) acc[j][i] += s_acc[w][j * SI + i][l];
+    }
+    __syncthreads();
+  }
+  if (a.db != nullptr && i0 == 0) {
+#pragma unroll
+    for (int j = 0; j < SJ; ++j) {
+      sum[j] += __shfl_xor(sum[j], 16, kWave);
+      sum[j] += __shfl_xor(sum[j], 32, kWave);
+      if (l < 16) s_b[w][j * 16 + l] = sum[j];
+    }
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (c < SJ * 16 && j0 + c < a.N) {
+      ll_store_sum<float>(a, unit, j0 + c, (s_b[0][c] + s_b[1][c]) + (s_b[2][c] + s_b[3][c]));
+    }
+  }
+  if (w == 0) ll_grad_store<float, SJ, SI>(acc, a, unit, j0, i0);
+}
+
+// Adds the partial matrices of the leaves with more than `run` rows, in 64 bits for f32 (and their
+// partial sums of dy, where the kernel above made them): one block per chunk in which such a leaf
+// starts and per 4 * kLlThreads elements.
 template <typename T>
 __global__ __launch_bounds__(kLlThreads) void ll_join_kernel(LlGrad a, int64_t blocks_per_chunk,
                                                              int64_t chunks) {
@@ -904,13 +1185,37 @@ __global__ __launch_bounds__(kLlThreads) void ll_join_kernel(LlGrad a, int64_t b
   const int64_t s1 = a.off[k1], e1 = a.off[k1 + 1];
   if (s1 < ca || e1 - s1 <= a.run) return;
   const int64_t size = (int64_t)a.N * a.K;
-  const int64_t e = (blk % blocks_per_chunk) * kLlThreads + threadIdx.x;
-  if (e >= size) return;
   const int64_t last = (e1 - 1) / a.run;
-  A sum = 0;
-  for (int64_t p = c; p <= last; ++p)
-    sum += (A)a.part[(2 * p + (p == c && k1 != k0 ? 1 : 0)) * size + e];
-  ((T*)a.dw)[k1 * size + e] = leaf_from<T>((float)sum);
+  const int64_t slot0 = 2 * c + (k1 != k0 ? 1 : 0);
+  const int64_t e = ((blk % blocks_per_chunk) * kLlThreads + threadIdx.x) * 4;
+  if (size % 4 == 0) {
+    if (e < size) {
+      A sum[4] = {};
+      for (int64_t p = c; p <= last; ++p) {
+        const f32x4 v = *(const f32x4*)(a.part + (p == c ? slot0 : 2 * p) * size + e);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum[u] += (A)v[u];
+      }
+      LeafVec<T, 4> o;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) o.v[u] = leaf_from<T>((float)sum[u]);
+      *(LeafVec<T, 4>*)((T*)a.dw + k1 * size + e) = o;
+    }
+  } else {
+    for (int u = 0; u < 4 && e + u < size; ++u) {
+      A sum = 0;
+      for (int64_t p = c; p <= last; ++p)
+        sum += (A)a.part[(p == c ? slot0 : 2 * p) * size + e + u];
+      ((T*)a.dw)[k1 * size + e + u] = leaf_from<T>((float)sum);
+    }
+  }
+  if (a.db != nullptr && blk % blocks_per_chunk == 0) {
+    for (int n = threadIdx.x; n < a.N; n += kLlThreads) {
+      double sum = 0;
+      for (int64_t p = c; p <= last; ++p) sum += a.part_b[(p == c ? slot0 : 2 * p) * a.N + n];
+      ((T*)a.db)[k1 * a.N + n] = leaf_from<T>((float)sum);
+    }
+  }
 }
 
 // ---- forward of at most 64 rows, straight from the leaf indices (no route). Each wave holds all of
@@ -1033,6 +1338,8 @@ void launch_leaf_linear_small(hipStream_t s, int type, const void* x, int64_t x_
   });
 }
 
+static bool ll_short_rows(int depth_bytes, int cols) { return depth_bytes <= 256 && cols <= 128; }
+
 // scratch for the tile list
 int64_t leaf_linear_tile_bytes(int64_t n, int G) {
   return n / G >= kLlBigRows ? 8 + 8 * ((n >> 8) + G + 1) : 0;
@@ -1072,7 +1379,30 @@ void launch_leaf_linear_tile(hipStream_t s, int type, bool dx, const void* src, 
                      (n >> 8) * ((a.cols + kBig - 1) / kBig) >= 512 &&
                      n * src_stride * (int64_t)sizeof(T) < (1ll << 32) &&
                      a.w_stride * (int64_t)sizeof(T) < (1ll << 32);
-    if (a.cols <= 16)
+    if (ll_short_rows(a.depth * (int)sizeof(T), a.cols)) {
+      // (a.cols <= 16: one fragment of columns; else four)
+      const int si = a.cols <= 16 ? 1 : 4;
+      a.col_tiles = (a.cols + si * 16 - 1) / (si * 16);
+      a.tiles = ((n >> kRowsShift) + G + 1) * a.col_tiles;
+      auto rows = [&](auto steps, auto cols) {
+        auto run = [&](auto kern) {
+          hipLaunchKernelGGL(kern, leaf_grid((a.tiles + kLlWaves - 1) / kLlWaves), dim3(kLlThreads),
+                             0, s, a);
+          MT_HIP_CHECK(hipGetLastError());
+        };
+        if (dx)
+          al ? run(ll_rows_kernel<T, true, steps(), cols(), true>)
+             : run(ll_rows_kernel<T, true, steps(), cols(), false>);
+        else
+          al ? run(ll_rows_kernel<T, false, steps(), cols(), true>)
+             : run(ll_rows_kernel<T, false, steps(), cols(), false>);
+      };
+      const bool half = a.depth * (int)sizeof(T) <= 128;
+      if (si == 1)
+        half ? rows(LlInt<2>{}, LlInt<1>{}) : rows(LlInt<4>{}, LlInt<1>{});
+      else
+        half ? rows(LlInt<2>{}, LlInt<4>{}) : rows(LlInt<4>{}, LlInt<4>{});
+    } else if (a.cols <= 16)
       go(LlInt<64>{}, LlInt<16>{}, LlInt<4>{}, LlInt<4>{});
     else if (mean < 32)
       go(LlInt<16>{}, LlInt<64>{}, LlInt<1>{}, LlInt<4>{});
@@ -1099,12 +1429,12 @@ void launch_leaf_linear_tile(hipStream_t s, int type, bool dx, const void* src, 
   });
 }
 
-// Rows a dW unit may have, a power of two: so many that about 1024 to 2048 tiles run at once, and
+// Rows a dW unit may have, a power of two: so many that about 512 to 1024 tiles run at once, and
 // where whole leaves are that many already, four times the mean leaf, so that only leaves far above
 // it are cut (a cut costs a partial matrix in 32 bits, written and read).
 static int64_t ll_grad_run(int64_t n, int G, int64_t tiles) {
   int64_t run = 256;
-  while (run < (1 << 20) && n / run * tiles > 2048) run <<= 1;
+  while (run < (1 << 20) && n / run * tiles > 1024) run <<= 1;
   if (G * tiles >= 1024)
     while (run < 4 * (n / G)) run <<= 1;
   return run;
@@ -1120,7 +1450,10 @@ static int64_t ll_grad_tiles(int b, int K, int N) {
   return (int64_t)((N + b - 1) / b) * ((K + b - 1) / b);
 }
 
-// scratch for the partial matrices, whichever tile is taken
+// f32 with few columns on either side: ll_rows_grad_kernel
+static bool ll_short_grad(int type, int K, int N) { return type == kLeafF32 && K <= 32 && N <= 16; }
+
+// scratch for the partial matrices (and sums), whichever tile is taken
 int64_t leaf_linear_grad_bytes(int type, int64_t n, int G, int K, int N) {
   int64_t chunks = 0;
   for (bool direct : {false, true}) {
@@ -1128,13 +1461,14 @@ int64_t leaf_linear_grad_bytes(int type, int64_t n, int G, int K, int N) {
     const int64_t run = ll_grad_run(n, G, ll_grad_tiles(b, K, N));
     if (n > run) chunks = std::max(chunks, (n + run - 1) / run);
   }
-  return 2 * chunks * (int64_t)N * K * 4;
+  return 2 * chunks * ((int64_t)N * K * 4 + 8 * N + 8);
 }
 
-void launch_leaf_linear_grad(hipStream_t s, int type, const void* x, int64_t x_stride,
+// dW, and db where it is asked for (not null); true: db was made
+bool launch_leaf_linear_grad(hipStream_t s, int type, const void* x, int64_t x_stride,
                              const void* dy, int64_t dy_stride, const int32_t* order,
                              const uint32_t* keys, const int32_t* off, int64_t n, int G, int K,
-                             int N, void* dw, void* work) {
+                             int N, void* dw, void* db, void* work) {
   LlGrad a{};
   a.x = x, a.dy = dy, a.dw = dw, a.part = (float*)work;
   a.order = order, a.keys = keys, a.off = off;
@@ -1157,22 +1491,27 @@ void launch_leaf_linear_grad(hipStream_t s, int type, const void* x, int64_t x_s
       MT_HIP_CHECK(hipGetLastError());
     };
     const int64_t all = a.units * tiles;
-    if (b == kBig) {
+    if (b != kBig) a.db = db;
+    a.part_b = (double*)((char*)work + (2 * chunks * (int64_t)N * K * 4 + 7) / 8 * 8);
+    if (ll_short_grad(type, K, N)) {
+      if constexpr (sizeof(T) == 4) run(ll_rows_grad_kernel<1, 2>, all, kLlThreads);
+    } else if (b == kBig) {
       if constexpr (sizeof(T) == 2) run(ll_big_grad_kernel<T>, ll_xcd_blocks(all), kBigThreads);
     } else if (b == 128) {
-      al ? run(ll_grad_kernel<T, 128, 128, 2, true>, all, kLlThreads)
-         : run(ll_grad_kernel<T, 128, 128, 2, false>, all, kLlThreads);
+      al ? run(ll_grad_kernel<T, 128, true>, all, kLlThreads)
+         : run(ll_grad_kernel<T, 128, false>, all, kLlThreads);
     } else {
-      al ? run(ll_grad_kernel<T, 64, 64, 2, true>, all, kLlThreads)
-         : run(ll_grad_kernel<T, 64, 64, 2, false>, all, kLlThreads);
+      al ? run(ll_grad_kernel<T, 64, true>, all, kLlThreads)
+         : run(ll_grad_kernel<T, 64, false>, all, kLlThreads);
     }
     if (chunks > 0) {
-      const int64_t per = ((int64_t)N * K + kLlThreads - 1) / kLlThreads;
+      const int64_t per = ((int64_t)N * K + 4 * kLlThreads - 1) / (4 * kLlThreads);
       hipLaunchKernelGGL(ll_join_kernel<T>, leaf_grid(chunks * per), dim3(kLlThreads), 0, s, a, per,
                          chunks);
       MT_HIP_CHECK(hipGetLastError());
     }
   });
+  return a.db != nullptr;
 }
 
 }  // namespace mt

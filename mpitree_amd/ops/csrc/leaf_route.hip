@@ -20,8 +20,8 @@
 
 namespace mt {
 
-constexpr int kLrThreads = 512;
-constexpr int kLrItems = 8;
+constexpr int kLrThreads = 1024;
+constexpr int kLrItems = 4;
 constexpr int kLrTile = kLrThreads * kLrItems;  // 4096 rows
 constexpr int kLrWaves = kLrThreads / kWave;
 constexpr int kLrSelfTiles = 512;
@@ -44,7 +44,7 @@ __device__ __forceinline__ unsigned long long lr_match(uint32_t d, bool in) {
   return m;
 }
 
-// Ranks the tile's keys by digit. Item k of lane l of wave w is tile entry w * 512 + k * 64 + l.
+// Ranks the tile's keys by digit. Item k of lane l of wave w is tile entry w * 256 + k * 64 + l.
 // On return rk holds each item's rank among the wave's equal digits, s_wh the waves' counts.
 __device__ __forceinline__ void lr_rank(const uint32_t (&key)[kLrItems], uint32_t (&rk)[kLrItems],
                                         int cnt, int shift, uint32_t (*s_wh)[256]) {
@@ -163,13 +163,18 @@ __global__ __launch_bounds__(kLrThreads) void lr_count_kernel(const void* __rest
                                                               int64_t n, int G, int shift,
                                                               uint32_t* __restrict__ counts) {
   __shared__ uint32_t s_wh[kLrWaves][256];
+  const int w = threadIdx.x / kWave;
   for (int i = threadIdx.x; i < kLrWaves * 256; i += kLrThreads) (&s_wh[0][0])[i] = 0u;
   const int64_t p0 = (int64_t)blockIdx.x * kLrTile;
   const int cnt = (int)min<int64_t>(kLrTile, n - p0);
-  uint32_t key[kLrItems], rk[kLrItems];
+  uint32_t key[kLrItems];
   lr_load<kFirst>(ids, wide, kin, p0, cnt, G, key);
   __syncthreads();
-  lr_rank(key, rk, cnt, shift, s_wh);
+  // counts alone do not depend on the order of these adds
+#pragma unroll
+  for (int k = 0; k < kLrItems; ++k)
+    if (w * (kWave * kLrItems) + k * kWave + lane_id() < cnt)
+      atomicAdd(&s_wh[w][(key[k] >> shift) & 255u], 1u);
   __syncthreads();
   if (threadIdx.x < 256) {
     uint32_t s = 0;
@@ -226,7 +231,7 @@ __global__ __launch_bounds__(kLrThreads) void lr_scatter_kernel(
       row[k] = i < cnt ? rin[p0 + i] : 0u;
   }
   if constexpr (kSelf) {
-    // wave w sums the counts of tiles w, w + 8, ...: four digits a lane
+    // wave w sums the counts of tiles w, w + 16, ...: four digits a lane
     uint4 pre = make_uint4(0, 0, 0, 0), tot = make_uint4(0, 0, 0, 0);
 #pragma unroll 4
     for (int t = w; t < T; t += kLrWaves) {
