@@ -25,8 +25,6 @@ plain path of the same results.
 
 from __future__ import annotations
 
-from contextlib import nullcontext
-
 import torch
 
 from . import native
@@ -115,24 +113,22 @@ def _check_device(first, *others):
             raise ValueError(f"operands on different devices: {first.device}, {t.device}")
 
 
-def _on(device):
-    """A context with ``device`` current (launches go to the current device)."""
-    if device.index == torch.cuda.current_device():
-        return nullcontext()
-    return torch.cuda.device(device)
+def _stream(dev: int) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
 
 
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+# (the same handle without a Stream object around it, where this torch has it: 1.7 us a call)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream)
 
 
-def _scratch(nbytes: int, device) -> torch.Tensor:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
+    return like.new_empty(nbytes, dtype=torch.uint8)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., C] as [rows, C] with unit column stride (any row stride)."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:  # (a view would be one more node for autograd to walk)
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 and t.stride(0) >= 0 else t.contiguous()
 
 
@@ -142,20 +138,18 @@ def leaf_route(leaves: torch.Tensor, n_leaves: int) -> LeafRoute:
     leaves = _check_leaves(leaves)
     n_leaves = _check_n_leaves(n_leaves)
     ids = leaves.detach().reshape(-1)
-    n, dev = ids.numel(), ids.device
+    n = ids.numel()
     if not ids.is_cuda:
         key = torch.where((ids >= 0) & (ids < n_leaves), ids, n_leaves).to(torch.int64)
         key, order = torch.sort(key, stable=True)
         bounds = torch.arange(n_leaves + 1, dtype=torch.int64)
         offsets = torch.cat([torch.searchsorted(key, bounds), torch.tensor([n])])
         return LeafRoute(leaves, n_leaves, torch.cat([order, key, offsets]).int())
-    hip = native.hip()
-    with _on(dev):
-        ids = ids.contiguous()
-        buf = torch.empty(hip.leaf_route_len(n, n_leaves), dtype=torch.int32, device=dev)
-        work = _scratch(4 * hip.leaf_route_words(n, n_leaves), dev)
-        hip.leaf_route(_stream(ids), ids.data_ptr(), ids.dtype == torch.int64, n, n_leaves,
-                       buf.data_ptr(), work.data_ptr())
+    hip, dev, ids = native.hip(), ids.get_device(), ids.contiguous()
+    buf = ids.new_empty(hip.leaf_route_len(n, n_leaves), dtype=torch.int32)
+    work = _scratch(4 * hip.leaf_route_words(n, n_leaves), ids)
+    hip.leaf_route(dev, _stream(dev), ids.data_ptr(), ids.dtype == torch.int64, n, n_leaves,
+                   buf.data_ptr(), work.data_ptr())
     return LeafRoute(leaves, n_leaves, buf)
 
 
@@ -167,14 +161,13 @@ def _embed_forward(ids: torch.Tensor, table: torch.Tensor, scale: float) -> torc
         has = (flat >= 0) & (flat < table.shape[0])
         y = table[torch.where(has, flat, 0)].float() * scale
         return torch.where(has[:, None], y, 0.0).to(table.dtype).reshape(*ids.shape, D)
-    y = torch.empty((*ids.shape, D), dtype=table.dtype, device=ids.device)
-    if table.stride(1) != 1 and D > 1:
+    y = table.new_empty((*ids.shape, D))
+    if D > 1 and table.stride(1) != 1:
         table = table.contiguous()
-    ids = ids.contiguous()
-    with _on(ids.device):
-        native.hip().leaf_embed(_stream(ids), _TYPES[table.dtype], ids.data_ptr(),
-                                ids.dtype == torch.int64, table.data_ptr(), table.stride(0),
-                                ids.numel(), table.shape[0], D, scale, y.data_ptr())
+    ids, dev = ids.contiguous(), table.get_device()
+    native.hip().leaf_embed(dev, _stream(dev), _TYPES[table.dtype], ids.data_ptr(),
+                            ids.dtype == torch.int64, table.data_ptr(), table.stride(0),
+                            ids.numel(), table.shape[0], D, scale, y.data_ptr())
     return y
 
 
@@ -191,16 +184,14 @@ def _embed_grad(dy, ids, route, n_leaves: int, scale: float) -> torch.Tensor:
     if not dy.is_cuda:
         route = route if route is not None else leaf_route(ids, n_leaves)
         return _sum_by_leaf_plain(dy.reshape(-1, D), route, scale)
-    hip, kind, dev = native.hip(), _TYPES[dy.dtype], dy.device
-    with _on(dev):
-        dy, ids = _rows(dy), ids.contiguous()
-        n = dy.shape[0]
-        out = torch.empty((n_leaves, D), dtype=dy.dtype, device=dev)
-        work = _scratch(hip.leaf_embed_grad_bytes(kind, n, n_leaves, D, route is not None), dev)
-        hip.leaf_embed_grad(_stream(dy), kind, dy.data_ptr(), dy.stride(0), ids.data_ptr(),
-                            ids.dtype == torch.int64,
-                            0 if route is None else route._buf.data_ptr(), n, n_leaves, D, scale,
-                            out.data_ptr(), work.data_ptr())
+    hip, kind, dev = native.hip(), _TYPES[dy.dtype], dy.get_device()
+    dy, ids = _rows(dy), ids.contiguous()
+    n = dy.shape[0]
+    out = dy.new_empty((n_leaves, D))
+    work = _scratch(hip.leaf_embed_grad_bytes(kind, n, n_leaves, D, route is not None), dy)
+    hip.leaf_embed_grad(dev, _stream(dev), kind, dy.data_ptr(), dy.stride(0), ids.data_ptr(),
+                        ids.dtype == torch.int64, 0 if route is None else route._buf.data_ptr(), n,
+                        n_leaves, D, scale, out.data_ptr(), work.data_ptr())
     return out
 
 
@@ -212,10 +203,16 @@ class _Embedding(torch.autograd.Function):
         return _embed_forward(ids, table, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
+    def _first(ctx, dy):
         (ids,) = ctx.saved_tensors
         return _embed_grad(dy, ids, ctx.route, ctx.n_leaves, ctx.scale), None, None, None
+
+    _marked = torch.autograd.function.once_differentiable(_first.__func__)
+
+    @staticmethod
+    def backward(ctx, dy):
+        # (with create_graph only: the marking costs 4 us)
+        return (_Embedding._marked if torch.is_grad_enabled() else _Embedding._first)(ctx, dy)
 
 
 def leaf_embedding(leaves, table: torch.Tensor, *, scale: float = 1.0) -> torch.Tensor:
@@ -272,39 +269,35 @@ def _linear_forward(x, ids, route, w, b):
     if not x.is_cuda:
         route = route if route is not None else leaf_route(ids, G)
         return _linear_plain(x, route, w, b), route
-    hip, kind, dev = native.hip(), _TYPES[x.dtype], x.device
-    with _on(dev):
-        ids = ids.contiguous()
-        wide, bias = ids.dtype == torch.int64, 0 if b is None else b.data_ptr()
-        y = torch.empty((n, N), dtype=x.dtype, device=dev)
-        if n <= hip.leaf_linear_small_rows():
-            hip.leaf_linear_small(_stream(x), kind, x.data_ptr(), x.stride(0), ids.data_ptr(), wide,
-                                  n, G, w.data_ptr(), bias, K, N, y.data_ptr())
-            return y, route
-        work = _scratch(hip.leaf_linear_bytes(n, G), dev)
-        sort = 0
-        if route is None:
-            sort = ids.data_ptr()
-            buf = torch.empty(hip.leaf_route_len(n, G), dtype=torch.int32, device=dev)
-            route = LeafRoute(ids, G, buf)
-        hip.leaf_linear(_stream(x), kind, x.data_ptr(), x.stride(0), sort, wide,
-                        route._buf.data_ptr(), n, G, w.data_ptr(), bias, K, N, y.data_ptr(),
-                        work.data_ptr())
+    hip, kind, dev, ids = native.hip(), _TYPES[x.dtype], x.get_device(), ids.contiguous()
+    wide, bias = ids.dtype == torch.int64, 0 if b is None else b.data_ptr()
+    y = x.new_empty((n, N))
+    if n <= hip.leaf_linear_small_rows():
+        hip.leaf_linear_small(dev, _stream(dev), kind, x.data_ptr(), x.stride(0), ids.data_ptr(),
+                              wide, n, G, w.data_ptr(), bias, K, N, y.data_ptr())
+        return y, route
+    work = _scratch(hip.leaf_linear_bytes(n, G), x)
+    sort = 0
+    if route is None:
+        sort = ids.data_ptr()
+        route = LeafRoute(ids, G, ids.new_empty(hip.leaf_route_len(n, G), dtype=torch.int32))
+    hip.leaf_linear(dev, _stream(dev), kind, x.data_ptr(), x.stride(0), sort, wide,
+                    route._buf.data_ptr(), n, G, w.data_ptr(), bias, K, N, y.data_ptr(),
+                    work.data_ptr())
     return y, route
 
 
 def _linear_grad(dy, x, route, w, need_x, need_w, need_b):
     n, (G, N, K) = x.shape[0], w.shape
-    hip, kind, dev = native.hip(), _TYPES[x.dtype], x.device
-    with _on(dev):
-        dy = _rows(dy)
-        dx, dw, db = (torch.empty(shape, dtype=x.dtype, device=dev) if need else None
-                      for need, shape in ((need_x, (n, K)), (need_w, (G, N, K)), (need_b, (G, N))))
-        work = _scratch(hip.leaf_linear_grad_bytes(kind, n, G, K, N), dev)
-        hip.leaf_linear_grad(_stream(x), kind, x.data_ptr(), x.stride(0), dy.data_ptr(),
-                             dy.stride(0), route._buf.data_ptr(), n, G, w.data_ptr(), K, N,
-                             *(0 if t is None else t.data_ptr() for t in (dx, dw, db)),
-                             work.data_ptr())
+    hip, kind, dev, dy = native.hip(), _TYPES[x.dtype], x.get_device(), _rows(dy)
+    dx = x.new_empty((n, K)) if need_x else None
+    dw = x.new_empty((G, N, K)) if need_w else None
+    db = x.new_empty((G, N)) if need_b else None
+    work = _scratch(hip.leaf_linear_grad_bytes(kind, n, G, K, N), x)
+    hip.leaf_linear_grad(dev, _stream(dev), kind, x.data_ptr(), x.stride(0), dy.data_ptr(),
+                         dy.stride(0), route._buf.data_ptr(), n, G, w.data_ptr(), K, N,
+                         *(0 if t is None else t.data_ptr() for t in (dx, dw, db)),
+                         work.data_ptr())
     return dx, dw, db
 
 
@@ -316,8 +309,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
+    def _first(ctx, dy):
         x, w, ids = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         route = ctx.route if ctx.route is not None else leaf_route(ids, w.shape[0])
@@ -327,6 +319,12 @@ class _Linear(torch.autograd.Function):
             grads = _linear_plain_grad(dy, x, route, w, need_x, need_w)
             grads += (_sum_by_leaf_plain(dy, route, 1.0) if need_b else None,)
         return (*grads, None, None)
+
+    _marked = torch.autograd.function.once_differentiable(_first.__func__)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return (_Linear._marked if torch.is_grad_enabled() else _Linear._first)(ctx, dy)
 
 
 def leaf_linear(inputs: torch.Tensor, leaves, weight: torch.Tensor, bias=None) -> torch.Tensor:
@@ -354,10 +352,11 @@ def leaf_linear(inputs: torch.Tensor, leaves, weight: torch.Tensor, bias=None) -
             raise ValueError(f"bias has shape {tuple(bias.shape)}, expected {(G, N)}")
         bias = bias.contiguous()
     _check_device(inputs, ids, weight, bias)
-    x, weight, flat = _rows(inputs), weight.contiguous(), ids.reshape(-1)
+    x, weight = _rows(inputs), weight.contiguous()
+    flat = ids if ids.dim() == 1 else ids.reshape(-1)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                     or bias is not None and bias.requires_grad):
         y = _Linear.apply(x, weight, bias, flat, route)
     else:
         y = _linear_forward(x, flat, route, weight, bias)[0]
-    return y.reshape(*ids.shape, N)
+    return y if ids.dim() == 1 else y.reshape(*ids.shape, N)
