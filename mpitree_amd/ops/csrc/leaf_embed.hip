@@ -18,8 +18,11 @@
 namespace mt {
 
 constexpr int kLeThreads = 256;
-constexpr int kLeUnroll = 4;  // rows of a group in flight: forward,
-constexpr int kLeBatch = 8;   // and gradient
+// Rows of a group in flight. Each takes dependent loads (number, row), so narrow vectors need more
+// rows: forward 4 of 16 bytes a lane, 16 of less (63 columns of f32: 86 -> XX us with 16);
+constexpr int le_unroll(int bytes) { return bytes >= 16 ? 4 : 16; }
+// gradient 8 and 16.
+constexpr int le_batch(int bytes) { return bytes >= 16 ? 8 : 16; }
 constexpr int kLeEmpty = 16;  // leaves that a group looks over for missing rows
 
 template <typename T>
@@ -37,35 +40,52 @@ struct LeCols {
   int col_blocks;  // column blocks of tpr * NC * W columns
 };
 
-template <typename T, int W, int NC, bool kScale, bool kWide>
+// kWave: a row's group is a whole wave, so the row's number and address are scalars (63 columns of
+// f32: the 64-bit address arithmetic of every lane bound the kernel before).
+template <bool kWave>
+__device__ __forceinline__ int32_t le_same(int32_t v) {
+  return kWave ? __builtin_amdgcn_readfirstlane(v) : v;
+}
+template <bool kWave>
+__device__ __forceinline__ int64_t le_same(int64_t v) {
+  if constexpr (!kWave) return v;
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)v >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
+template <typename T, int W, int NC, bool kScale, bool kWide, bool kWave>
 __global__ __launch_bounds__(kLeThreads) void le_forward_kernel(
     const void* __restrict__ ids, const T* __restrict__ table, int64_t stride, int64_t n,
     int64_t V, int D, float scale, LeCols lc, T* __restrict__ y) {
+  constexpr int kUnroll = le_unroll(W * (int)sizeof(T));
   const int tpr = 1 << lc.tpr_shift, rpb = kLeThreads >> lc.tpr_shift;
-  const int sub = threadIdx.x >> lc.tpr_shift, lr = threadIdx.x & (tpr - 1);
+  const int sub = le_same<kWave>((int32_t)(threadIdx.x >> lc.tpr_shift));
+  const int lr = threadIdx.x & (tpr - 1);
   const int64_t blk = leaf_block();
-  const int64_t r0 = (blk / lc.col_blocks) * (rpb * kLeUnroll) + sub;
+  const int64_t r0 = (blk / lc.col_blocks) * (rpb * kUnroll) + sub;
   const int c0 = ((int)(blk % lc.col_blocks) * NC * tpr + lr) * W;
-  int64_t id[kLeUnroll];
+  int64_t id[kUnroll];
 #pragma unroll
-  for (int u = 0; u < kLeUnroll; ++u) {
+  for (int u = 0; u < kUnroll; ++u) {
     const int64_t r = r0 + (int64_t)u * rpb;
     id[u] = -1;
     if (r < n) id[u] = kWide ? ((const int64_t*)ids)[r] : (int64_t)((const int32_t*)ids)[r];
+    id[u] = le_same<kWave>(id[u]);
   }
 #pragma unroll
   for (int q = 0; q < NC; ++q) {
     const int c = c0 + q * tpr * W;
     if (c >= D) break;
-    LeafVec<T, W> v[kLeUnroll];
+    LeafVec<T, W> v[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kLeUnroll; ++u) {
+    for (int u = 0; u < kUnroll; ++u) {
       v[u] = LeafVec<T, W>{};
       if ((uint64_t)id[u] < (uint64_t)V)
         v[u] = *(const LeafVec<T, W>*)(table + id[u] * stride + c);
     }
 #pragma unroll
-    for (int u = 0; u < kLeUnroll; ++u) {
+    for (int u = 0; u < kUnroll; ++u) {
       const int64_t r = r0 + (int64_t)u * rpb;
       if (r >= n) break;
       if constexpr (kScale) {
@@ -107,16 +127,19 @@ __device__ __forceinline__ void le_store(T* __restrict__ out, float scale, const
 
 // Blocks below `chunk_blocks`: a chunk of 1 << run_shift sorted positions for each group of lanes,
 // partial rows into `part` ([2 * chunks][D]: of the leaf that reaches into the chunk, of the one
-// that starts in it and reaches out). Blocks from there on: zeros for the leaves without rows.
-template <typename T, int W>
+// that starts in it and reaches out; open[chunk]: that one's number + 1, or 0). Blocks from there on: zeros for the leaves without rows.
+template <typename T, int W, bool kWave>
 __global__ __launch_bounds__(kLeThreads) void le_backward_kernel(
     const T* __restrict__ dy, int64_t stride, const int32_t* __restrict__ order,
     const uint32_t* __restrict__ keys, const int32_t* __restrict__ off, int64_t V, int D,
-    float scale, LeCols lc, int run_shift,
-    int64_t chunk_blocks, T* __restrict__ dtable, typename LeAcc<T>::type* __restrict__ part) {
+    float scale, LeCols lc, int run_shift, int64_t chunks, int64_t chunk_blocks,
+    T* __restrict__ dtable, typename LeAcc<T>::type* __restrict__ part,
+    uint32_t* __restrict__ open) {
   using A = typename LeAcc<T>::type;
+  constexpr int kBatch = le_batch(W * (int)sizeof(T));
   const int tpr = 1 << lc.tpr_shift, rpb = kLeThreads >> lc.tpr_shift;
-  const int sub = threadIdx.x >> lc.tpr_shift, lr = threadIdx.x & (tpr - 1);
+  const int sub = le_same<kWave>((int32_t)(threadIdx.x >> lc.tpr_shift));
+  const int lr = threadIdx.x & (tpr - 1);
   const int64_t blk = leaf_block();
   if (blk >= chunk_blocks) {
     const int64_t v0 = ((blk - chunk_blocks) * rpb + sub) * kLeEmpty;
@@ -135,28 +158,32 @@ __global__ __launch_bounds__(kLeThreads) void le_backward_kernel(
   const int64_t chunk = blk / lc.col_blocks * rpb + sub, m = off[V];
   const int c0 = ((int)(blk % lc.col_blocks) * tpr + lr) * W;
   const int64_t a = chunk << run_shift, b = min<int64_t>(a + (1 << run_shift), m);
-  if (a >= m || c0 >= D) return;
+  if (a >= m || c0 >= D) {
+    if (c0 == 0 && chunk < chunks) open[chunk] = 0;
+    return;
+  }
   const bool into = a > 0 && keys[a - 1] == keys[a];
   const bool out_of = b < m && keys[b] == keys[b - 1];
+  if (c0 == 0) open[chunk] = out_of && !(into && keys[a] == keys[b - 1]) ? keys[b - 1] + 1 : 0;
   A acc[W] = {};
-  uint32_t cur = keys[a];
+  uint32_t cur = (uint32_t)le_same<kWave>((int32_t)keys[a]);
   bool first = true;
   auto partial = [&](int which) {
     A* const to = part + (2 * chunk + which) * D + c0;
 #pragma unroll
     for (int e = 0; e < W; ++e) to[e] = acc[e];
   };
-  for (int64_t p = a; p < b; p += kLeBatch) {
-    uint32_t key[kLeBatch];
-    LeafVec<T, W> v[kLeBatch];
+  for (int64_t p = a; p < b; p += kBatch) {
+    uint32_t key[kBatch];
+    LeafVec<T, W> v[kBatch];
 #pragma unroll
-    for (int u = 0; u < kLeBatch; ++u) {
+    for (int u = 0; u < kBatch; ++u) {
       const int64_t pu = min(p + u, b - 1);
-      key[u] = keys[pu];
-      v[u] = *(const LeafVec<T, W>*)(dy + order[pu] * stride + c0);
+      key[u] = (uint32_t)le_same<kWave>((int32_t)keys[pu]);
+      v[u] = *(const LeafVec<T, W>*)(dy + le_same<kWave>(order[pu]) * stride + c0);
     }
 #pragma unroll
-    for (int u = 0; u < kLeBatch; ++u) {
+    for (int u = 0; u < kBatch; ++u) {
       if (p + u >= b) break;
       if (key[u] != cur) {
         if (first && into)
@@ -184,23 +211,22 @@ __global__ __launch_bounds__(kLeThreads) void le_backward_kernel(
 // it, and adds that leaf's partial rows.
 template <typename T, int W>
 __global__ __launch_bounds__(kLeThreads) void le_join_kernel(
-    const typename LeAcc<T>::type* __restrict__ part, const uint32_t* __restrict__ keys,
-    const int32_t* __restrict__ off, int64_t V, int D, float scale, LeCols lc, int run_shift,
+    const typename LeAcc<T>::type* __restrict__ part, const uint32_t* __restrict__ open,
+    const int32_t* __restrict__ off, int64_t chunks, int D, float scale, LeCols lc, int run_shift,
     T* __restrict__ dtable) {
   using A = typename LeAcc<T>::type;
   __shared__ A s_acc[W * kLeThreads / 2];
+  const int64_t blk = leaf_block(), chunk = blk / lc.col_blocks;
+  if (chunk >= chunks) return;
+  const uint32_t k = open[chunk] - 1;
+  if (k == 0xffffffffu) return;
   const int tpr = 1 << lc.tpr_shift, rpb = kLeThreads >> lc.tpr_shift;
   const int sub = threadIdx.x >> lc.tpr_shift, lr = threadIdx.x & (tpr - 1);
-  const int64_t blk = leaf_block(), chunk = blk / lc.col_blocks;
   const int c0 = ((int)(blk % lc.col_blocks) * tpr + lr) * W;
-  const int64_t m = off[V], a = chunk << run_shift, b = a + (1 << run_shift);
-  if (b >= m) return;
-  const uint32_t k = keys[b - 1];
-  if (keys[b] != k || off[k] < a) return;
   const int64_t last = (off[k + 1] - 1) >> run_shift;
   A acc[W] = {};
   if (c0 < D) {
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t p = chunk + sub; p <= last; p += rpb) {
       const A* const in = part + (2 * p + (p == chunk ? 1 : 0)) * D + c0;
 #pragma unroll
@@ -255,7 +281,7 @@ static void le_forward(hipStream_t s, const void* ids, bool wide, const T* table
   // wide rows: four vectors a lane while that leaves no lane idle
   const bool four = D >= 4 * kWave * W;
   const LeCols lc = le_cols(D, W, four ? 4 : 1);
-  const int rows = (kLeThreads >> lc.tpr_shift) * kLeUnroll;
+  const int rows = (kLeThreads >> lc.tpr_shift) * le_unroll(W * (int)sizeof(T));
   const dim3 grid = leaf_grid((n + rows - 1) / rows * lc.col_blocks);
   auto go = [&](auto kern) {
     hipLaunchKernelGGL(kern, grid, dim3(kLeThreads), 0, s, ids, table, stride, n, V, D, scale, lc,
@@ -263,11 +289,14 @@ static void le_forward(hipStream_t s, const void* ids, bool wide, const T* table
     MT_HIP_CHECK(hipGetLastError());
   };
   if (four)
-    wide ? go(le_forward_kernel<T, W, 4, kScale, true>)
-         : go(le_forward_kernel<T, W, 4, kScale, false>);
+    wide ? go(le_forward_kernel<T, W, 4, kScale, true, true>)
+         : go(le_forward_kernel<T, W, 4, kScale, false, true>);
+  else if (lc.tpr_shift == 6)
+    wide ? go(le_forward_kernel<T, W, 1, kScale, true, true>)
+         : go(le_forward_kernel<T, W, 1, kScale, false, true>);
   else
-    wide ? go(le_forward_kernel<T, W, 1, kScale, true>)
-         : go(le_forward_kernel<T, W, 1, kScale, false>);
+    wide ? go(le_forward_kernel<T, W, 1, kScale, true, false>)
+         : go(le_forward_kernel<T, W, 1, kScale, false, false>);
 }
 
 void launch_leaf_embed(hipStream_t s, int type, const void* ids, bool wide, const void* table,
@@ -309,7 +338,7 @@ static int le_run_shift(int64_t n, const LeCols& lc) {
 int64_t leaf_embed_grad_bytes(int type, int64_t n, int D) {
   int shift = 8;
   for (int W : {8, 4, 2, 1}) shift = std::min(shift, le_run_shift(n, le_cols(D, W, 1)));
-  return 2 * ((n >> shift) + 1) * D * (type == kLeafF32 ? 8 : 4);
+  return ((n >> shift) + 1) * (2 * (int64_t)D * (type == kLeafF32 ? 8 : 4) + 4);
 }
 
 template <typename T, int W>
@@ -322,13 +351,17 @@ static void le_backward(hipStream_t s, const T* dy, int64_t stride, const int32_
   const int64_t chunks = (n + (1 << shift) - 1) >> shift;
   const int64_t chunk_blocks = (chunks + rpb - 1) / rpb * lc.col_blocks;
   const int64_t empty = (V + rpb * kLeEmpty - 1) / (rpb * kLeEmpty);
-  hipLaunchKernelGGL((le_backward_kernel<T, W>), leaf_grid(chunk_blocks + empty), dim3(kLeThreads), 0,
-                     s, dy, stride, order, keys, off, V, D, scale, lc, shift, chunk_blocks, dtable,
-                     (A*)work);
-  MT_HIP_CHECK(hipGetLastError());
+  A* const part = (A*)work;
+  uint32_t* const open = (uint32_t*)(part + 2 * chunks * D);
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, leaf_grid(chunk_blocks + empty), dim3(kLeThreads), 0, s, dy, stride, order,
+                       keys, off, V, D, scale, lc, shift, chunks, chunk_blocks, dtable, part, open);
+    MT_HIP_CHECK(hipGetLastError());
+  };
+  lc.tpr_shift == 6 ? go(le_backward_kernel<T, W, true>) : go(le_backward_kernel<T, W, false>);
   if (chunks > 1) {
     hipLaunchKernelGGL((le_join_kernel<T, W>), leaf_grid((chunks - 1) * lc.col_blocks),
-                       dim3(kLeThreads), 0, s, (const A*)work, keys, off, V, D, scale, lc, shift,
+                       dim3(kLeThreads), 0, s, part, open, off, chunks - 1, D, scale, lc, shift,
                        dtable);
     MT_HIP_CHECK(hipGetLastError());
   }

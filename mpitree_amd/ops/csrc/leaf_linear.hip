@@ -1380,8 +1380,7 @@ void launch_leaf_linear_tile(hipStream_t s, int type, bool dx, const void* src, 
                      n * src_stride * (int64_t)sizeof(T) < (1ll << 32) &&
                      a.w_stride * (int64_t)sizeof(T) < (1ll << 32);
     if (ll_short_rows(a.depth * (int)sizeof(T), a.cols)) {
-      // (a.cols <= 16: one fragment of columns; else four)
-      const int si = a.cols <= 16 ? 1 : 4;
+      const int si = a.cols <= 16 ? 1 : a.cols <= 32 ? 2 : 4;  // fragments of columns a wave holds
       a.col_tiles = (a.cols + si * 16 - 1) / (si * 16);
       a.tiles = ((n >> kRowsShift) + G + 1) * a.col_tiles;
       auto rows = [&](auto steps, auto cols) {
@@ -1398,10 +1397,10 @@ void launch_leaf_linear_tile(hipStream_t s, int type, bool dx, const void* src, 
              : run(ll_rows_kernel<T, false, steps(), cols(), false>);
       };
       const bool half = a.depth * (int)sizeof(T) <= 128;
-      if (si == 1)
-        half ? rows(LlInt<2>{}, LlInt<1>{}) : rows(LlInt<4>{}, LlInt<1>{});
-      else
-        half ? rows(LlInt<2>{}, LlInt<4>{}) : rows(LlInt<4>{}, LlInt<4>{});
+      auto steps = [&](auto cols) {
+        half ? rows(LlInt<2>{}, cols) : rows(LlInt<4>{}, cols);
+      };
+      si == 1 ? steps(LlInt<1>{}) : si == 2 ? steps(LlInt<2>{}) : steps(LlInt<4>{});
     } else if (a.cols <= 16)
       go(LlInt<64>{}, LlInt<16>{}, LlInt<4>{}, LlInt<4>{});
     else if (mean < 32)
