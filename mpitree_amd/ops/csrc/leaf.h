@@ -13,7 +13,7 @@
 namespace mt {
 
 // element types as the bindings number them
-enum LeafType { kLeafF32 = 0, kLeafF16 = 1, kLeafBF16 = 2, kLeafRaw32 = 3 };
+enum LeafType { kLeafF32 = 0, kLeafF16 = 1, kLeafBF16 = 2 };
 
 // A launch of `total` blocks of 256 threads: HIP's limit is 2^32 threads in a grid's x, so
 // more blocks go to y; kernels number them with leaf_block() and leave past `total`.

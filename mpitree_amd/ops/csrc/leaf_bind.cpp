@@ -68,8 +68,8 @@ int64_t pad16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 void bind_leaf(py::module_& m) {
   m.def("leaf_route_len", &route_len);      // int32 words of a route
   m.def("leaf_route_words", &leaf_route_words);  // ... of the scratch of its sort
-  m.def("leaf_route", [](int dev, uintptr_t s, uintptr_t ids, bool wide, int64_t n, int G, uintptr_t buf,
-                         uintptr_t work) {
+  m.def("leaf_route", [](int dev, uintptr_t s, uintptr_t ids, bool wide, int64_t n, int G,
+                         uintptr_t buf, uintptr_t work) {
     const OnDevice on(dev);
     const Route r(buf, n);
     launch_leaf_route(S(s), P<void>(ids), wide, n, G, r.order, r.keys, r.off, P<uint32_t>(work));
@@ -85,9 +85,9 @@ void bind_leaf(py::module_& m) {
     return leaf_embed_grad_bytes(type, n, D) +
            (routed ? 0 : pad16(4 * leaf_route_words(n, G)) + pad16(4 * route_len(n, G)));
   });
-  m.def("leaf_embed_grad", [](int dev, uintptr_t s, int type, uintptr_t dy, int64_t dy_stride, uintptr_t ids,
-                              bool wide, uintptr_t route, int64_t n, int G, int D, float scale,
-                              uintptr_t dtable, uintptr_t work) {
+  m.def("leaf_embed_grad", [](int dev, uintptr_t s, int type, uintptr_t dy, int64_t dy_stride,
+                              uintptr_t ids, bool wide, uintptr_t route, int64_t n, int G, int D,
+                              float scale, uintptr_t dtable, uintptr_t work) {
     const OnDevice on(dev);
     if (route == 0) {
       route = work + pad16(4 * leaf_route_words(n, G));
@@ -101,9 +101,9 @@ void bind_leaf(py::module_& m) {
                            scale, P<void>(dtable), P<void>(work));
   });
   m.def("leaf_linear_small_rows", &leaf_linear_small_rows);
-  m.def("leaf_linear_small", [](int dev, uintptr_t s, int type, uintptr_t x, int64_t x_stride, uintptr_t ids,
-                                bool wide, int n, int G, uintptr_t w, uintptr_t bias, int K, int N,
-                                uintptr_t y) {
+  m.def("leaf_linear_small", [](int dev, uintptr_t s, int type, uintptr_t x, int64_t x_stride,
+                                uintptr_t ids, bool wide, int n, int G, uintptr_t w,
+                                uintptr_t bias, int K, int N, uintptr_t y) {
     const OnDevice on(dev);
     launch_leaf_linear_small(S(s), type, P<void>(x), x_stride, P<void>(ids), wide, n, G,
                              P<void>(w), P<void>(bias), K, N, P<void>(y));
@@ -112,9 +112,9 @@ void bind_leaf(py::module_& m) {
   m.def("leaf_linear_bytes", [](int64_t n, int G) {
     return std::max(4 * leaf_route_words(n, G), leaf_linear_tile_bytes(n, G));
   });
-  m.def("leaf_linear", [](int dev, uintptr_t s, int type, uintptr_t x, int64_t x_stride, uintptr_t ids,
-                          bool wide, uintptr_t route, int64_t n, int G, uintptr_t w, uintptr_t bias,
-                          int K, int N, uintptr_t y, uintptr_t work) {
+  m.def("leaf_linear", [](int dev, uintptr_t s, int type, uintptr_t x, int64_t x_stride,
+                          uintptr_t ids, bool wide, uintptr_t route, int64_t n, int G, uintptr_t w,
+                          uintptr_t bias, int K, int N, uintptr_t y, uintptr_t work) {
     const OnDevice on(dev);
     const Route r(route, n);
     if (ids != 0)
@@ -128,9 +128,9 @@ void bind_leaf(py::module_& m) {
     return std::max({leaf_linear_tile_bytes(n, G), leaf_linear_grad_bytes(type, n, G, K, N),
                      leaf_embed_grad_bytes(type, n, N)});
   });
-  m.def("leaf_linear_grad", [](int dev, uintptr_t s, int type, uintptr_t x, int64_t x_stride, uintptr_t dy,
-                               int64_t dy_stride, uintptr_t route, int64_t n, int G, uintptr_t w,
-                               int K, int N, uintptr_t dx, uintptr_t dw, uintptr_t db,
+  m.def("leaf_linear_grad", [](int dev, uintptr_t s, int type, uintptr_t x, int64_t x_stride,
+                               uintptr_t dy, int64_t dy_stride, uintptr_t route, int64_t n, int G,
+                               uintptr_t w, int K, int N, uintptr_t dx, uintptr_t dw, uintptr_t db,
                                uintptr_t work) {
     const OnDevice on(dev);
     const Route r(route, n);
@@ -139,11 +139,12 @@ void bind_leaf(py::module_& m) {
                               P<void>(w), nullptr, K, N, P<void>(dx), P<void>(work));
     bool made = false;
     if (dw != 0)
-      made = launch_leaf_linear_grad(S(s), type, P<void>(x), x_stride, P<void>(dy), dy_stride, r.order,
-                              r.keys, r.off, n, G, K, N, P<void>(dw), P<void>(db), P<void>(work));
+      made = launch_leaf_linear_grad(S(s), type, P<void>(x), x_stride, P<void>(dy), dy_stride,
+                                     r.order, r.keys, r.off, n, G, K, N, P<void>(dw), P<void>(db),
+                                     P<void>(work));
     if (db != 0 && !made)
-      launch_leaf_embed_grad(S(s), type, P<void>(dy), dy_stride, r.order, r.keys, r.off, n, G, N, 1.f,
-                             P<void>(db), P<void>(work));
+      launch_leaf_embed_grad(S(s), type, P<void>(dy), dy_stride, r.order, r.keys, r.off, n, G, N,
+                             1.f, P<void>(db), P<void>(work));
   });
 }
 

@@ -5,11 +5,11 @@
 //
 // Gradient: dtable[v] = scale * sum of dy over the rows of leaf v, for every v (zeros where no row
 // is). The rows are sorted by leaf first (leaf_route.hip), so a leaf's rows are a run of `order`,
-// and every sum has one fixed order: the result does not depend on the launch. The sorted
-// positions are cut into chunks, one for a group of lanes, which streams its chunk's rows (their
-// numbers are known at once, so a batch of rows is in flight) and writes out a sum where the leaf
-// changes. A leaf that reaches over a chunk's end leaves partial rows there, at most two a chunk,
-// and a second launch adds a leaf's partial rows. Leaves without rows are found through the offsets.
+// and every sum has one fixed order: the result does not depend on the launch. The sorted positions
+// are cut into chunks, one for a group of lanes, which streams its chunk's rows (their numbers are
+// known at once, so a batch of rows is in flight) and writes out a sum where the leaf changes. A
+// leaf that reaches over a chunk's end leaves partial rows there, at most two a chunk, and a second
+// launch adds a leaf's partial rows. Leaves without rows are found through the offsets.
 //
 // Sums are held in 32 bits for 16-bit types and in 64 bits for f32: a leaf may hold most of a
 // million rows, and a 64-bit add costs no more than a 32-bit one here, where memory is the bound.
@@ -18,10 +18,10 @@
 namespace mt {
 
 constexpr int kLeThreads = 256;
-// Rows of a group in flight. Each takes dependent loads (number, row), so narrow vectors need more
-// rows: forward 4 of 16 bytes a lane, 16 of less (63 columns of f32: 86 -> XX us with 16);
+// Rows of a group in flight, in the forward pass and in the gradient. Each takes dependent loads
+// (number, row), so narrow vectors need more of them (63 columns of f32 forward: 86 us with 4, 80
+// with 16).
 constexpr int le_unroll(int bytes) { return bytes >= 16 ? 4 : 16; }
-// gradient 8 and 16.
 constexpr int le_batch(int bytes) { return bytes >= 16 ? 8 : 16; }
 constexpr int kLeEmpty = 16;  // leaves that a group looks over for missing rows
 
@@ -54,7 +54,7 @@ __device__ __forceinline__ int64_t le_same(int64_t v) {
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
-template <typename T, int W, int NC, bool kScale, bool kWide, bool kWave>
+template <typename T, int W, int NC, bool kWide, bool kWave>
 __global__ __launch_bounds__(kLeThreads) void le_forward_kernel(
     const void* __restrict__ ids, const T* __restrict__ table, int64_t stride, int64_t n,
     int64_t V, int D, float scale, LeCols lc, T* __restrict__ y) {
@@ -88,10 +88,8 @@ __global__ __launch_bounds__(kLeThreads) void le_forward_kernel(
     for (int u = 0; u < kUnroll; ++u) {
       const int64_t r = r0 + (int64_t)u * rpb;
       if (r >= n) break;
-      if constexpr (kScale) {
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[u].v[e] = leaf_from<T>(leaf_f32(v[u].v[e]) * scale);
-      }
+      for (int e = 0; e < W; ++e) v[u].v[e] = leaf_from<T>(leaf_f32(v[u].v[e]) * scale);
       *(LeafVec<T, W>*)(y + r * D + c) = v[u];
     }
   }
@@ -127,7 +125,8 @@ __device__ __forceinline__ void le_store(T* __restrict__ out, float scale, const
 
 // Blocks below `chunk_blocks`: a chunk of 1 << run_shift sorted positions for each group of lanes,
 // partial rows into `part` ([2 * chunks][D]: of the leaf that reaches into the chunk, of the one
-// that starts in it and reaches out; open[chunk]: that one's number + 1, or 0). Blocks from there on: zeros for the leaves without rows.
+// that starts in it and reaches out; open[chunk]: that one's number + 1, or 0). Blocks from there
+// on: zeros for the leaves without rows.
 template <typename T, int W, bool kWave>
 __global__ __launch_bounds__(kLeThreads) void le_backward_kernel(
     const T* __restrict__ dy, int64_t stride, const int32_t* __restrict__ order,
@@ -275,7 +274,7 @@ static void le_dispatch_32(int W, F f) {
     f(std::integral_constant<int, 1>{});
 }
 
-template <typename T, bool kScale, int W>
+template <typename T, int W>
 static void le_forward(hipStream_t s, const void* ids, bool wide, const T* table, int64_t stride,
                        int64_t n, int64_t V, int D, float scale, T* y) {
   // wide rows: four vectors a lane while that leaves no lane idle
@@ -289,40 +288,34 @@ static void le_forward(hipStream_t s, const void* ids, bool wide, const T* table
     MT_HIP_CHECK(hipGetLastError());
   };
   if (four)
-    wide ? go(le_forward_kernel<T, W, 4, kScale, true, true>)
-         : go(le_forward_kernel<T, W, 4, kScale, false, true>);
+    wide ? go(le_forward_kernel<T, W, 4, true, true>)
+         : go(le_forward_kernel<T, W, 4, false, true>);
   else if (lc.tpr_shift == 6)
-    wide ? go(le_forward_kernel<T, W, 1, kScale, true, true>)
-         : go(le_forward_kernel<T, W, 1, kScale, false, true>);
+    wide ? go(le_forward_kernel<T, W, 1, true, true>)
+         : go(le_forward_kernel<T, W, 1, false, true>);
   else
-    wide ? go(le_forward_kernel<T, W, 1, kScale, true, false>)
-         : go(le_forward_kernel<T, W, 1, kScale, false, false>);
+    wide ? go(le_forward_kernel<T, W, 1, true, false>)
+         : go(le_forward_kernel<T, W, 1, false, false>);
 }
 
 void launch_leaf_embed(hipStream_t s, int type, const void* ids, bool wide, const void* table,
                        int64_t stride, int64_t n, int64_t V, int D, float scale, void* y) {
   if (n <= 0 || D <= 0) return;
-  const int elem = type == kLeafF32 || type == kLeafRaw32 ? 4 : 2;
-  const int W = le_width(elem, D, stride, table, y);
+  const int W = le_width(type == kLeafF32 ? 4 : 2, D, stride, table, y);
   if (type == kLeafF32)
     le_dispatch_32(W, [&](auto w) {
-      le_forward<float, true, w()>(s, ids, wide, (const float*)table, stride, n, V, D, scale,
-                                   (float*)y);
-    });
-  else if (type == kLeafRaw32)
-    le_dispatch_32(W, [&](auto w) {
-      le_forward<uint32_t, false, w()>(s, ids, wide, (const uint32_t*)table, stride, n, V, D, scale,
-                                       (uint32_t*)y);
+      le_forward<float, w()>(s, ids, wide, (const float*)table, stride, n, V, D, scale,
+                             (float*)y);
     });
   else if (type == kLeafF16)
     le_dispatch_16(W, [&](auto w) {
-      le_forward<f16_t, true, w()>(s, ids, wide, (const f16_t*)table, stride, n, V, D, scale,
-                                   (f16_t*)y);
+      le_forward<f16_t, w()>(s, ids, wide, (const f16_t*)table, stride, n, V, D, scale,
+                             (f16_t*)y);
     });
   else
     le_dispatch_16(W, [&](auto w) {
-      le_forward<bf16_t, true, w()>(s, ids, wide, (const bf16_t*)table, stride, n, V, D, scale,
-                                    (bf16_t*)y);
+      le_forward<bf16_t, w()>(s, ids, wide, (const bf16_t*)table, stride, n, V, D, scale,
+                              (bf16_t*)y);
     });
 }
 
@@ -343,8 +336,8 @@ int64_t leaf_embed_grad_bytes(int type, int64_t n, int D) {
 
 template <typename T, int W>
 static void le_backward(hipStream_t s, const T* dy, int64_t stride, const int32_t* order,
-                        const uint32_t* keys, const int32_t* off, int64_t n, int64_t V, int D, float scale, T* dtable,
-                        void* work) {
+                        const uint32_t* keys, const int32_t* off, int64_t n, int64_t V, int D,
+                        float scale, T* dtable, void* work) {
   using A = typename LeAcc<T>::type;
   const LeCols lc = le_cols(D, W, 1);
   const int rpb = kLeThreads >> lc.tpr_shift, shift = le_run_shift(n, lc);
@@ -354,8 +347,9 @@ static void le_backward(hipStream_t s, const T* dy, int64_t stride, const int32_
   A* const part = (A*)work;
   uint32_t* const open = (uint32_t*)(part + 2 * chunks * D);
   auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, leaf_grid(chunk_blocks + empty), dim3(kLeThreads), 0, s, dy, stride, order,
-                       keys, off, V, D, scale, lc, shift, chunks, chunk_blocks, dtable, part, open);
+    hipLaunchKernelGGL(kern, leaf_grid(chunk_blocks + empty), dim3(kLeThreads), 0, s, dy, stride,
+                       order, keys, off, V, D, scale, lc, shift, chunks, chunk_blocks, dtable, part,
+                       open);
     MT_HIP_CHECK(hipGetLastError());
   };
   lc.tpr_shift == 6 ? go(le_backward_kernel<T, W, true>) : go(le_backward_kernel<T, W, false>);
@@ -368,8 +362,8 @@ static void le_backward(hipStream_t s, const T* dy, int64_t stride, const int32_
 }
 
 void launch_leaf_embed_grad(hipStream_t s, int type, const void* dy, int64_t stride,
-                            const int32_t* order, const uint32_t* keys, const int32_t* off, int64_t n, int64_t V, int D,
-                            float scale, void* dtable, void* work) {
+                            const int32_t* order, const uint32_t* keys, const int32_t* off,
+                            int64_t n, int64_t V, int D, float scale, void* dtable, void* work) {
   if (D <= 0) return;
   const int W = le_width(type == kLeafF32 ? 4 : 2, D, stride, dy, dtable);
   if (type == kLeafF32)

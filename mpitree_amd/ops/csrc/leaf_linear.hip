@@ -16,7 +16,7 @@ namespace mt {
 constexpr int kLlThreads = 256;
 constexpr int kLlWaves = kLlThreads / kWave;
 constexpr int kLlSmallRows = 64;
-constexpr int kLlBigRows = 512;  // rows a leaf on average from which on 256-row tiles are taken
+constexpr int kLlBigRows = 256;  // rows a leaf on average from which on 256-row tiles are taken
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -239,9 +239,9 @@ struct LlTile {
   const int32_t* plan_count;  // how many there are
 };
 
-// The tiles of kBig rows in order of their leaves, {leaf, first sorted position}, and how many there
-// are: with many column tiles, tiles without rows between them would keep neighbours from
-// sharing what they read. One workgroup; a leaf has at least 512 rows on average here.
+// The tiles of kBig rows in order of their leaves, {leaf, first sorted position}, and how many
+// there are: with many column tiles, tiles without rows between them would keep neighbours from
+// sharing what they read. One workgroup; a leaf has at least kLlBigRows rows on average here.
 constexpr int kLlPlanThreads = 1024;
 __global__ __launch_bounds__(kLlPlanThreads) void ll_plan_kernel(const int32_t* __restrict__ off,
                                                                  int G, int bj_shift,
@@ -508,10 +508,15 @@ __global__ __launch_bounds__(kLlThreads) void ll_rows_kernel(LlTile a) {
   const int rows = (int)max<int64_t>(-1, min<int64_t>(kRowsTile, a.off[g + 1] - m0));
   if (rows <= 0) return;
   // 16 rows at a time; the row of this lane in the j-th 16 (past the last one: that one)
-  const int32_t ord0 = a.order[m0 + min(l, rows - 1)];
-  const int32_t ord1 = a.order[m0 + min(kWave + l, rows - 1)];
+  constexpr int kOrd = kRowsTile / kWave;
+  int32_t ord[kOrd];
+#pragma unroll
+  for (int i = 0; i < kOrd; ++i) ord[i] = a.order[m0 + min(i * kWave + l, rows - 1)];
   auto row_of = [&](int j) {
-    return __shfl(j < 4 ? ord0 : ord1, ((16 * j) & (kWave - 1)) + (l & 15), kWave);
+    int32_t o = ord[0];
+#pragma unroll
+    for (int i = 1; i < kOrd; ++i) o = j >= 4 * i ? ord[i] : o;
+    return __shfl(o, ((16 * j) & (kWave - 1)) + (l & 15), kWave);
   };
   const bool vec = a.cols % 4 == 0 && (uintptr_t)a.out % (4 * sizeof(T)) == 0;
   const int c0 = i0 + 4 * (l >> 4);
@@ -618,8 +623,8 @@ __global__ __launch_bounds__(kLlThreads) void ll_rows_kernel(LlTile a) {
 // (Behind the last tile the same happens with zeros, which nothing uses.)
 //
 // A turned operand's depth rows lie in pairs, kPair bytes apart: 512 bytes a row and 32 to spare,
-// and the odd row's slabs lie at s ^ 2. So the four rows that 16 lanes read at once, and those of the
-// next 16 lanes, are in different banks, and a fragment's address is one of two lane constants
+// and the odd row's slabs lie at s ^ 2. So the four rows that 16 lanes read at once, and those of
+// the next 16 lanes, are in different banks, and a fragment's address is one of two lane constants
 // plus an immediate.
 constexpr int kBig = 256, kBigWaves = 8, kBigThreads = kBigWaves * kWave;
 constexpr int kBigPair = 2 * 512 + 32;
@@ -778,8 +783,9 @@ __global__ __launch_bounds__(kBigThreads, 2) void ll_big_kernel(LlTile a) {
   ll_store_rows<T, 32, SJ, SI>(acc, a, at, wj, wi);
 }
 
-// ---- dW. A unit is a leaf with at most `run` rows (units below G), or a leaf's piece of a chunk of
-// `run` sorted positions into a partial matrix (as in leaf_embed.hip: at most two pieces a chunk).
+// ---- dW. A unit is a leaf with at most `run` rows (units below G), or a leaf's piece of a chunk
+// of `run` sorted positions into a partial matrix (as in leaf_embed.hip: at most two pieces a
+// chunk).
 struct LlGrad {
   const void* x;
   const void* dy;
@@ -852,8 +858,9 @@ __device__ __forceinline__ void ll_store_sum(const LlGrad& a, int64_t unit, int 
 }
 
 // One B x B tile (rows of W, columns of W) of one unit: both operands are gathered rows with the
-// rows as depth, turned. The row numbers of a tile of depth are fetched a tile ahead of the rows. The
-// sums of dy (db) fall out of its fragments, in 64 bits for f32. kAligned: as in ll_tile_kernel.
+// rows as depth, turned. The row numbers of a tile of depth are fetched a tile ahead of the rows.
+// The sums of dy (db) fall out of its fragments, in 64 bits for f32. kAligned: as in
+// ll_tile_kernel.
 template <typename T, int B, bool kAligned>
 __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
   using A = std::conditional_t<sizeof(T) == 4, double, float>;
@@ -861,6 +868,7 @@ __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
   constexpr int S = B / 2 / 16, Q = B * 8 / kLlThreads;  // 2 x 2 waves
   __shared__ uint4 s_j0[B * 8], s_i0[B * 8];
   __shared__ uint4 s_j1[kAligned ? B * 8 : 1], s_i1[kAligned ? B * 8 : 1];
+  __shared__ A s_sum[kLlWaves][S * 16];
   const int64_t blk = leaf_block();
   const int tiles = a.n_tiles * a.k_tiles;
   const int64_t unit = blk / tiles;
@@ -876,7 +884,8 @@ __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
 
   f32x4 acc[S][S] = {};
   A sum[S] = {};
-  const bool sums = a.db != nullptr && i0 + wi == 0;
+  // two waves hold the same rows of dy: each sums one half of the depth
+  const bool sums = a.db != nullptr && i0 == 0;
   const LlLane<T> ln;
   auto products = [&](const uint4* sj, const uint4* si) {
 #pragma unroll
@@ -890,7 +899,7 @@ __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
       for (int j = 0; j < S; ++j)
 #pragma unroll
         for (int i = 0; i < S; ++i) acc[j][i] = ll_mma<T>(fi[i], fj[j], acc[j][i]);
-      if (sums) {
+      if (sums && step == (w & 1)) {
 #pragma unroll
         for (int j = 0; j < S; ++j) {
           T e[E];
@@ -972,9 +981,13 @@ __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
     for (int j = 0; j < S; ++j) {
       sum[j] += __shfl_xor(sum[j], 16, kWave);
       sum[j] += __shfl_xor(sum[j], 32, kWave);
-      const int c = j0 + wj + j * 16 + l;
-      if (l < 16 && c < a.N) ll_store_sum<T>(a, unit, c, (double)sum[j]);
+      if (l < 16) s_sum[w][j * 16 + l] = sum[j];
     }
+    __syncthreads();
+    const int c = tid % B, q = c / (S * 16) * 2;
+    if (tid < B && j0 + c < a.N)
+      ll_store_sum<T>(a, unit, j0 + c,
+                      (double)s_sum[q][c % (S * 16)] + (double)s_sum[q + 1][c % (S * 16)]);
   }
   ll_grad_store<T, S, S>(acc, a, unit, j0 + wj, i0 + wi);
 }
@@ -1081,8 +1094,8 @@ __global__ __launch_bounds__(kBigThreads, 2) void ll_big_grad_kernel(LlGrad a) {
 }
 
 // The same for f32 and few columns on either side: the waves of a block take 16 rows in turn, from
-// memory straight into fragments, each for the whole 16 SJ x 16 SI tile, and their sums meet in LDS.
-// The sums of dy (db) fall out of its fragments, in 64 bits.
+// memory straight into fragments, each for the whole 16 SJ x 16 SI tile, and their sums meet in
+// LDS. The sums of dy (db) fall out of its fragments, in 64 bits.
 template <int SJ, int SI>
 __global__ __launch_bounds__(kLlThreads) void ll_rows_grad_kernel(LlGrad a) {
   __shared__ f32x4 s_acc[2][SJ * SI][kWave];
@@ -1172,7 +1185,7 @@ __global__ __launch_bounds__(kLlThreads) void ll_rows_grad_kernel(LlGrad a) {
 
 // Adds the partial matrices of the leaves with more than `run` rows, in 64 bits for f32 (and their
 // partial sums of dy, where the kernel above made them): one block per chunk in which such a leaf
-// starts and per 4 * kLlThreads elements.
+// starts, up to 512 times, each taking 4 elements a thread in turn.
 template <typename T>
 __global__ __launch_bounds__(kLlThreads) void ll_join_kernel(LlGrad a, int64_t blocks_per_chunk,
                                                              int64_t chunks) {
@@ -1187,9 +1200,10 @@ __global__ __launch_bounds__(kLlThreads) void ll_join_kernel(LlGrad a, int64_t b
   const int64_t size = (int64_t)a.N * a.K;
   const int64_t last = (e1 - 1) / a.run;
   const int64_t slot0 = 2 * c + (k1 != k0 ? 1 : 0);
-  const int64_t e = ((blk % blocks_per_chunk) * kLlThreads + threadIdx.x) * 4;
+  const int64_t e0 = ((blk % blocks_per_chunk) * kLlThreads + threadIdx.x) * 4;
+  const int64_t stride = blocks_per_chunk * kLlThreads * 4;
   if (size % 4 == 0) {
-    if (e < size) {
+    for (int64_t e = e0; e < size; e += stride) {
       A sum[4] = {};
       for (int64_t p = c; p <= last; ++p) {
         const f32x4 v = *(const f32x4*)(a.part + (p == c ? slot0 : 2 * p) * size + e);
@@ -1202,12 +1216,13 @@ __global__ __launch_bounds__(kLlThreads) void ll_join_kernel(LlGrad a, int64_t b
       *(LeafVec<T, 4>*)((T*)a.dw + k1 * size + e) = o;
     }
   } else {
-    for (int u = 0; u < 4 && e + u < size; ++u) {
-      A sum = 0;
-      for (int64_t p = c; p <= last; ++p)
-        sum += (A)a.part[(p == c ? slot0 : 2 * p) * size + e + u];
-      ((T*)a.dw)[k1 * size + e + u] = leaf_from<T>((float)sum);
-    }
+    for (int64_t e = e0; e < size; e += stride)
+      for (int u = 0; u < 4 && e + u < size; ++u) {
+        A sum = 0;
+        for (int64_t p = c; p <= last; ++p)
+          sum += (A)a.part[(p == c ? slot0 : 2 * p) * size + e + u];
+        ((T*)a.dw)[k1 * size + e + u] = leaf_from<T>((float)sum);
+      }
   }
   if (a.db != nullptr && blk % blocks_per_chunk == 0) {
     for (int n = threadIdx.x; n < a.N; n += kLlThreads) {
@@ -1218,11 +1233,11 @@ __global__ __launch_bounds__(kLlThreads) void ll_join_kernel(LlGrad a, int64_t b
   }
 }
 
-// ---- forward of at most 64 rows, straight from the leaf indices (no route). Each wave holds all of
-// them, one a lane. Block (column tile, row i): row i leads the tile of up to 16 rows of its leaf
-// that start with it; rows that follow another row of their leaf inside its 16 leave. So a leaf's
-// matrix is read once for 16 rows. The waves split the depth, from memory straight into fragments,
-// and their sums meet in LDS.
+// ---- forward of at most 64 rows, straight from the leaf indices (no route). Each wave holds all
+// of them, one a lane. Block (column tile, row i): row i leads the tile of up to 16 rows of its
+// leaf that start with it; rows that follow another row of their leaf inside its 16 leave. So a
+// leaf's matrix is read once for 16 rows. The waves split the depth, from memory straight into
+// fragments, and their sums meet in LDS.
 struct LlSmall {
   const void* x;
   const void* ids;
@@ -1338,7 +1353,13 @@ void launch_leaf_linear_small(hipStream_t s, int type, const void* x, int64_t x_
   });
 }
 
-static bool ll_short_rows(int depth_bytes, int cols) { return depth_bytes <= 256 && cols <= 128; }
+// Rows short enough for ll_rows_kernel. 500k rows in 2000 leaves, us of it / of the tiles: f32 64
+// deep, 16 columns 36 / 32, 32: 47 / 68, 64: 82 / 92, 128: 153 / 167; bf16 64 deep, 64 columns 38 /
+// 44, 128: 67 / 73; bf16 128 deep, 128 columns 121 / 108, its row gradient 143 / 106.
+static bool ll_short_rows(int elem, int depth, int cols) {
+  if (cols > 128) return false;
+  return depth * elem <= 128 || (elem == 4 && depth * elem <= 256 && cols > 16);
+}
 
 // scratch for the tile list
 int64_t leaf_linear_tile_bytes(int64_t n, int G) {
@@ -1375,11 +1396,14 @@ void launch_leaf_linear_tile(hipStream_t s, int type, bool dx, const void* src, 
            : run(ll_tile_kernel<T, false, bj(), bi(), wj(), nw(), false>);
     };
     const int64_t mean = n / G;
+    // 256 x 256 tiles from 256 of them on (16384 rows in 16 leaves, 1024 -> 1024 bf16: 41 us, 57
+    // with 128 x 128; 8192 rows: 44 and 39), and leaves that fill them (128 rows a leaf, 2048 ->
+    // 2048: 364 and 329; 256 rows, 1024 -> 1024: 44 and 49)
     const bool big = sizeof(T) == 2 && al && mean >= kLlBigRows &&
-                     (n >> 8) * ((a.cols + kBig - 1) / kBig) >= 512 &&
-                     n * src_stride * (int64_t)sizeof(T) < (1ll << 32) &&
+                     (n >> 8) * ((a.cols + kBig - 1) / kBig) >= 256 &&
+                     (n * src_stride + a.depth) * (int64_t)sizeof(T) < (1ll << 32) &&
                      a.w_stride * (int64_t)sizeof(T) < (1ll << 32);
-    if (ll_short_rows(a.depth * (int)sizeof(T), a.cols)) {
+    if (ll_short_rows(sizeof(T), a.depth, a.cols)) {
       const int si = a.cols <= 16 ? 1 : a.cols <= 32 ? 2 : 4;  // fragments of columns a wave holds
       a.col_tiles = (a.cols + si * 16 - 1) / (si * 16);
       a.tiles = ((n >> kRowsShift) + G + 1) * a.col_tiles;
@@ -1396,16 +1420,28 @@ void launch_leaf_linear_tile(hipStream_t s, int type, bool dx, const void* src, 
           al ? run(ll_rows_kernel<T, false, steps(), cols(), true>)
              : run(ll_rows_kernel<T, false, steps(), cols(), false>);
       };
-      const bool half = a.depth * (int)sizeof(T) <= 128;
-      auto steps = [&](auto cols) {
-        half ? rows(LlInt<2>{}, cols) : rows(LlInt<4>{}, cols);
-      };
-      si == 1 ? steps(LlInt<1>{}) : si == 2 ? steps(LlInt<2>{}) : steps(LlInt<4>{});
+      [[maybe_unused]] const bool half = a.depth * (int)sizeof(T) <= 128;
+      if constexpr (sizeof(T) == 4) {
+        if (half)
+          si == 1   ? rows(LlInt<2>{}, LlInt<1>{})
+          : si == 2 ? rows(LlInt<2>{}, LlInt<2>{})
+                    : rows(LlInt<2>{}, LlInt<4>{});
+        else
+          si == 2 ? rows(LlInt<4>{}, LlInt<2>{}) : rows(LlInt<4>{}, LlInt<4>{});
+      } else {
+        si == 1   ? rows(LlInt<2>{}, LlInt<1>{})
+        : si == 2 ? rows(LlInt<2>{}, LlInt<2>{})
+                  : rows(LlInt<2>{}, LlInt<4>{});
+      }
     } else if (a.cols <= 16)
       go(LlInt<64>{}, LlInt<16>{}, LlInt<4>{}, LlInt<4>{});
-    else if (mean < 32)
+    // Rows of a tile by the mean rows of a leaf; 16384 rows, 1024 -> 1024 bf16, us with 16 / 64 /
+    // 128 rows: mean 8: 757 / 792 / 827, mean 16: 412 / 429 / 430, mean 32: 262 / 236 / 234, mean
+    // 64: 192 / 133 / 128, mean 256: 127 / 67 / 49. 512 -> 512 f32: mean 16: 219 / 259 / 509, mean
+    // 32: 139 / 143 / 267, mean 64: 116 / 99 / 142, mean 128: 114 / 93 / 82.
+    else if (mean < (sizeof(T) == 4 ? 48 : 24))
       go(LlInt<16>{}, LlInt<64>{}, LlInt<1>{}, LlInt<4>{});
-    else if (mean < 128 || a.cols <= 64)
+    else if ((sizeof(T) == 4 && mean < 96) || a.cols <= 64)
       go(LlInt<64>{}, LlInt<64>{}, LlInt<2>{}, LlInt<4>{});
     else if (!big)
       go(LlInt<128>{}, LlInt<128>{}, LlInt<2>{}, LlInt<4>{});
@@ -1428,20 +1464,29 @@ void launch_leaf_linear_tile(hipStream_t s, int type, bool dx, const void* src, 
   });
 }
 
-// Rows a dW unit may have, a power of two: so many that about 512 to 1024 tiles run at once, and
-// where whole leaves are that many already, four times the mean leaf, so that only leaves far above
-// it are cut (a cut costs a partial matrix in 32 bits, written and read).
-static int64_t ll_grad_run(int64_t n, int G, int64_t tiles) {
+// Rows a dW unit may have, a power of two; leaves with more are cut, and a cut costs a partial
+// matrix in 32 bits, written and read. Where whole leaves make 2048 tiles, only those above four
+// times the mean are cut; otherwise pieces make up to 512 tiles (256 of the largest). us as chosen,
+// and with other cuts: 16384 rows of one leaf, 1024 x 1024 bf16 55, with twice the pieces 77; 1M
+// rows of 8 leaves, 64 x 64 f32 208, with four times the pieces 297; 10007 rows of 12 leaves of
+// very different sizes, 1000 x 601 f16 57, with half the pieces 50.
+static int64_t ll_grad_run(int64_t n, int G, int b, int64_t tiles) {
   int64_t run = 256;
-  while (run < (1 << 20) && n / run * tiles > 1024) run <<= 1;
-  if (G * tiles >= 1024)
+  if (G * tiles >= 2048) {
     while (run < 4 * (n / G)) run <<= 1;
+  } else {
+    while (run < (1 << 20) && n / run * tiles > (b == kBig ? 256 : 512)) run <<= 1;
+  }
   return run;
 }
-// tile edge of dW; direct: operands are 16-byte aligned and lie within 4 GiB
+// Tile edge of dW; direct: operands are 16-byte aligned and lie within 4 GiB. 256 where leaves are
+// long and fill the GPU, whole or in pieces; bf16 1024 x 1024, us with 256 / 128: 4096 rows in 4
+// leaves 39 / 22, in 16 25 / 31, in 64 68 / 57; 16384 rows in 1 55 / 61, in 16 44 / 62, in 64 81 /
+// 90.
 static int ll_grad_tile(int type, bool direct, int64_t n, int G, int K, int N) {
   const int64_t big = (int64_t)((N + kBig - 1) / kBig) * ((K + kBig - 1) / kBig);
-  if (type != kLeafF32 && direct && N > 128 && K > 128 && n / G >= 256 && big * G >= 256)
+  if (type != kLeafF32 && direct && N > 128 && K > 128 && n / G >= 256 &&
+      (G * big >= 256 || (n / 256) * big >= 1024))
     return kBig;
   return N > 64 && K > 64 ? 128 : 64;
 }
@@ -1457,7 +1502,7 @@ int64_t leaf_linear_grad_bytes(int type, int64_t n, int G, int K, int N) {
   int64_t chunks = 0;
   for (bool direct : {false, true}) {
     const int b = ll_grad_tile(type, direct, n, G, K, N);
-    const int64_t run = ll_grad_run(n, G, ll_grad_tiles(b, K, N));
+    const int64_t run = ll_grad_run(n, G, b, ll_grad_tiles(b, K, N));
     if (n > run) chunks = std::max(chunks, (n + run - 1) / run);
   }
   return 2 * chunks * ((int64_t)N * K * 4 + 8 * N + 8);
@@ -1476,11 +1521,12 @@ bool launch_leaf_linear_grad(hipStream_t s, int type, const void* x, int64_t x_s
   const int64_t elem = type == kLeafF32 ? 4 : 2;
   const bool al = (elem == 4 ? ll_aligned<float> : ll_aligned<f16_t>)(
       {x, dy}, {K, N, x_stride, dy_stride});
-  const bool direct = al && n * std::max(x_stride, dy_stride) * elem < (1ll << 32);
+  const bool direct =
+      al && (n * std::max(x_stride, dy_stride) + std::max(K, N)) * elem < (1ll << 32);
   const int b = ll_grad_tile(type, direct, n, G, K, N);
   const int64_t tiles = ll_grad_tiles(b, K, N);
   a.n_tiles = (N + b - 1) / b, a.k_tiles = (K + b - 1) / b;
-  a.run = ll_grad_run(n, G, tiles);
+  a.run = ll_grad_run(n, G, b, tiles);
   const int64_t chunks = n > a.run ? (n + a.run - 1) / a.run : 0;
   a.units = G + 2 * chunks;
   ll_dispatch_type(type, [&](auto t) {
@@ -1504,7 +1550,10 @@ bool launch_leaf_linear_grad(hipStream_t s, int type, const void* x, int64_t x_s
          : run(ll_grad_kernel<T, 64, false>, all, kLlThreads);
     }
     if (chunks > 0) {
-      const int64_t per = ((int64_t)N * K + 4 * kLlThreads - 1) / (4 * kLlThreads);
+      // (few chunks hold such a leaf's start: at most 512 blocks each, or the empty ones take
+      // longer)
+      const int64_t per =
+          std::min<int64_t>(512, ((int64_t)N * K + 4 * kLlThreads - 1) / (4 * kLlThreads));
       hipLaunchKernelGGL(ll_join_kernel<T>, leaf_grid(chunks * per), dim3(kLlThreads), 0, s, a, per,
                          chunks);
       MT_HIP_CHECK(hipGetLastError());

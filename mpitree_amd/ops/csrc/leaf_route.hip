@@ -57,9 +57,10 @@ __device__ __forceinline__ void lr_rank(const uint32_t (&key)[kLrItems], uint32_
     const unsigned long long m = lr_match(d, in);
     const uint32_t c = s_wh[w][d];
     rk[k] = c + (uint32_t)__popcll(m & lt);
-    __builtin_amdgcn_wave_barrier();
+    // (the wave's reads come before its writes, and those before the next item's reads)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (in && (m & lt) == 0ull) s_wh[w][d] = c + (uint32_t)__popcll(m);
-    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
