@@ -19,8 +19,9 @@ bfloat16, all of one type; sums are held in 32 bits (float32: 64 bits where only
 and rounded once. Gradients do not depend on the launch: the same inputs give the same bits.
 
 CUDA tensors run the gfx950 kernels (``ops/csrc/leaf_*.hip``) on the tensors' device and its current
-stream, without host synchronisation, so calls can be captured into a graph; CPU tensors take a
-plain path of the same results.
+stream, without host synchronisation, so calls can be captured into a graph (one with a backward
+pass: while no eager autograd graph of the same parameters is alive, as for every operator of
+torch). CPU tensors take a plain path of the same results.
 """
 
 from __future__ import annotations
@@ -33,6 +34,7 @@ __all__ = ["LeafRoute", "leaf_route", "leaf_embedding", "leaf_linear"]
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _MAX_ROWS = 2 ** 31 - 1
+_MAX_LEAVES = 2 ** 30
 _MAX_WIDTH = 2 ** 20
 
 
@@ -40,9 +42,9 @@ class LeafRoute:
     """Rows sorted by leaf, from :func:`leaf_route`: ``order[offsets[g]:offsets[g + 1]]`` are leaf
     ``g``'s rows in their order, for ``g == n_leaves`` the rows without a leaf.
 
-    ``leaves`` are the leaf numbers it was made from, ``keys`` [n] the leaf at each sorted position
-    (``n_leaves``: none), ``order`` [n] and ``offsets`` [n_leaves + 2]: int32 tensors. It stays
-    valid when ``leaves`` is changed later; the operators then still follow the route."""
+    ``leaves`` is its own copy of the leaf numbers it was made from, ``keys`` [n] the leaf at each
+    sorted position (``n_leaves``: none), ``order`` [n] and ``offsets`` [n_leaves + 2]: int32
+    tensors, not to be written. It stays as it is when the numbers are changed later."""
 
     __slots__ = ("leaves", "n_leaves", "_buf")
 
@@ -85,8 +87,8 @@ def _check_leaves(leaves) -> torch.Tensor:
 
 def _check_n_leaves(n_leaves) -> int:
     n_leaves = int(n_leaves)
-    if not 1 <= n_leaves <= _MAX_ROWS - 1:
-        raise ValueError(f"n_leaves must be in [1, {_MAX_ROWS - 1}], got {n_leaves}")
+    if not 1 <= n_leaves <= _MAX_LEAVES:
+        raise ValueError(f"n_leaves must be in [1, {_MAX_LEAVES}], got {n_leaves}")
     return n_leaves
 
 
@@ -135,9 +137,12 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 # -------------------------------------------------------------------------------- route
 def leaf_route(leaves: torch.Tensor, n_leaves: int) -> LeafRoute:
     """Sort the rows by leaf (stable). ``leaves``: int32 or int64 of any shape."""
-    leaves = _check_leaves(leaves)
-    n_leaves = _check_n_leaves(n_leaves)
-    ids = leaves.detach().reshape(-1)
+    return _route(_check_leaves(leaves).clone(memory_format=torch.contiguous_format),
+                  _check_n_leaves(n_leaves))
+
+
+def _route(leaves: torch.Tensor, n_leaves: int) -> LeafRoute:
+    ids = leaves.reshape(-1)
     n = ids.numel()
     if not ids.is_cuda:
         key = torch.where((ids >= 0) & (ids < n_leaves), ids, n_leaves).to(torch.int64)
@@ -182,7 +187,7 @@ def _embed_grad(dy, ids, route, n_leaves: int, scale: float) -> torch.Tensor:
     """scale * the sum of dy's rows of each leaf, [n_leaves, D]."""
     D = dy.shape[-1]
     if not dy.is_cuda:
-        route = route if route is not None else leaf_route(ids, n_leaves)
+        route = route if route is not None else _route(ids, n_leaves)
         return _sum_by_leaf_plain(dy.reshape(-1, D), route, scale)
     hip, kind, dev = native.hip(), _TYPES[dy.dtype], dy.get_device()
     dy, ids = _rows(dy), ids.contiguous()
@@ -267,7 +272,7 @@ def _linear_forward(x, ids, route, w, b):
     """Returns (y, route): the route is made where the kernel needs one."""
     n, (G, N, K) = x.shape[0], w.shape
     if not x.is_cuda:
-        route = route if route is not None else leaf_route(ids, G)
+        route = route if route is not None else _route(ids, G)
         return _linear_plain(x, route, w, b), route
     hip, kind, dev, ids = native.hip(), _TYPES[x.dtype], x.get_device(), ids.contiguous()
     wide, bias = ids.dtype == torch.int64, 0 if b is None else b.data_ptr()
@@ -312,7 +317,7 @@ class _Linear(torch.autograd.Function):
     def _first(ctx, dy):
         x, w, ids = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        route = ctx.route if ctx.route is not None else leaf_route(ids, w.shape[0])
+        route = ctx.route if ctx.route is not None else _route(ids, w.shape[0])
         if x.is_cuda:
             grads = _linear_grad(dy, x, route, w, need_x, need_w, need_b)
         else:

@@ -384,6 +384,8 @@ def test_refusals():
     with pytest.raises(ValueError, match="n_leaves"):
         leaf_route(ids, 0)
     with pytest.raises(ValueError, match="n_leaves"):
+        leaf_route(ids, 2 ** 30 + 1)
+    with pytest.raises(ValueError, match="n_leaves"):
         leaf_embedding(ids, t[:0])
     with pytest.raises(TypeError, match="float32, float16 or bfloat16"):
         leaf_embedding(ids, t.double())
@@ -422,6 +424,26 @@ def test_changed_leaves_are_noticed():
     ids += 1
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [30, 300])
+def test_a_route_keeps_its_leaves(device, n):
+    # leaf numbers rewritten after the route was made change nothing that follows the route
+    g = gen(n)
+    ids = draw_leaves(g, n, 7, none=0.1).to(device)
+    t = torch.randn(7, 6, generator=g).to(device).requires_grad_()
+    w = torch.randn(7, 5, 6, generator=g).to(device).requires_grad_()
+    r = leaf_route(ids, 7)
+
+    def step():
+        y = leaf_linear(leaf_embedding(r, t), r, w)
+        return (y.detach(), *torch.autograd.grad(y.sum(), (t, w)))
+
+    want = step()
+    ids.zero_()
+    for a, b in zip(want, step()):
+        assert torch.equal(a, b)
 
 
 # ---------------------------------------------------------------- through the estimators
@@ -572,3 +594,132 @@ def test_captured_and_replayed(n):
             torch.cuda.synchronize()
             for a, b in zip(out, want):
                 assert torch.equal(a, b), (k, q)
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed_large():
+    # the largest tiles, in all three directions
+    n, G, K, N = 16_500, 16, 1024, 1032
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+
+    def make(seed):
+        h = gen(seed)
+        return [draw_leaves(h, n, G, skew=0.5, none=0.1).cuda(),
+                *(torch.randn(*shape, generator=h).to(**bf).requires_grad_()
+                  for shape in ((n, K), (G, N, K), (G, N)))]
+
+    def step(ids, x, w, b):
+        y = leaf_linear(x, ids, w, b)
+        return (y.detach(), *torch.autograd.grad(y, (x, w, b), torch.ones_like(y)))
+
+    static = make(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*static)
+    for k in range(3):
+        fresh = make(10 + k)
+        with torch.no_grad():
+            for a, b in zip(static, fresh):
+                a.copy_(b)
+        graph.replay()
+        want = step(*fresh)
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), k
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once():
+    # two streams at work together, each with its own scratch, against the calls one by one
+    g = gen(51)
+    cases = [(20_000, 17, 512, 520), (18_000, 40, 520, 264), (3000, 5, 64, 48)]
+    data = [(draw_leaves(g, n, G, skew=1.0, none=0.05).cuda(),
+             torch.randn(n, K, generator=g).cuda().half().requires_grad_(),
+             (torch.randn(G, N, K, generator=g) * 0.05).cuda().half().requires_grad_(),
+             torch.randn(G, N, generator=g).cuda().half().requires_grad_())
+            for n, G, K, N in cases]
+
+    def step(ids, x, w, b):
+        y = leaf_linear(x, ids, w, b) * leaf_embedding(ids, b)
+        return (y.detach(), *torch.autograd.grad(y, (x, w, b), torch.ones_like(y)))
+
+    want = [step(*d) for d in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    got = []
+    for _ in range(3):
+        for s, d in zip(streams, data):
+            with torch.cuda.stream(s):
+                got.append(step(*d))
+    torch.cuda.synchronize()
+    for i, res in enumerate(got):
+        for a, b in zip(res, want[i % len(data)]):
+            assert torch.equal(a, b), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_operands_past_32_bits(dtype):
+    # rows so far apart that their last offsets pass 2^32 elements, and a table as long
+    n, G, K, N = 8400, 3, 1800, 1816  # (near ones run on the largest tiles)
+    stride = 2 ** 32 // n // 8 * 8 + 4096
+    g = gen(61)
+    big = torch.empty(n * stride, device="cuda", dtype=dtype)
+    x = torch.as_strided(big, (n, K), (stride, 1))
+    dy = torch.as_strided(big, (n, N), (stride, 1), 2048)
+    x.copy_(torch.randn(n, K, generator=g))
+    dy.copy_(torch.randn(n, N, generator=g))
+    ids = draw_leaves(g, n, G, none=0.1).cuda()
+    w = (torch.randn(G, N, K, generator=g) * 0.05).cuda().to(dtype).requires_grad_()
+    px = x.requires_grad_()
+    y = leaf_linear(px, ids, w)
+    far = (y, *torch.autograd.grad(y, (px, w), dy))
+    near = x.detach().contiguous().requires_grad_()
+    y = leaf_linear(near, ids, w)
+    for a, b in zip(far, (y, *torch.autograd.grad(y, (near, w), dy.contiguous()))):
+        # the same terms, in tiles of another size: 32-bit sums of up to 3100 terms of order 1
+        assert torch.allclose(a.float(), b.float(), rtol=2 * torch.finfo(dtype).eps, atol=5e-3)
+    rows = torch.randint(0, n, (500,), generator=g).cuda()
+    assert torch.equal(leaf_embedding(rows, x.detach(), scale=2.0), x.detach()[rows] * 2)
+    p = torch.zeros(G, N, device="cuda", dtype=dtype, requires_grad=True)
+    dt = [torch.autograd.grad(leaf_embedding(ids, p), p, d)[0] for d in (dy, dy.contiguous())]
+    assert torch.equal(*dt)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("n", [40, 700])
+def test_linear_rows_that_are_one_row(device, dtype, n):
+    # an input row and an incoming gradient broadcast over the rows, int32 leaf numbers; every
+    # subset of the gradients is the same as all of them
+    G, K, N = 5, 72, 48
+    g = gen(n)
+    ids = draw_leaves(g, n, G, none=0.1, dtype=torch.int32).to(device)
+    one, d1 = (torch.randn(1, c, generator=g).to(device, dtype) for c in (K, N))
+    w, b = (torch.randn(*s, generator=g).to(device, dtype) for s in ((G, N, K), (G, N)))
+
+    def grads(x, dy, need):
+        args = [t.detach().clone().requires_grad_() if k in need else t.detach()
+                for k, t in zip("xwb", (x, w, b))]
+        y = leaf_linear(args[0], ids, *args[1:])
+        return y, dict(zip(need, torch.autograd.grad(
+            y, [t for t in args if t.requires_grad], dy)))
+
+    want_y, want = grads(one.expand(n, K).contiguous(), d1.expand(n, N).contiguous(), "xwb")
+    for need in ("xwb", "x", "w", "b", "xw", "wb", "xb"):
+        y, got = grads(one.expand(n, K), d1.expand(n, N), need)
+        assert torch.equal(y, want_y)
+        for k in need:
+            if k == "b" and "w" not in need:  # (another kernel's order of its sums)
+                assert torch.allclose(got[k], want[k], rtol=torch.finfo(dtype).eps, atol=1e-3)
+            else:
+                assert torch.equal(got[k], want[k]), (need, k)
+    p = one.detach().clone().requires_grad_()  # ... and the gradient of the row itself
+    (dp,) = torch.autograd.grad(leaf_linear(p.expand(n, K), ids, w), p, d1.expand(n, N))
+    full = want["x"].double().sum(0)
+    assert torch.allclose(dp[0].double(), full, rtol=2 * n * torch.finfo(dtype).eps, atol=1e-1)
