@@ -12,7 +12,7 @@
 //
 // The sort is an LSD radix sort with 8-bit digits: ceil(bits(G) / 8) stable passes, so one up to
 // 255 leaves and three up to 2^24. Up to kLrTile rows one workgroup runs all passes in LDS (one
-// launch); beyond, a pass is a count of every tile's digits and a scatter that takes its own
+// launch; 16384 rows so: 22 us a pass, 12 with the tiles); beyond, a pass is a count of every tile's digits and a scatter that takes its own
 // prefix over the earlier tiles (two launches; with more than kLrSelfTiles tiles a scan between
 // them, since every scatter block reads all tiles' counts). It moves 8 to 16 bytes a row and
 // pass; at a million rows it is bound by its launches and the latency inside them, not by memory.
@@ -24,6 +24,10 @@ constexpr int kLrThreads = 1024;
 constexpr int kLrItems = 4;
 constexpr int kLrTile = kLrThreads * kLrItems;  // 4096 rows
 constexpr int kLrWaves = kLrThreads / kWave;
+// Leaves a row up to which the one workgroup fills the offsets too. us so / with a launch that
+// searches: 4096 rows, 200 leaves 7.3 / 9.9, 16000 leaves 15.3 / 16.5; 1000 rows, 16000 leaves 20.8
+// / 11.8.
+constexpr int kLrFillLeaves = 4;
 constexpr int kLrSelfTiles = 512;
 constexpr int kLrOwn = 16;  // positions a lane fills by itself before the wave helps
 
@@ -86,11 +90,31 @@ __device__ __forceinline__ uint32_t lr_digit_prefix(uint32_t v, uint32_t* s_w4) 
   return before + incl - v;
 }
 
-// ---- up to kLrTile rows: all passes in one workgroup
+// Position i starts every leaf after the key before it, up to its own; a run of more than kLrOwn
+// leaves without rows is filled by the whole wave, all of whose lanes have to come here. i == n:
+// the end, i > n: nothing.
+__device__ __forceinline__ void lr_fill(int64_t i, int64_t n, int64_t prev, int64_t cur, int G,
+                                        int32_t* __restrict__ offsets) {
+  if (i == n) offsets[G + 1] = (int32_t)n;
+  const bool wide = cur - prev > kLrOwn;
+  if (!wide)
+    for (int64_t g = prev + 1; g <= cur; ++g) offsets[g] = (int32_t)i;
+  unsigned long long big = __ballot(wide);
+  while (big) {
+    const int src = __ffsll((long long)big) - 1;
+    big &= big - 1;
+    const int a = __shfl((int)prev, src, kWave), b = __shfl((int)cur, src, kWave);
+    const int v = __shfl((int)i, src, kWave);
+    for (int64_t g = (int64_t)a + 1 + lane_id(); g <= b; g += kWave) offsets[g] = v;
+  }
+}
+
+// ---- up to kLrTile rows: all passes in one workgroup. offsets: null, or filled here.
 __global__ __launch_bounds__(kLrThreads) void lr_small_kernel(const void* __restrict__ ids,
                                                               bool wide, int n, int G, int passes,
                                                               int32_t* __restrict__ order,
-                                                              uint32_t* __restrict__ keys) {
+                                                              uint32_t* __restrict__ keys,
+                                                              int32_t* __restrict__ offsets) {
   __shared__ uint32_t s_key[kLrTile], s_row[kLrTile];
   __shared__ uint32_t s_wh[kLrWaves][256];
   __shared__ uint32_t s_base[256], s_w4[4];
@@ -140,6 +164,17 @@ __global__ __launch_bounds__(kLrThreads) void lr_small_kernel(const void* __rest
       keys[i] = key[k];
     }
   }
+  if (offsets == nullptr) return;
+#pragma unroll
+  for (int k = 0; k < kLrItems; ++k) {
+    const int i = w * (kWave * kLrItems) + k * kWave + lane;
+    lr_fill(i, n, i > 0 && i <= n ? (int64_t)s_key[i - 1] : i == 0 ? -1 : 0,
+            i < n ? (int64_t)key[k] : i == n ? (int64_t)G : 0, G, offsets);
+  }
+  // (all positions taken by rows: the end is one more)
+  if (n == kLrTile && w == kLrWaves - 1)
+    lr_fill(n + lane, n, lane == 0 ? (int64_t)s_key[n - 1] : 0, lane == 0 ? (int64_t)G : 0, G,
+            offsets);
 }
 
 // ---- one pass over many tiles. kFirst: keys come from the leaf indices, rows are 0..n-1
@@ -301,8 +336,7 @@ __global__ __launch_bounds__(256) void lr_offsets_search_kernel(const uint32_t* 
   offsets[g] = lo;
 }
 
-// Many rows: position i starts every leaf after the key before it, up to its own. A run of leaves
-// without rows is filled by the whole wave.
+// Many rows: lr_fill for every position.
 __global__ __launch_bounds__(256) void lr_offsets_fill_kernel(const uint32_t* __restrict__ keys,
                                                               int64_t n, int G,
                                                               int32_t* __restrict__ offsets) {
@@ -312,18 +346,7 @@ __global__ __launch_bounds__(256) void lr_offsets_fill_kernel(const uint32_t* __
     prev = i > 0 ? (int64_t)keys[i - 1] : -1;
     cur = i < n ? (int64_t)keys[i] : (int64_t)G;
   }
-  if (i == n) offsets[G + 1] = (int32_t)n;
-  const bool wide = cur - prev > kLrOwn;
-  if (!wide)
-    for (int64_t g = prev + 1; g <= cur; ++g) offsets[g] = (int32_t)i;
-  unsigned long long big = __ballot(wide);
-  while (big) {
-    const int src = __ffsll((long long)big) - 1;
-    big &= big - 1;
-    const int a = __shfl((int)prev, src, kWave), b = __shfl((int)cur, src, kWave);
-    const int v = __shfl((int)i, src, kWave);
-    for (int64_t g = (int64_t)a + 1 + lane_id(); g <= b; g += kWave) offsets[g] = v;
-  }
+  lr_fill(i, n, prev, cur, G, offsets);
 }
 
 int leaf_route_passes(int G) {
@@ -343,14 +366,17 @@ void launch_leaf_route(hipStream_t stream, const void* ids, bool wide, int64_t n
                        int32_t* order, uint32_t* keys, int32_t* offsets, uint32_t* work) {
   const int passes = leaf_route_passes(G);
   if (n <= kLrTile) {
+    const bool fill = G <= kLrFillLeaves * n;
     if (n > 0) {
       hipLaunchKernelGGL(lr_small_kernel, dim3(1), dim3(kLrThreads), 0, stream, ids, wide, (int)n,
-                         G, passes, order, keys);
+                         G, passes, order, keys, fill ? offsets : nullptr);
       MT_HIP_CHECK(hipGetLastError());
     }
-    hipLaunchKernelGGL(lr_offsets_search_kernel, leaf_grid(((int64_t)G + 2 + 255) / 256), dim3(256),
-                       0, stream, keys, (int)n, G, offsets);
-    MT_HIP_CHECK(hipGetLastError());
+    if (!fill) {
+      hipLaunchKernelGGL(lr_offsets_search_kernel, leaf_grid(((int64_t)G + 2 + 255) / 256),
+                         dim3(256), 0, stream, keys, (int)n, G, offsets);
+      MT_HIP_CHECK(hipGetLastError());
+    }
     return;
   }
   const int T = (int)((n + kLrTile - 1) / kLrTile);
