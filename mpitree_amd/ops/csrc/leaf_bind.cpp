@@ -5,7 +5,7 @@
 
 #include <algorithm>
 
-#include "common.h"
+#include "leaf.h"
 
 namespace py = pybind11;
 
@@ -27,9 +27,9 @@ void launch_leaf_linear_tile(hipStream_t, int, bool, const void*, int64_t, const
                              void*, void*);
 int64_t leaf_linear_tile_bytes(int64_t, int);
 int64_t leaf_linear_grad_bytes(int, int64_t, int, int, int);
-bool launch_leaf_linear_grad(hipStream_t, int, const void*, int64_t, const void*, int64_t,
-                             const int32_t*, const uint32_t*, const int32_t*, int64_t, int, int,
-                             int, void*, void*, void*);
+LlMade launch_leaf_linear_grad(hipStream_t, int, const void*, int64_t, const void*, int64_t,
+                               const int32_t*, const uint32_t*, const int32_t*, int64_t, int,
+                               const void*, int, int, void*, void*, void*, void*);
 
 namespace {
 hipStream_t S(uintptr_t s) { return reinterpret_cast<hipStream_t>(s); }
@@ -134,15 +134,15 @@ void bind_leaf(py::module_& m) {
                                uintptr_t work) {
     const OnDevice on(dev);
     const Route r(route, n);
-    if (dx != 0)
-      launch_leaf_linear_tile(S(s), type, true, P<void>(dy), dy_stride, r.order, r.off, n, G,
-                              P<void>(w), nullptr, K, N, P<void>(dx), P<void>(work));
-    bool made = false;
+    LlMade made{};
     if (dw != 0)
       made = launch_leaf_linear_grad(S(s), type, P<void>(x), x_stride, P<void>(dy), dy_stride,
-                                     r.order, r.keys, r.off, n, G, K, N, P<void>(dw), P<void>(db),
-                                     P<void>(work));
-    if (db != 0 && !made)
+                                     r.order, r.keys, r.off, n, G, P<void>(w), K, N, P<void>(dx),
+                                     P<void>(dw), P<void>(db), P<void>(work));
+    if (dx != 0 && !made.dx)
+      launch_leaf_linear_tile(S(s), type, true, P<void>(dy), dy_stride, r.order, r.off, n, G,
+                              P<void>(w), nullptr, K, N, P<void>(dx), P<void>(work));
+    if (db != 0 && !made.db)
       launch_leaf_embed_grad(S(s), type, P<void>(dy), dy_stride, r.order, r.keys, r.off, n, G, N,
                              1.f, P<void>(db), P<void>(work));
   });

@@ -192,7 +192,8 @@ __device__ __forceinline__ void ll_dma_at(const void* g, const void* lds) {
                : "s"(to), "v"(g)
                : "memory", "m0");
 }
-// every fetch of this wave has landed, and every wave has come here
+// Every fetch of this wave has landed, and every wave has come here. (__syncthreads() does not do:
+// it waits for a wave's own reads and writes of LDS, not for its fetches into LDS.)
 __device__ __forceinline__ void ll_dma_wait() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
@@ -426,11 +427,11 @@ __global__ __launch_bounds__(NW* kWave) void ll_tile_kernel(LlTile a) {
       };
       load(s_j0, s_i0, 0);
       for (int k0 = 0; k0 < a.depth; k0 += 2 * KD) {
-        __syncthreads();
+        ll_dma_wait();
         if (k0 + KD < a.depth) load(s_j1, s_i1, k0 + KD);
         products(s_j0, s_i0);
         if (k0 + KD >= a.depth) break;
-        __syncthreads();
+        ll_dma_wait();
         if (k0 + 2 * KD < a.depth) load(s_j0, s_i0, k0 + 2 * KD);
         products(s_j1, s_i1);
       }
@@ -791,6 +792,8 @@ struct LlGrad {
   const void* dy;
   void* dw;
   void* db;        // null: not made here
+  const void* w;   // with dx: W
+  void* dx;        // rows of K
   float* part;     // [2 * chunks][N][K]
   double* part_b;  // [2 * chunks][N]
   const int32_t* order;
@@ -800,6 +803,12 @@ struct LlGrad {
   int G, N, K, k_tiles, n_tiles;
   int64_t run, units;
 };
+
+// the unit of the i-th blocks: pieces come first, so that no long one is left for the end
+__device__ __forceinline__ int64_t ll_grad_unit(const LlGrad& a, int64_t i) {
+  const int64_t pieces = a.units - a.G;
+  return i < pieces ? a.G + i : i - pieces;
+}
 
 // sorted positions [pa, pb) of a unit; false: there is no such unit
 __device__ __forceinline__ bool ll_grad_rows(const LlGrad& a, int64_t unit, int64_t& pa,
@@ -857,12 +866,28 @@ __device__ __forceinline__ void ll_store_sum(const LlGrad& a, int64_t unit, int 
     a.part_b[(unit - a.G) * a.N + c] = sum;
 }
 
+// zeros to dx of the rows without a leaf: 16 bytes a lane, block `part` of kLlZeroBlocks
+constexpr int kLlZeroBlocks = 64;
+template <typename T>
+__device__ __forceinline__ void ll_grad_zeros(const LlGrad& a, int64_t part) {
+  const int per = a.K / Ll<T>::kEpc;
+  const int64_t first = a.off[a.G], chunks = (a.off[a.G + 1] - first) * per;
+  for (int64_t i = part * kLlThreads + threadIdx.x; i < chunks; i += kLlZeroBlocks * kLlThreads)
+    ((uint4*)((T*)a.dx + (int64_t)a.order[first + i / per] * a.K))[i % per] =
+        make_uint4(0, 0, 0, 0);
+}
+
 // One B x B tile (rows of W, columns of W) of one unit: both operands are gathered rows with the
 // rows as depth, turned. The row numbers of a tile of depth are fetched a tile ahead of the rows.
 // The sums of dy (db) fall out of its fragments, in 64 bits for f32. kAligned: as in
 // ll_tile_kernel.
-template <typename T, int B, bool kAligned>
+//
+// kDx (one tile holds all of W): dx is made of the same tiles of dy, read once for both. Each wave
+// holds 16 columns of the leaf's W and multiplies all rows of a tile with them (B = 32: half of
+// them). Blocks behind the units' write the zeros of the rows without a leaf.
+template <typename T, int B, bool kAligned, bool kDx = false>
 __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
+  static_assert(!kDx || (B <= 64 && kAligned), "");
   using A = std::conditional_t<sizeof(T) == 4, double, float>;
   constexpr int E = Ll<T>::kEpc, KD = Ll<T>::kDepth, kRow = B / E;
   constexpr int S = B / 2 / 16, Q = B * 8 / kLlThreads;  // 2 x 2 waves
@@ -871,8 +896,11 @@ __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
   __shared__ A s_sum[kLlWaves][S * 16];
   const int64_t blk = leaf_block();
   const int tiles = a.n_tiles * a.k_tiles;
-  const int64_t unit = blk / tiles;
-  if (unit >= a.units) return;
+  if (blk >= a.units * tiles) {
+    if constexpr (kDx) ll_grad_zeros<T>(a, blk - a.units);
+    return;
+  }
+  const int64_t unit = ll_grad_unit(a, blk / tiles);
   const int t = (int)(blk % tiles);
   const int j0 = t / a.k_tiles * B, i0 = t % a.k_tiles * B;
   const int tid = threadIdx.x, l = lane_id(), w = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -912,6 +940,38 @@ __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
       }
     }
   };
+  // dx: this wave's columns of W (zeros past its last row), where in a tile a lane's chunks lie
+  constexpr int CW = kDx ? B / 16 : kLlWaves, RJ = KD / 16 * CW / kLlWaves;
+  constexpr int DT = kDx ? (B + 4 * E - 1) / (4 * E) : 1;
+  const int dc = w % CW * 16, dr = w / CW * (RJ * 16);
+  uint4 fw[DT];
+  int at_c[DT];
+  if constexpr (kDx) {
+    const int64_t g = unit < a.G ? unit : (int64_t)a.keys[pa];
+    const T* const wg = (const T*)a.w + g * a.N * a.K + min(dc + (l & 15), a.K - 1);
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      T e[E];
+#pragma unroll
+      for (int u = 0; u < E; ++u) {
+        const int k = (4 * t + (l >> 4)) * E + u;
+        e[u] = ll_load_or_zeros<T>(rows > 0 && k < a.N, wg + (int64_t)k * a.K);
+      }
+      __builtin_memcpy(&fw[t], e, 16);
+      at_c[t] = ll_turn_chunk<T, B>(dr + (l & 15), 4 * t + (l >> 4));
+    }
+  }
+  auto dx_rows = [&](const uint4* sj, int p0, const int32_t (&to)[RJ]) {
+#pragma unroll
+    for (int j = 0; j < RJ; ++j) {
+      f32x4 d = {};
+#pragma unroll
+      for (int t = 0; t < DT; ++t) d = ll_mma<T>(fw[t], sj[j * 16 * kRow + at_c[t]], d);
+      const int c = dc + 4 * (l >> 4);
+      if (p0 + dr + j * 16 + (l & 15) < rows)
+        ll_store4<true>((T*)a.dx + (int64_t)to[j] * a.K + c, d, a.K - c);
+    }
+  };
   if (rows > 0) {
     const T* const x = (const T*)a.x;
     const T* const dy = (const T*)a.dy;
@@ -922,7 +982,12 @@ __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
         row[q] = order[min(p0 + (q * kLlThreads + tid) / kRow, rows - 1)];
     };
     if constexpr (kAligned) {
-      auto load = [&](uint4* sj, uint4* si, int p0) {
+      int32_t to0[RJ], to1[RJ];  // dx: the rows of this lane in either buffer
+      auto load = [&](uint4* sj, uint4* si, int p0, int32_t (&to)[RJ]) {
+        if constexpr (kDx) {
+#pragma unroll
+          for (int j = 0; j < RJ; ++j) to[j] = order[min(p0 + dr + j * 16 + (l & 15), rows - 1)];
+        }
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
           const int id = q * kLlThreads + tid, k = id / kRow;
@@ -930,21 +995,25 @@ __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
           const bool in = p0 + k < rows;
           const T* const pj = dy + row[q] * a.dy_stride + min(j0 + c * E, a.N - E);
           const T* const pi = x + row[q] * a.x_stride + min(i0 + c * E, a.K - E);
-          ll_dma(in ? (const void*)pj : kLlZeros, sj + q * kLlThreads + w * kWave);
+          // (dx sums over dy's columns: zeros behind the last)
+          ll_dma(in && (!kDx || c * E < a.N) ? (const void*)pj : kLlZeros,
+                 sj + q * kLlThreads + w * kWave);
           ll_dma(in ? (const void*)pi : kLlZeros, si + q * kLlThreads + w * kWave);
         }
         next_rows(p0 + KD);
       };
       next_rows(0);
-      load(s_j0, s_i0, 0);
+      load(s_j0, s_i0, 0, to0);
       for (int p0 = 0; p0 < rows; p0 += 2 * KD) {
-        __syncthreads();
-        if (p0 + KD < rows) load(s_j1, s_i1, p0 + KD);
+        ll_dma_wait();
+        if (p0 + KD < rows) load(s_j1, s_i1, p0 + KD, to1);
         products(s_j0, s_i0);
+        if constexpr (kDx) dx_rows(s_j0, p0, to0);
         if (p0 + KD >= rows) break;
-        __syncthreads();
-        if (p0 + 2 * KD < rows) load(s_j0, s_i0, p0 + 2 * KD);
+        ll_dma_wait();
+        if (p0 + 2 * KD < rows) load(s_j0, s_i0, p0 + 2 * KD, to0);
         products(s_j1, s_i1);
+        if constexpr (kDx) dx_rows(s_j1, p0 + KD, to1);
       }
     } else {
       uint4 vj[Q], vi[Q];
@@ -1001,8 +1070,8 @@ __global__ __launch_bounds__(kBigThreads, 2) void ll_big_grad_kernel(LlGrad a) {
   __shared__ alignas(16) char s0[2 * kBigTurnBytes], s1[2 * kBigTurnBytes];  // dy, then x
   const int64_t blk = ll_xcd_order(leaf_block());
   const int tiles = a.n_tiles * a.k_tiles;
-  const int64_t unit = blk / tiles;
-  if (unit >= a.units) return;
+  if (blk >= a.units * tiles) return;
+  const int64_t unit = ll_grad_unit(a, blk / tiles);
   const int t = (int)(blk % tiles);
   const int j0 = t / a.k_tiles * kBig, i0 = t % a.k_tiles * kBig;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -1093,143 +1162,91 @@ __global__ __launch_bounds__(kBigThreads, 2) void ll_big_grad_kernel(LlGrad a) {
   ll_grad_store<T, SJ, SI>(acc, a, unit, j0 + wj, i0 + wi);
 }
 
-// The same for f32 and few columns on either side: the waves of a block take 16 rows in turn, from
-// memory straight into fragments, each for the whole 16 SJ x 16 SI tile, and their sums meet in
-// LDS. The sums of dy (db) fall out of its fragments, in 64 bits.
-template <int SJ, int SI>
-__global__ __launch_bounds__(kLlThreads) void ll_rows_grad_kernel(LlGrad a) {
-  __shared__ f32x4 s_acc[2][SJ * SI][kWave];
-  __shared__ double s_b[kLlWaves][SJ * 16];
-  const int64_t blk = leaf_block();
-  const int tiles = a.n_tiles * a.k_tiles;
-  const int64_t unit = blk / tiles;
-  if (unit >= a.units) return;
-  const int t = (int)(blk % tiles);
-  const int j0 = t / a.k_tiles * (SJ * 16), i0 = t % a.k_tiles * (SI * 16);
-  const int l = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  int64_t pa, pb;
-  if (!ll_grad_rows(a, unit, pa, pb)) return;
-  const int rows = (int)(pb - pa);
-  const int32_t* const order = a.order + pa;
-  const float* const x = (const float*)a.x + i0 + (l & 15);
-  const float* const dy = (const float*)a.dy + j0 + (l & 15);
-
-  f32x4 acc[SJ][SI] = {};
-  double sum[SJ] = {};
-  auto load = [&](int p, f32x4 (&fj)[SJ], f32x4 (&fi)[SI]) {
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int q = p + 4 * (l >> 4) + u;
-      const int64_t row = q < rows ? order[q] : -1;
-#pragma unroll
-      for (int j = 0; j < SJ; ++j)
-        fj[j][u] = row >= 0 && j0 + j * 16 + (l & 15) < a.N ? dy[row * a.dy_stride + j * 16] : 0.f;
-#pragma unroll
-      for (int i = 0; i < SI; ++i)
-        fi[i][u] = row >= 0 && i0 + i * 16 + (l & 15) < a.K ? x[row * a.x_stride + i * 16] : 0.f;
-    }
-  };
-  auto products = [&](const f32x4 (&fj)[SJ], const f32x4 (&fi)[SI]) {
-#pragma unroll
-    for (int j = 0; j < SJ; ++j) {
-#pragma unroll
-      for (int i = 0; i < SI; ++i)
-        acc[j][i] = ll_mma<float>(__builtin_bit_cast(uint4, fi[i]),
-                                  __builtin_bit_cast(uint4, fj[j]), acc[j][i]);
-      sum[j] += ((double)fj[j][0] + fj[j][1]) + ((double)fj[j][2] + fj[j][3]);
-    }
-  };
-  constexpr int kTurn = 16 * kLlWaves;
-  f32x4 fj0[SJ], fi0[SI], fj1[SJ], fi1[SI];
-  int p = 16 * w;
-  load(p, fj0, fi0);
-  for (; p < rows; p += 2 * kTurn) {
-    load(p + kTurn, fj1, fi1);
-    products(fj0, fi0);
-    load(p + 2 * kTurn, fj0, fi0);
-    products(fj1, fi1);
-  }
-  // waves 2, 3 hand theirs to 0, 1, then 1 to 0
-#pragma unroll
-  for (int half = 2; half > 0; half >>= 1) {
-    if (w >= half && w < 2 * half) {
-#pragma unroll
-      for (int j = 0; j < SJ; ++j)
-#pragma unroll
-        for (int i = 0; i < SI; ++i) s_acc[w - half][j * SI + i][l] = acc[j][i];
-    }
-    __syncthreads();
-    if (w < half) {
-#pragma unroll
-      for (int j = 0; j < SJ; ++j)
-#pragma unroll
-        for (int i = 0; i < SI; ++i) acc[j][i] += s_acc[w][j * SI + i][l];
-    }
-    __syncthreads();
-  }
-  if (a.db != nullptr && i0 == 0) {
-#pragma unroll
-    for (int j = 0; j < SJ; ++j) {
-      sum[j] += __shfl_xor(sum[j], 16, kWave);
-      sum[j] += __shfl_xor(sum[j], 32, kWave);
-      if (l < 16) s_b[w][j * 16 + l] = sum[j];
-    }
-    __syncthreads();
-    const int c = threadIdx.x;
-    if (c < SJ * 16 && j0 + c < a.N) {
-      ll_store_sum<float>(a, unit, j0 + c, (s_b[0][c] + s_b[1][c]) + (s_b[2][c] + s_b[3][c]));
-    }
-  }
-  if (w == 0) ll_grad_store<float, SJ, SI>(acc, a, unit, j0, i0);
-}
-
 // Adds the partial matrices of the leaves with more than `run` rows, in 64 bits for f32 (and their
-// partial sums of dy, where the kernel above made them): one block per chunk in which such a leaf
-// starts, up to 512 times, each taking 4 elements a thread in turn.
+// partial sums of dy, where the kernel above made them). Such leaves are looked for among the
+// leaves, or, if these are fewer, among the chunks in which they start: `per` blocks each, which
+// take a leaf's elements in turn, 4 a lane. Up to 16 waves share a leaf's pieces and meet in LDS,
+// so that many pieces of a small matrix are not one chain of loads (1M rows of one leaf, 64 x 64
+// f32: 342 -> 218 us).
+constexpr int kLlJoinThreads = 1024, kLlJoinWaves = kLlJoinThreads / kWave;
 template <typename T>
-__global__ __launch_bounds__(kLlThreads) void ll_join_kernel(LlGrad a, int64_t blocks_per_chunk,
-                                                             int64_t chunks) {
+__global__ __launch_bounds__(kLlJoinThreads) void ll_join_kernel(LlGrad a, bool by_leaf, int per) {
   using A = std::conditional_t<sizeof(T) == 4, double, float>;
-  const int64_t blk = leaf_block();
-  const int64_t c = blk / blocks_per_chunk, m = a.off[a.G];
-  const int64_t ca = c * a.run, cb = min<int64_t>(ca + a.run, m);
-  if (c >= chunks || ca >= m) return;
-  const int64_t k0 = a.keys[ca], k1 = a.keys[cb - 1];
-  const int64_t s1 = a.off[k1], e1 = a.off[k1 + 1];
-  if (s1 < ca || e1 - s1 <= a.run) return;
-  const int64_t size = (int64_t)a.N * a.K;
-  const int64_t last = (e1 - 1) / a.run;
-  const int64_t slot0 = 2 * c + (k1 != k0 ? 1 : 0);
-  const int64_t e0 = ((blk % blocks_per_chunk) * kLlThreads + threadIdx.x) * 4;
-  const int64_t stride = blocks_per_chunk * kLlThreads * 4;
-  if (size % 4 == 0) {
-    for (int64_t e = e0; e < size; e += stride) {
-      A sum[4] = {};
-      for (int64_t p = c; p <= last; ++p) {
-        const f32x4 v = *(const f32x4*)(a.part + (p == c ? slot0 : 2 * p) * size + e);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) sum[u] += (A)v[u];
-      }
-      LeafVec<T, 4> o;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) o.v[u] = leaf_from<T>((float)sum[u]);
-      *(LeafVec<T, 4>*)((T*)a.dw + k1 * size + e) = o;
-    }
+  __shared__ A s_sum[kLlJoinWaves][4][kWave];
+  __shared__ double s_b[kLlJoinWaves][kWave];
+  const int64_t blk = leaf_block(), i0 = blk / per, m = a.off[a.G];
+  int64_t k1 = i0;
+  if (by_leaf) {
+    if (i0 >= a.G) return;
   } else {
-    for (int64_t e = e0; e < size; e += stride)
-      for (int u = 0; u < 4 && e + u < size; ++u) {
-        A sum = 0;
-        for (int64_t p = c; p <= last; ++p)
-          sum += (A)a.part[(p == c ? slot0 : 2 * p) * size + e + u];
-        ((T*)a.dw)[k1 * size + e + u] = leaf_from<T>((float)sum);
-      }
+    if (i0 * a.run >= m) return;
+    k1 = a.keys[min<int64_t>((i0 + 1) * a.run, m) - 1];
   }
-  if (a.db != nullptr && blk % blocks_per_chunk == 0) {
-    for (int n = threadIdx.x; n < a.N; n += kLlThreads) {
-      double sum = 0;
-      for (int64_t p = c; p <= last; ++p) sum += a.part_b[(p == c ? slot0 : 2 * p) * a.N + n];
+  const int64_t s1 = a.off[k1], e1 = a.off[k1 + 1];
+  if (e1 - s1 <= a.run || (!by_leaf && s1 < i0 * a.run)) return;
+  const int64_t c = s1 / a.run, k0 = a.keys[c * a.run];
+  const int64_t size = (int64_t)a.N * a.K;
+  const int pieces = (int)((e1 - 1) / a.run - c) + 1;
+  // piece i's place in the partial matrices
+  auto place = [&](int i) { return i == 0 ? 2 * c + (k1 != k0 ? 1 : 0) : 2 * (c + i); };
+  int share = 1;  // waves that share the pieces of the same elements
+  while (share < kLlJoinWaves && 2 * share <= pieces) share <<= 1;
+  const int l = lane_id(), w = threadIdx.x / kWave, q = w & (share - 1), sub = w / share;
+  const int64_t step = (int64_t)(kLlJoinWaves / share) * kWave * 4;
+  for (int64_t b0 = (blk % per) * step; b0 < size; b0 += per * step) {
+    const int64_t e = b0 + (sub * kWave + l) * 4;
+    A sum[4] = {};
+    if (e < size) {
+      if (size % 4 == 0) {
+#pragma unroll 8
+        for (int i = q; i < pieces; i += share) {
+          const f32x4 v = *(const f32x4*)(a.part + place(i) * size + e);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) sum[u] += (A)v[u];
+        }
+      } else {
+        for (int i = q; i < pieces; i += share)
+          for (int u = 0; u < 4 && e + u < size; ++u) sum[u] += (A)a.part[place(i) * size + e + u];
+      }
+    }
+    if (share > 1) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s_sum[w][u][l] = sum[u];
+      __syncthreads();
+      if (q == 0) {
+        for (int i = 1; i < share; ++i)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) sum[u] += s_sum[w + i][u][l];
+      }
+      __syncthreads();
+    }
+    if (q == 0 && e < size) {
+      T* const to = (T*)a.dw + k1 * size + e;
+      if (size % 4 == 0) {
+        LeafVec<T, 4> o;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) o.v[u] = leaf_from<T>((float)sum[u]);
+        *(LeafVec<T, 4>*)to = o;
+      } else {
+        for (int u = 0; u < 4 && e + u < size; ++u) to[u] = leaf_from<T>((float)sum[u]);
+      }
+    }
+  }
+  if (a.db == nullptr || blk % per != 0) return;
+  for (int n0 = 0; n0 < a.N; n0 += kLlJoinThreads / share) {
+    const int n = n0 + sub * kWave + l;
+    double sum = 0;
+    if (n < a.N) {
+#pragma unroll 8
+      for (int i = q; i < pieces; i += share) sum += a.part_b[place(i) * a.N + n];
+    }
+    s_b[w][l] = sum;
+    __syncthreads();
+    if (q == 0 && n < a.N) {
+      for (int i = 1; i < share; ++i) sum += s_b[w + i][l];
       ((T*)a.db)[k1 * a.N + n] = leaf_from<T>((float)sum);
     }
+    __syncthreads();
   }
 }
 
@@ -1466,36 +1483,42 @@ void launch_leaf_linear_tile(hipStream_t s, int type, bool dx, const void* src, 
 
 // Rows a dW unit may have, a power of two; leaves with more are cut, and a cut costs a partial
 // matrix in 32 bits, written and read. Where whole leaves make 2048 tiles, only those above four
-// times the mean are cut; otherwise pieces make up to 512 tiles (256 of the largest). us as chosen,
-// and with other cuts: 16384 rows of one leaf, 1024 x 1024 bf16 55, with twice the pieces 77; 1M
-// rows of 8 leaves, 64 x 64 f32 208, with four times the pieces 297; 10007 rows of 12 leaves of
-// very different sizes, 1000 x 601 f16 57, with half the pieces 50.
+// times the mean are cut (us with 1, 2, 4, 8 times: 1M rows of 4096 leaves, 64 x 64 f32 227, 189,
+// 176, 192; 65536 rows of 64 leaves, 2048 x 2048 bf16 1452, 953, 830, 891). Otherwise pieces make
+// up to 1024 tiles of 32, 512 of 64 and 128, 256 of 256 (500k rows of 2000 leaves, 32 x 32 f32 38
+// with 512, 33 with 1024, 43 with 2048; 1M rows of 64 leaves, 64 x 64 bf16 75 with 512, 81 with
+// 1024; 16384 rows of one leaf, 1024 x 1024 bf16 55 with 256, 77 with 512).
 static int64_t ll_grad_run(int64_t n, int G, int b, int64_t tiles) {
   int64_t run = 256;
   if (G * tiles >= 2048) {
     while (run < 4 * (n / G)) run <<= 1;
   } else {
-    while (run < (1 << 20) && n / run * tiles > (b == kBig ? 256 : 512)) run <<= 1;
+    const int most = b == 32 ? 1024 : b == kBig ? 256 : 512;
+    while (run < (1 << 20) && n / run * tiles > most) run <<= 1;
   }
   return run;
 }
 // Tile edge of dW; direct: operands are 16-byte aligned and lie within 4 GiB. 256 where leaves are
 // long and fill the GPU, whole or in pieces; bf16 1024 x 1024, us with 256 / 128: 4096 rows in 4
 // leaves 39 / 22, in 16 25 / 31, in 64 68 / 57; 16384 rows in 1 55 / 61, in 16 44 / 62, in 64 81 /
-// 90.
+// 90. 32 for short rows (500k rows of 2000 leaves, 32 x 32 f32 37, 83 with 64).
 static int ll_grad_tile(int type, bool direct, int64_t n, int G, int K, int N) {
   const int64_t big = (int64_t)((N + kBig - 1) / kBig) * ((K + kBig - 1) / kBig);
   if (type != kLeafF32 && direct && N > 128 && K > 128 && n / G >= 256 &&
       (G * big >= 256 || (n / 256) * big >= 1024))
     return kBig;
-  return N > 64 && K > 64 ? 128 : 64;
+  return N > 64 && K > 64 ? 128 : N > 32 || K > 32 ? 64 : 32;
 }
 static int64_t ll_grad_tiles(int b, int K, int N) {
   return (int64_t)((N + b - 1) / b) * ((K + b - 1) / b);
 }
 
-// f32 with few columns on either side: ll_rows_grad_kernel
-static bool ll_short_grad(int type, int K, int N) { return type == kLeafF32 && K <= 32 && N <= 16; }
+// dx together with dW, where one tile holds W and there are leaves enough; us together / apart: 1M
+// rows, 64 x 64: 4096 leaves f32 294 / 350, bf16 146 / 177, 64 leaves f32 374 / 352, bf16 164 /
+// 148; 500k rows, 32 x 32: 2000 leaves f32 57 / 68, 50 leaves 69 / 66, bf16 30 leaves 43 / 51.
+static bool ll_fuse_dx(int b, int G, int K, int N) {
+  return N <= b && K <= b && (b == 32 || (b == 64 && G >= 2048));
+}
 
 // scratch for the partial matrices (and sums), whichever tile is taken
 int64_t leaf_linear_grad_bytes(int type, int64_t n, int G, int K, int N) {
@@ -1508,11 +1531,12 @@ int64_t leaf_linear_grad_bytes(int type, int64_t n, int G, int K, int N) {
   return 2 * chunks * ((int64_t)N * K * 4 + 8 * N + 8);
 }
 
-// dW, and db where it is asked for (not null); true: db was made
-bool launch_leaf_linear_grad(hipStream_t s, int type, const void* x, int64_t x_stride,
-                             const void* dy, int64_t dy_stride, const int32_t* order,
-                             const uint32_t* keys, const int32_t* off, int64_t n, int G, int K,
-                             int N, void* dw, void* db, void* work) {
+// dW, and dx and db where they are asked for (not null); whether they were made here
+LlMade launch_leaf_linear_grad(hipStream_t s, int type, const void* x, int64_t x_stride,
+                               const void* dy, int64_t dy_stride, const int32_t* order,
+                               const uint32_t* keys, const int32_t* off, int64_t n, int G,
+                               const void* w, int K, int N, void* dx, void* dw, void* db,
+                               void* work) {
   LlGrad a{};
   a.x = x, a.dy = dy, a.dw = dw, a.part = (float*)work;
   a.order = order, a.keys = keys, a.off = off;
@@ -1538,28 +1562,34 @@ bool launch_leaf_linear_grad(hipStream_t s, int type, const void* x, int64_t x_s
     const int64_t all = a.units * tiles;
     if (b != kBig) a.db = db;
     a.part_b = (double*)((char*)work + (2 * chunks * (int64_t)N * K * 4 + 7) / 8 * 8);
-    if (ll_short_grad(type, K, N)) {
-      if constexpr (sizeof(T) == 4) run(ll_rows_grad_kernel<1, 2>, all, kLlThreads);
-    } else if (b == kBig) {
+    auto tile = [&](auto edge) {
+      if constexpr (edge() <= 64) {
+        if (a.dx != nullptr)
+          return run(ll_grad_kernel<T, edge(), true, true>, all + kLlZeroBlocks, kLlThreads);
+      }
+      al ? run(ll_grad_kernel<T, edge(), true>, all, kLlThreads)
+         : run(ll_grad_kernel<T, edge(), false>, all, kLlThreads);
+    };
+    if (dx != nullptr && al && ll_aligned<T>({dx}, {}) && ll_fuse_dx(b, G, K, N))
+      a.w = w, a.dx = dx;
+    if (b == kBig) {
       if constexpr (sizeof(T) == 2) run(ll_big_grad_kernel<T>, ll_xcd_blocks(all), kBigThreads);
-    } else if (b == 128) {
-      al ? run(ll_grad_kernel<T, 128, true>, all, kLlThreads)
-         : run(ll_grad_kernel<T, 128, false>, all, kLlThreads);
     } else {
-      al ? run(ll_grad_kernel<T, 64, true>, all, kLlThreads)
-         : run(ll_grad_kernel<T, 64, false>, all, kLlThreads);
+      b == 128  ? tile(LlInt<128>{})
+      : b == 64 ? tile(LlInt<64>{})
+                : tile(LlInt<32>{});
     }
     if (chunks > 0) {
-      // (few chunks hold such a leaf's start: at most 512 blocks each, or the empty ones take
-      // longer)
-      const int64_t per =
-          std::min<int64_t>(512, ((int64_t)N * K + 4 * kLlThreads - 1) / (4 * kLlThreads));
-      hipLaunchKernelGGL(ll_join_kernel<T>, leaf_grid(chunks * per), dim3(kLlThreads), 0, s, a, per,
-                         chunks);
+      // (a block that finds nothing to do costs 5 ns: more of them only for large matrices)
+      const int64_t starts = std::min<int64_t>(G, chunks), size = (int64_t)N * K;
+      const int64_t per = std::clamp<int64_t>(std::max<int64_t>(1024, size / 512) / starts, 1,
+                                              std::min<int64_t>(512, (size + 255) / 256));
+      hipLaunchKernelGGL(ll_join_kernel<T>, leaf_grid(starts * per), dim3(kLlJoinThreads), 0, s, a,
+                         G <= chunks, (int)per);
       MT_HIP_CHECK(hipGetLastError());
     }
   });
-  return a.db != nullptr;
+  return LlMade{a.dx != nullptr, a.db != nullptr};
 }
 
 }  // namespace mt

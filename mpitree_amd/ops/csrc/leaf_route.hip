@@ -12,10 +12,12 @@
 //
 // The sort is an LSD radix sort with 8-bit digits: ceil(bits(G) / 8) stable passes, so one up to
 // 255 leaves and three up to 2^24. Up to kLrTile rows one workgroup runs all passes in LDS (one
-// launch; 16384 rows so: 22 us a pass, 12 with the tiles); beyond, a pass is a count of every tile's digits and a scatter that takes its own
-// prefix over the earlier tiles (two launches; with more than kLrSelfTiles tiles a scan between
-// them, since every scatter block reads all tiles' counts). It moves 8 to 16 bytes a row and
-// pass; at a million rows it is bound by its launches and the latency inside them, not by memory.
+// launch; 16384 rows so: 22 us a pass, 12 with the tiles); beyond, a pass is a count of every
+// tile's digits and a scatter that takes its own prefix over the earlier tiles (two launches; with
+// more than kLrSelfTiles tiles a scan between them, since every scatter block reads all counts).
+// It moves 8 to 16 bytes a row and pass; at a million rows it is bound by its launches and the
+// latency inside them, not by memory: 19 us with 64 leaves, 41 with 4096; 100k rows of 1500 leaves
+// 25.
 #include "leaf.h"
 
 namespace mt {

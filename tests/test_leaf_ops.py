@@ -238,6 +238,32 @@ def test_linear_long_leaves(dtype, skew):
     linear_case("cuda", 40_000, 9, 24, 20, dtype, bias=True, skew=skew, none=0.05)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,G,K,N,skew", [(9000, 2300, 64, 48, 0.3), (9000, 2300, 40, 64, 2.0),
+                                          (2000, 3000, 24, 64, 0.0), (5000, 600, 32, 24, 1.5)])
+def test_linear_many_leaves(device, dtype, n, G, K, N, skew):
+    # row and weight gradients from one pass over dy; leaves that are cut, leaves without rows
+    linear_case(device, n, G, K, N, dtype, bias=True, skew=skew, none=0.1)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K,N,G", [(24, 24, 3), (64, 40, 2100), (200, 24, 3)])
+def test_linear_inf_in_an_incoming_gradient(device, dtype, K, N, G):
+    # it reaches its own row's gradient as inf, not as NaN from padding behind the last column
+    n, g = 400, gen(K + N)
+    x, w, dy = torch.randn(n, K, generator=g), torch.rand(G, N, K, generator=g) + 0.5, \
+        torch.rand(n, N, generator=g)
+    dy[7, N - 1] = float("inf")
+    ids = draw_leaves(g, n, G)
+    px, pw = (t.to(device, dtype).requires_grad_() for t in (x, w))
+    y = leaf_linear(px, ids.to(device), pw)
+    dx, _ = torch.autograd.grad(y, (px, pw), dy.to(device, dtype))
+    assert (dx[7] == float("inf")).all()
+    assert torch.isfinite(dx[:7]).all() and torch.isfinite(dx[8:]).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,G,K,N,skew", [(33_000, 21, 1032, 1048, 0.0),
