@@ -34,10 +34,11 @@ struct LeAcc<float> {
   using type = double;
 };
 
-// Columns of a lane: NC vectors of W elements, a vector every `tpr` lanes of the column block.
+// Columns of a lane: one vector of W elements. (Several, with the row's number read once for all of
+// them, take longer: 2048 columns of f16 290 us with four, 261 with one.)
 struct LeCols {
   int tpr_shift;   // lanes of a row's group: 1 << tpr_shift, at most 64
-  int col_blocks;  // column blocks of tpr * NC * W columns
+  int col_blocks;  // column blocks of tpr * W columns
 };
 
 // kWave: a row's group is a whole wave, so the row's number and address are scalars (63 columns of
@@ -54,7 +55,7 @@ __device__ __forceinline__ int64_t le_same(int64_t v) {
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
-template <typename T, int W, int NC, bool kWide, bool kWave>
+template <typename T, int W, bool kWide, bool kWave>
 __global__ __launch_bounds__(kLeThreads) void le_forward_kernel(
     const void* __restrict__ ids, const T* __restrict__ table, int64_t stride, int64_t n,
     int64_t V, int D, float scale, LeCols lc, T* __restrict__ y) {
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(kLeThreads) void le_forward_kernel(
   const int lr = threadIdx.x & (tpr - 1);
   const int64_t blk = leaf_block();
   const int64_t r0 = (blk / lc.col_blocks) * (rpb * kUnroll) + sub;
-  const int c0 = ((int)(blk % lc.col_blocks) * NC * tpr + lr) * W;
+  const int c = ((int)(blk % lc.col_blocks) * tpr + lr) * W;
   int64_t id[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
@@ -73,25 +74,21 @@ __global__ __launch_bounds__(kLeThreads) void le_forward_kernel(
     if (r < n) id[u] = kWide ? ((const int64_t*)ids)[r] : (int64_t)((const int32_t*)ids)[r];
     id[u] = le_same<kWave>(id[u]);
   }
+  if (c >= D) return;
+  LeafVec<T, W> v[kUnroll];
 #pragma unroll
-  for (int q = 0; q < NC; ++q) {
-    const int c = c0 + q * tpr * W;
-    if (c >= D) break;
-    LeafVec<T, W> v[kUnroll];
+  for (int u = 0; u < kUnroll; ++u) {
+    v[u] = LeafVec<T, W>{};
+    if ((uint64_t)id[u] < (uint64_t)V)
+      v[u] = *(const LeafVec<T, W>*)(table + id[u] * stride + c);
+  }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      v[u] = LeafVec<T, W>{};
-      if ((uint64_t)id[u] < (uint64_t)V)
-        v[u] = *(const LeafVec<T, W>*)(table + id[u] * stride + c);
-    }
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t r = r0 + (int64_t)u * rpb;
+    if (r >= n) break;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t r = r0 + (int64_t)u * rpb;
-      if (r >= n) break;
-#pragma unroll
-      for (int e = 0; e < W; ++e) v[u].v[e] = leaf_from<T>(leaf_f32(v[u].v[e]) * scale);
-      *(LeafVec<T, W>*)(y + r * D + c) = v[u];
-    }
+    for (int e = 0; e < W; ++e) v[u].v[e] = leaf_from<T>(leaf_f32(v[u].v[e]) * scale);
+    *(LeafVec<T, W>*)(y + r * D + c) = v[u];
   }
 }
 
@@ -236,13 +233,12 @@ __global__ __launch_bounds__(kLeThreads) void le_join_kernel(
   if (sub == 0 && c0 < D) le_store<T, W, A>(dtable + (int64_t)k * D + c0, scale, acc);
 }
 
-static LeCols le_cols(int D, int W, int NC) {
+static LeCols le_cols(int D, int W) {
   const int vecs = (D + W - 1) / W;
   LeCols lc;
   lc.tpr_shift = 0;
   while (lc.tpr_shift < 6 && (1 << lc.tpr_shift) < vecs) ++lc.tpr_shift;
-  const int per = NC << lc.tpr_shift;
-  lc.col_blocks = (vecs + per - 1) / per;
+  lc.col_blocks = (vecs + (1 << lc.tpr_shift) - 1) >> lc.tpr_shift;
   return lc;
 }
 
@@ -277,9 +273,7 @@ static void le_dispatch_32(int W, F f) {
 template <typename T, int W>
 static void le_forward(hipStream_t s, const void* ids, bool wide, const T* table, int64_t stride,
                        int64_t n, int64_t V, int D, float scale, T* y) {
-  // wide rows: four vectors a lane while that leaves no lane idle
-  const bool four = D >= 4 * kWave * W;
-  const LeCols lc = le_cols(D, W, four ? 4 : 1);
+  const LeCols lc = le_cols(D, W);
   const int rows = (kLeThreads >> lc.tpr_shift) * le_unroll(W * (int)sizeof(T));
   const dim3 grid = leaf_grid((n + rows - 1) / rows * lc.col_blocks);
   auto go = [&](auto kern) {
@@ -287,15 +281,10 @@ static void le_forward(hipStream_t s, const void* ids, bool wide, const T* table
                        y);
     MT_HIP_CHECK(hipGetLastError());
   };
-  if (four)
-    wide ? go(le_forward_kernel<T, W, 4, true, true>)
-         : go(le_forward_kernel<T, W, 4, false, true>);
-  else if (lc.tpr_shift == 6)
-    wide ? go(le_forward_kernel<T, W, 1, true, true>)
-         : go(le_forward_kernel<T, W, 1, false, true>);
+  if (lc.tpr_shift == 6)
+    wide ? go(le_forward_kernel<T, W, true, true>) : go(le_forward_kernel<T, W, false, true>);
   else
-    wide ? go(le_forward_kernel<T, W, 1, true, false>)
-         : go(le_forward_kernel<T, W, 1, false, false>);
+    wide ? go(le_forward_kernel<T, W, true, false>) : go(le_forward_kernel<T, W, false, false>);
 }
 
 void launch_leaf_embed(hipStream_t s, int type, const void* ids, bool wide, const void* table,
@@ -320,17 +309,21 @@ void launch_leaf_embed(hipStream_t s, int type, const void* ids, bool wide, cons
 }
 
 // Sorted positions of a chunk: 16 to 256, so few that the chunks make about 4096 waves (16 on each
-// CU); longer chunks leave fewer partial rows.
-static int le_run_shift(int64_t n, const LeCols& lc) {
+// CU) of 16-byte vectors, 2048 of narrower ones; longer chunks leave fewer partial rows. us with
+// 1024 or 2048 / 4096 / 8192 or 16384 waves: 1M rows, 63 columns of f32 66 / 79 / 111; 200k rows,
+// 2048 columns of f16 302 / 290 / 303.
+static int le_run_shift(int64_t n, const LeCols& lc, int bytes) {
+  const int64_t waves = bytes >= 16 ? 4096 : 2048;
   int shift = 8;
-  while (shift > 4 && ((n >> shift) * lc.col_blocks << lc.tpr_shift) / kWave < 4096) --shift;
+  while (shift > 4 && ((n >> shift) * lc.col_blocks << lc.tpr_shift) / kWave < waves) --shift;
   return shift;
 }
 
 // bytes of scratch for the partial rows, whichever width is taken
 int64_t leaf_embed_grad_bytes(int type, int64_t n, int D) {
+  const int elem = type == kLeafF32 ? 4 : 2;
   int shift = 8;
-  for (int W : {8, 4, 2, 1}) shift = std::min(shift, le_run_shift(n, le_cols(D, W, 1)));
+  for (int W : {8, 4, 2, 1}) shift = std::min(shift, le_run_shift(n, le_cols(D, W), W * elem));
   return ((n >> shift) + 1) * (2 * (int64_t)D * (type == kLeafF32 ? 8 : 4) + 4);
 }
 
@@ -339,8 +332,8 @@ static void le_backward(hipStream_t s, const T* dy, int64_t stride, const int32_
                         const uint32_t* keys, const int32_t* off, int64_t n, int64_t V, int D,
                         float scale, T* dtable, void* work) {
   using A = typename LeAcc<T>::type;
-  const LeCols lc = le_cols(D, W, 1);
-  const int rpb = kLeThreads >> lc.tpr_shift, shift = le_run_shift(n, lc);
+  const LeCols lc = le_cols(D, W);
+  const int rpb = kLeThreads >> lc.tpr_shift, shift = le_run_shift(n, lc, W * (int)sizeof(T));
   const int64_t chunks = (n + (1 << shift) - 1) >> shift;
   const int64_t chunk_blocks = (chunks + rpb - 1) / rpb * lc.col_blocks;
   const int64_t empty = (V + rpb * kLeEmpty - 1) / (rpb * kLeEmpty);
