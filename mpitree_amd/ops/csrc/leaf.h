@@ -20,10 +20,10 @@ struct LlMade {
   bool dx, db;
 };
 
-// A launch of `total` blocks of 256 threads: HIP's limit is 2^32 threads in a grid's x, so
+// A launch of `total` blocks of up to 1024 threads: a grid's x has to stay below 2^32 threads, so
 // more blocks go to y; kernels number them with leaf_block() and leave past `total`.
 inline dim3 leaf_grid(int64_t total) {
-  constexpr int64_t kX = 1 << 22;
+  constexpr int64_t kX = 1 << 21;
   if (total <= kX) return dim3((unsigned)total);
   const int64_t y = (total + kX - 1) / kX;
   if (y > 65535) throw std::runtime_error("leaf operator: too many blocks for one launch");
