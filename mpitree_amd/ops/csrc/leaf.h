@@ -15,11 +15,6 @@ namespace mt {
 // element types as the bindings number them
 enum LeafType { kLeafF32 = 0, kLeafF16 = 1, kLeafBF16 = 2 };
 
-// which gradients launch_leaf_linear_grad made beside dW
-struct LlMade {
-  bool dx, db;
-};
-
 // A launch of `total` blocks of up to 1024 threads: a grid's x has to stay below 2^32 threads, so
 // more blocks go to y; kernels number them with leaf_block() and leave past `total`.
 inline dim3 leaf_grid(int64_t total) {

@@ -22,14 +22,14 @@ void launch_leaf_embed_grad(hipStream_t, int, const void*, int64_t, const int32_
 int leaf_linear_small_rows();
 void launch_leaf_linear_small(hipStream_t, int, const void*, int64_t, const void*, bool, int, int,
                               const void*, const void*, int, int, void*);
-void launch_leaf_linear_tile(hipStream_t, int, bool, const void*, int64_t, const int32_t*,
-                             const int32_t*, int64_t, int, const void*, const void*, int, int,
-                             void*, void*);
-int64_t leaf_linear_tile_bytes(int64_t, int);
-int64_t leaf_linear_grad_bytes(int, int64_t, int, int, int);
-LlMade launch_leaf_linear_grad(hipStream_t, int, const void*, int64_t, const void*, int64_t,
-                               const int32_t*, const uint32_t*, const int32_t*, int64_t, int,
-                               const void*, int, int, void*, void*, void*, void*);
+int64_t leaf_linear_bytes(int, const void*, int64_t, const void*, int64_t, int, int, int);
+void launch_leaf_linear(hipStream_t, int, const void*, int64_t, const int32_t*, const int32_t*,
+                        int64_t, int, const void*, const void*, int, int, void*, void*);
+int64_t leaf_linear_grad_bytes(int, const void*, int64_t, const void*, int64_t, const void*,
+                               int64_t, int, int, int, bool, bool);
+void launch_leaf_linear_grad(hipStream_t, int, const void*, int64_t, const void*, int64_t,
+                             const int32_t*, const uint32_t*, const int32_t*, int64_t, int,
+                             const void*, int, int, void*, void*, void*, void*);
 
 namespace {
 hipStream_t S(uintptr_t s) { return reinterpret_cast<hipStream_t>(s); }
@@ -109,8 +109,10 @@ void bind_leaf(py::module_& m) {
                              P<void>(w), P<void>(bias), K, N, P<void>(y));
   });
   // ids != 0: the rows are sorted into `route` first; else it holds the sort
-  m.def("leaf_linear_bytes", [](int64_t n, int G) {
-    return std::max(4 * leaf_route_words(n, G), leaf_linear_tile_bytes(n, G));
+  m.def("leaf_linear_bytes", [](int type, uintptr_t x, int64_t x_stride, uintptr_t w, int64_t n,
+                                int G, int K, int N) {
+    return std::max(4 * leaf_route_words(n, G),
+                    leaf_linear_bytes(type, P<void>(x), x_stride, P<void>(w), n, G, K, N));
   });
   m.def("leaf_linear", [](int dev, uintptr_t s, int type, uintptr_t x, int64_t x_stride,
                           uintptr_t ids, bool wide, uintptr_t route, int64_t n, int G, uintptr_t w,
@@ -120,13 +122,15 @@ void bind_leaf(py::module_& m) {
     if (ids != 0)
       launch_leaf_route(S(s), P<void>(ids), wide, n, G, r.order, r.keys, r.off,
                         P<uint32_t>(work));
-    launch_leaf_linear_tile(S(s), type, false, P<void>(x), x_stride, r.order, r.off, n, G,
-                            P<void>(w), P<void>(bias), K, N, P<void>(y), P<void>(work));
+    launch_leaf_linear(S(s), type, P<void>(x), x_stride, r.order, r.off, n, G, P<void>(w),
+                       P<void>(bias), K, N, P<void>(y), P<void>(work));
   });
-  // dx, dw and db, each where its address is not 0; one scratch, used by one after the other
-  m.def("leaf_linear_grad_bytes", [](int type, int64_t n, int G, int K, int N) {
-    return std::max({leaf_linear_tile_bytes(n, G), leaf_linear_grad_bytes(type, n, G, K, N),
-                     leaf_embed_grad_bytes(type, n, N)});
+  // dx, dw and db, each where its address is not 0
+  m.def("leaf_linear_grad_bytes", [](int type, uintptr_t x, int64_t x_stride, uintptr_t dy,
+                                     int64_t dy_stride, uintptr_t w, int64_t n, int G, int K, int N,
+                                     bool dx, bool dw) {
+    return leaf_linear_grad_bytes(type, P<void>(x), x_stride, P<void>(dy), dy_stride, P<void>(w), n,
+                                  G, K, N, dx, dw);
   });
   m.def("leaf_linear_grad", [](int dev, uintptr_t s, int type, uintptr_t x, int64_t x_stride,
                                uintptr_t dy, int64_t dy_stride, uintptr_t route, int64_t n, int G,
@@ -134,17 +138,9 @@ void bind_leaf(py::module_& m) {
                                uintptr_t work) {
     const OnDevice on(dev);
     const Route r(route, n);
-    LlMade made{};
-    if (dw != 0)
-      made = launch_leaf_linear_grad(S(s), type, P<void>(x), x_stride, P<void>(dy), dy_stride,
-                                     r.order, r.keys, r.off, n, G, P<void>(w), K, N, P<void>(dx),
-                                     P<void>(dw), P<void>(db), P<void>(work));
-    if (dx != 0 && !made.dx)
-      launch_leaf_linear_tile(S(s), type, true, P<void>(dy), dy_stride, r.order, r.off, n, G,
-                              P<void>(w), nullptr, K, N, P<void>(dx), P<void>(work));
-    if (db != 0 && !made.db)
-      launch_leaf_embed_grad(S(s), type, P<void>(dy), dy_stride, r.order, r.keys, r.off, n, G, N,
-                             1.f, P<void>(db), P<void>(work));
+    launch_leaf_linear_grad(S(s), type, P<void>(x), x_stride, P<void>(dy), dy_stride, r.order,
+                            r.keys, r.off, n, G, P<void>(w), K, N, P<void>(dx), P<void>(dw),
+                            P<void>(db), P<void>(work));
   });
 }
 

@@ -13,6 +13,10 @@
 
 namespace mt {
 
+int64_t leaf_embed_grad_bytes(int, int64_t, int);
+void launch_leaf_embed_grad(hipStream_t, int, const void*, int64_t, const int32_t*, const uint32_t*,
+                            const int32_t*, int64_t, int64_t, int, float, void*, void*);
+
 constexpr int kLlThreads = 256;
 constexpr int kLlWaves = kLlThreads / kWave;
 constexpr int kLlSmallRows = 64;
@@ -233,7 +237,7 @@ struct LlTile {
   const int32_t* order;
   const int32_t* off;
   int64_t src_stride, w_stride;  // elements between src rows; between leaves' matrices
-  int G, depth, cols, w_row;     // w_row: elements of a row of W (K)
+  int G, depth, cols, w_row;     // w_row: elements of a row of W (K, or more of a packed one)
   int col_tiles, bj_shift;
   int64_t tiles;              // a bound
   const int2* plan;           // the tiles' leaves and positions, or null: found through off
@@ -419,7 +423,7 @@ __global__ __launch_bounds__(NW* kWave) void ll_tile_kernel(LlTile a) {
             constexpr int kRow = BI / E;
             const int k = id / kRow;
             const int c = ll_turn_chunk<T, BI>(k, id % kRow) - k * kRow;
-            p = wg + (int64_t)(k0 + k) * a.w_row + min(i0 + c * E, a.cols - E);
+            p = wg + (int64_t)(k0 + k) * a.w_row + min(i0 + c * E, a.w_row - E);
             if (k0 + k >= a.depth) p = kLlZeros;
           }
           ll_dma(p, si + q * NT + w * kWave);
@@ -698,7 +702,7 @@ __global__ __launch_bounds__(kBigThreads, 2) void ll_big_kernel(LlTile a) {
         wo[q] = ((uint32_t)min(i0 + r, a.cols - 1) * a.w_row + kc) * sizeof(T);
       else
         wo[q] = ((uint32_t)ll_big_turn_row(w, q) * a.w_row +
-                 min(i0 + ll_big_turn_col() * E, a.cols - E)) * sizeof(T);
+                 min(i0 + ll_big_turn_col() * E, a.w_row - E)) * sizeof(T);
     }
     // tail: the tile may reach past the depth
     auto load = [&](auto tail, char* s, int k0) {
@@ -801,6 +805,7 @@ struct LlGrad {
   const int32_t* off;
   int64_t x_stride, dy_stride;
   int G, N, K, k_tiles, n_tiles;
+  int n_row, k_row;  // elements of a row of dy and x: N and K, or more of packed ones
   int64_t run, units;
 };
 
@@ -993,8 +998,8 @@ __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
           const int id = q * kLlThreads + tid, k = id / kRow;
           const int c = ll_turn_chunk<T, B>(k, id % kRow) - k * kRow;
           const bool in = p0 + k < rows;
-          const T* const pj = dy + row[q] * a.dy_stride + min(j0 + c * E, a.N - E);
-          const T* const pi = x + row[q] * a.x_stride + min(i0 + c * E, a.K - E);
+          const T* const pj = dy + row[q] * a.dy_stride + min(j0 + c * E, a.n_row - E);
+          const T* const pi = x + row[q] * a.x_stride + min(i0 + c * E, a.k_row - E);
           // (dx sums over dy's columns: zeros behind the last)
           ll_dma(in && (!kDx || c * E < a.N) ? (const void*)pj : kLlZeros,
                  sj + q * kLlThreads + w * kWave);
@@ -1085,8 +1090,8 @@ __global__ __launch_bounds__(kBigThreads, 2) void ll_big_grad_kernel(LlGrad a) {
   if (rows > 0) {
     const LlBigLane lt;
     const i32x4 dy_rsrc = ll_rsrc(a.dy), x_rsrc = ll_rsrc(a.x);
-    const uint32_t jc = (uint32_t)min(j0 + ll_big_turn_col() * E, a.N - E) * sizeof(T);
-    const uint32_t ic = (uint32_t)min(i0 + ll_big_turn_col() * E, a.K - E) * sizeof(T);
+    const uint32_t jc = (uint32_t)min(j0 + ll_big_turn_col() * E, a.n_row - E) * sizeof(T);
+    const uint32_t ic = (uint32_t)min(i0 + ll_big_turn_col() * E, a.k_row - E) * sizeof(T);
     const uint32_t js = (uint32_t)a.dy_stride * sizeof(T), is = (uint32_t)a.x_stride * sizeof(T);
     int32_t row[kBigQ];  // of the next tile to fetch
     auto next_rows = [&](int p0) {
@@ -1326,6 +1331,19 @@ __global__ __launch_bounds__(kLlThreads) void ll_small_kernel(LlSmall a) {
   vec ? ll_store4<true>(to, acc, a.N - c) : ll_store4<false>(to, acc, a.N - c);
 }
 
+// Rows of `cols` elements as rows of whole 16-byte chunks, zeros behind the last column: what the
+// tiles that fetch straight into LDS can read. One chunk a thread; memory is the bound.
+template <typename T>
+__global__ __launch_bounds__(kLlThreads) void ll_pack_kernel(const T* __restrict__ src,
+                                                             int64_t stride, int64_t rows, int cols,
+                                                             int chunks, uint4* __restrict__ dst) {
+  const int64_t i = leaf_block() * kLlThreads + threadIdx.x;
+  if (i >= rows * chunks) return;
+  const int64_t r = i / chunks;
+  const int c = (int)(i - r * chunks) * Ll<T>::kEpc;
+  dst[i] = ll_chunk<T, false>(src + r * stride + c, cols - c);
+}
+
 // ---------------------------------------------------------------------------- launches
 template <typename T>
 static bool ll_aligned(std::initializer_list<const void*> ptrs,
@@ -1378,24 +1396,95 @@ static bool ll_short_rows(int elem, int depth, int cols) {
   return depth * elem <= 128 || (elem == 4 && depth * elem <= 256 && cols > 16);
 }
 
+// ---- operands whose rows do not start on 16 bytes, or whose width is no multiple of them
+static bool ll_rows_aligned(int type, const void* p, int64_t stride, int width) {
+  const int e = type == kLeafF32 ? 4 : 8;
+  return (uintptr_t)p % 16 == 0 && stride % e == 0 && width % e == 0;
+}
+static int ll_packed_width(int type, int width) {
+  const int e = type == kLeafF32 ? 4 : 8;
+  return (width + e - 1) / e * e;
+}
+static int64_t ll_packed_bytes(int type, int64_t rows, int width) {
+  return rows * ll_packed_width(type, width) * (type == kLeafF32 ? 4 : 2);
+}
+static const void* ll_pack(hipStream_t s, int type, const void* src, int64_t stride, int64_t rows,
+                           int width, void*& work) {
+  void* const to = work;
+  work = (char*)work + ll_packed_bytes(type, rows, width);
+  ll_dispatch_type(type, [&](auto t) {
+    using T = decltype(t);
+    const int chunks = (int)(ll_packed_width(type, width) / Ll<T>::kEpc);
+    const int64_t blocks = (rows * chunks + kLlThreads - 1) / kLlThreads;
+    hipLaunchKernelGGL(ll_pack_kernel<T>, leaf_grid(blocks), dim3(kLlThreads), 0, s, (const T*)src,
+                       stride, rows, width, chunks, (uint4*)to);
+    MT_HIP_CHECK(hipGetLastError());
+  });
+  return to;
+}
+
+// Which operands a pass copies into whole chunks first.
+struct LlPacks {
+  bool x = false, dy = false, w = false;
+  bool any() const { return x || dy || w; }
+  int64_t bytes(int type, int64_t n, int G, int K, int N) const {
+    return (x ? ll_packed_bytes(type, n, K) : 0) + (dy ? ll_packed_bytes(type, n, N) : 0) +
+           (w ? ll_packed_bytes(type, (int64_t)G * N, K) : 0);
+  }
+};
+// Such a copy is two passes over an operand and lets the products fetch straight into LDS. us
+// without / with, a forward pass, a row gradient, all gradients, bf16 and f16 unless noted:
+//   65536 rows, 64 leaves, 2047 -> 2049: 1466 / 1169, 1760 / 1118, 5032 / 2443
+//   20000 rows, 300 leaves, 511 -> 513: 104 / 166, 155 / 158, 414 / 349; 100 leaves: 77 / 77 (no
+//     copy), 101 / 73, 250 / 174; 20 leaves: 63 / 59, 88 / 58, 226 / 134; 30 leaves, f32 498 / 456
+//   10007 rows, 12 leaves, 1001 -> 601: 45 / 50, 66 / 56, 162 / 130
+//   300000 rows, 100 leaves, 301 -> 199: 265 / 294, 325 / 428, 1026 / 806; 129 -> 127: 104 / 160,
+//     176 / 152, 459 / 298
+//   1500 rows, 2 leaves, 511 -> 513: 23 / 23, 35 / 26, 70 / 54
+// So gradients copy from widths of about 64 on, the row gradient alone from about 256 on, a forward
+// pass where the largest tiles follow; W, which a leaf's rows have to pay for, from 64 rows a leaf
+// on with dW and 192 without, 384 in a forward pass, and not in f32, whose products are slower.
+constexpr int kLlPackRows = 1024;
+static LlPacks ll_forward_packs(int type, const void* x, int64_t x_stride, const void* w, int64_t n,
+                                int G, int K, int N) {
+  LlPacks p;
+  const bool xa = ll_rows_aligned(type, x, x_stride, K), wa = ll_rows_aligned(type, w, K, K);
+  if ((xa && wa) || type == kLeafF32 || K < 512 || n / G < 384) return p;
+  if ((n >> 8) * ((N + kBig - 1) / kBig) < 256) return p;
+  p.x = !xa, p.w = !wa;
+  return p;
+}
+static LlPacks ll_grad_packs(int type, const void* x, int64_t x_stride, const void* dy,
+                             int64_t dy_stride, const void* w, int64_t n, int G, int K, int N,
+                             bool dx, bool dw) {
+  LlPacks p;
+  const bool xa = ll_rows_aligned(type, x, x_stride, K), wa = ll_rows_aligned(type, w, K, K);
+  const bool ya = ll_rows_aligned(type, dy, dy_stride, N);
+  const int64_t width = (int64_t)K * N / (K + N);  // half of it where both are the same
+  if (width < (dw ? 32 : 128) || n / G < 32 || n < kLlPackRows) return p;
+  if (dw) p.x = !xa, p.dy = !ya;
+  if (dx && (wa || (type != kLeafF32 && n / G >= (dw ? 64 : 192)))) p.dy = !ya, p.w = !wa;
+  return p;
+}
+
 // scratch for the tile list
-int64_t leaf_linear_tile_bytes(int64_t n, int G) {
+static int64_t ll_plan_bytes(int64_t n, int G) {
   return n / G >= kLlBigRows ? 8 + 8 * ((n >> 8) + G + 1) : 0;
 }
 
-// forward (dx false: src = x, depth = K, cols = N) or dx (src = dy, depth = N, cols = K)
-void launch_leaf_linear_tile(hipStream_t s, int type, bool dx, const void* src, int64_t src_stride,
-                             const int32_t* order, const int32_t* off, int64_t n, int G,
-                             const void* w, const void* bias, int K, int N, void* out,
-                             void* work) {
-  if (n <= 0) return;
+// forward (dx false: src = x, depth = K, cols = N) or dx (src = dy, depth = N, cols = K). Rows of
+// src and W may be wider than that, with zeros behind (src_width, w_row).
+static void ll_launch_tile(hipStream_t s, int type, bool dx, const void* src, int64_t src_stride,
+                           int src_width, const int32_t* order, const int32_t* off, int64_t n,
+                           int G, const void* w, int w_row, const void* bias, int K, int N,
+                           void* out, void* work) {
   LlTile a{};
   a.src = src, a.w = w, a.bias = bias, a.out = out, a.order = order, a.off = off;
-  a.src_stride = src_stride, a.w_stride = (int64_t)N * K;
-  a.G = G, a.depth = dx ? N : K, a.cols = dx ? K : N, a.w_row = K;
+  a.src_stride = src_stride, a.w_stride = (int64_t)N * w_row;
+  a.G = G, a.depth = dx ? N : w_row, a.cols = dx ? K : N, a.w_row = w_row;
   ll_dispatch_type(type, [&](auto t) {
     using T = decltype(t);
-    const bool al = ll_aligned<T>({src, w}, {K, src_stride, dx ? N : K});
+    const bool al = ll_aligned<T>({src, w}, {w_row, src_stride, src_width});
     auto go = [&](auto bj, auto bi, auto wj, auto nw) {
       a.bj_shift = __builtin_ctz((unsigned)bj());
       a.col_tiles = (a.cols + bi() - 1) / bi();
@@ -1521,7 +1610,7 @@ static bool ll_fuse_dx(int b, int G, int K, int N) {
 }
 
 // scratch for the partial matrices (and sums), whichever tile is taken
-int64_t leaf_linear_grad_bytes(int type, int64_t n, int G, int K, int N) {
+static int64_t ll_part_bytes(int type, int64_t n, int G, int K, int N) {
   int64_t chunks = 0;
   for (bool direct : {false, true}) {
     const int b = ll_grad_tile(type, direct, n, G, K, N);
@@ -1531,22 +1620,26 @@ int64_t leaf_linear_grad_bytes(int type, int64_t n, int G, int K, int N) {
   return 2 * chunks * ((int64_t)N * K * 4 + 8 * N + 8);
 }
 
-// dW, and dx and db where they are asked for (not null); whether they were made here
-LlMade launch_leaf_linear_grad(hipStream_t s, int type, const void* x, int64_t x_stride,
-                               const void* dy, int64_t dy_stride, const int32_t* order,
-                               const uint32_t* keys, const int32_t* off, int64_t n, int G,
-                               const void* w, int K, int N, void* dx, void* dw, void* db,
-                               void* work) {
+// dW, and dx and db where they are asked for (not null); whether they were made here. Rows of x and
+// dy may be wider than K and N, with zeros behind (k_row, n_row).
+struct LlMade {
+  bool dx, db;
+};
+static LlMade ll_launch_grad(hipStream_t s, int type, const void* x, int64_t x_stride, int k_row,
+                             const void* dy, int64_t dy_stride, int n_row, const int32_t* order,
+                             const uint32_t* keys, const int32_t* off, int64_t n, int G,
+                             const void* w, int K, int N, void* dx, void* dw, void* db,
+                             void* work) {
   LlGrad a{};
   a.x = x, a.dy = dy, a.dw = dw, a.part = (float*)work;
   a.order = order, a.keys = keys, a.off = off;
   a.x_stride = x_stride, a.dy_stride = dy_stride;
-  a.G = G, a.N = N, a.K = K;
+  a.G = G, a.N = N, a.K = K, a.n_row = n_row, a.k_row = k_row;
   const int64_t elem = type == kLeafF32 ? 4 : 2;
   const bool al = (elem == 4 ? ll_aligned<float> : ll_aligned<f16_t>)(
-      {x, dy}, {K, N, x_stride, dy_stride});
+      {x, dy}, {k_row, n_row, x_stride, dy_stride});
   const bool direct =
-      al && (n * std::max(x_stride, dy_stride) + std::max(K, N)) * elem < (1ll << 32);
+      al && (n * std::max(x_stride, dy_stride) + std::max(k_row, n_row)) * elem < (1ll << 32);
   const int b = ll_grad_tile(type, direct, n, G, K, N);
   const int64_t tiles = ll_grad_tiles(b, K, N);
   a.n_tiles = (N + b - 1) / b, a.k_tiles = (K + b - 1) / b;
@@ -1590,6 +1683,68 @@ LlMade launch_leaf_linear_grad(hipStream_t s, int type, const void* x, int64_t x
     }
   });
   return LlMade{a.dx != nullptr, a.db != nullptr};
+}
+
+// ---- a forward and a backward pass
+int64_t leaf_linear_bytes(int type, const void* x, int64_t x_stride, const void* w, int64_t n,
+                          int G, int K, int N) {
+  const LlPacks p = ll_forward_packs(type, x, x_stride, w, n, G, K, N);
+  return p.bytes(type, n, G, K, N) + ll_plan_bytes(n, G);
+}
+
+void launch_leaf_linear(hipStream_t s, int type, const void* x, int64_t x_stride,
+                        const int32_t* order, const int32_t* off, int64_t n, int G, const void* w,
+                        const void* bias, int K, int N, void* y, void* work) {
+  if (n <= 0) return;
+  const LlPacks p = ll_forward_packs(type, x, x_stride, w, n, G, K, N);
+  const int k_row = p.any() ? ll_packed_width(type, K) : K;
+  if (p.x) x = ll_pack(s, type, x, x_stride, n, K, work), x_stride = k_row;
+  if (p.w) w = ll_pack(s, type, w, K, (int64_t)G * N, K, work);
+  ll_launch_tile(s, type, false, x, x_stride, k_row, order, off, n, G, w, k_row, bias, K, N, y,
+                 work);
+}
+
+int64_t leaf_linear_grad_bytes(int type, const void* x, int64_t x_stride, const void* dy,
+                               int64_t dy_stride, const void* w, int64_t n, int G, int K, int N,
+                               bool dx, bool dw) {
+  const LlPacks p = ll_grad_packs(type, x, x_stride, dy, dy_stride, w, n, G, K, N, dx, dw);
+  return p.bytes(type, n, G, K, N) + std::max({ll_plan_bytes(n, G),
+                                               ll_part_bytes(type, n, G, K, N),
+                                               leaf_embed_grad_bytes(type, n, N)});
+}
+
+// dx, dw and db, each where it is not null; their scratch is used by one after the other
+void launch_leaf_linear_grad(hipStream_t s, int type, const void* x, int64_t x_stride,
+                             const void* dy, int64_t dy_stride, const int32_t* order,
+                             const uint32_t* keys, const int32_t* off, int64_t n, int G,
+                             const void* w, int K, int N, void* dx, void* dw, void* db,
+                             void* work) {
+  const LlPacks p = ll_grad_packs(type, x, x_stride, dy, dy_stride, w, n, G, K, N, dx != nullptr,
+                                  dw != nullptr);
+  int k_row = K, n_row = N, w_row = K;
+  const void* const dy0 = dy;
+  const int64_t dy0_stride = dy_stride;
+  if (p.x) {
+    k_row = ll_packed_width(type, K);
+    x = ll_pack(s, type, x, x_stride, n, K, work), x_stride = k_row;
+  }
+  if (p.dy) {
+    n_row = ll_packed_width(type, N);
+    dy = ll_pack(s, type, dy, dy_stride, n, N, work), dy_stride = n_row;
+  }
+  if (p.w) {
+    w_row = ll_packed_width(type, K);
+    w = ll_pack(s, type, w, K, (int64_t)G * N, K, work);
+  }
+  LlMade made{};
+  if (dw != nullptr)
+    made = ll_launch_grad(s, type, x, x_stride, k_row, dy, dy_stride, n_row, order, keys, off, n,
+                          G, w, K, N, dx, dw, db, work);
+  if (dx != nullptr && !made.dx && n > 0)
+    ll_launch_tile(s, type, true, dy, dy_stride, n_row, order, off, n, G, w, w_row, nullptr, K, N,
+                   dx, work);
+  if (db != nullptr && !made.db)
+    launch_leaf_embed_grad(s, type, dy0, dy0_stride, order, keys, off, n, G, N, 1.f, db, work);
 }
 
 }  // namespace mt

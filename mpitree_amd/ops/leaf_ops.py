@@ -281,7 +281,8 @@ def _linear_forward(x, ids, route, w, b):
         hip.leaf_linear_small(dev, _stream(dev), kind, x.data_ptr(), x.stride(0), ids.data_ptr(),
                               wide, n, G, w.data_ptr(), bias, K, N, y.data_ptr())
         return y, route
-    work = _scratch(hip.leaf_linear_bytes(n, G), x)
+    work = _scratch(hip.leaf_linear_bytes(kind, x.data_ptr(), x.stride(0), w.data_ptr(), n, G, K,
+                                          N), x)
     sort = 0
     if route is None:
         sort = ids.data_ptr()
@@ -298,7 +299,9 @@ def _linear_grad(dy, x, route, w, need_x, need_w, need_b):
     dx = x.new_empty((n, K)) if need_x else None
     dw = x.new_empty((G, N, K)) if need_w else None
     db = x.new_empty((G, N)) if need_b else None
-    work = _scratch(hip.leaf_linear_grad_bytes(kind, n, G, K, N), x)
+    work = _scratch(hip.leaf_linear_grad_bytes(kind, x.data_ptr(), x.stride(0), dy.data_ptr(),
+                                               dy.stride(0), w.data_ptr(), n, G, K, N, need_x,
+                                               need_w), x)
     hip.leaf_linear_grad(dev, _stream(dev), kind, x.data_ptr(), x.stride(0), dy.data_ptr(),
                          dy.stride(0), route._buf.data_ptr(), n, G, w.data_ptr(), K, N,
                          *(0 if t is None else t.data_ptr() for t in (dx, dw, db)),

@@ -270,14 +270,19 @@ def test_linear_inf_in_an_incoming_gradient(device, dtype, K, N, G):
                                           (33_000, 23, 1048, 1032, 1.0),
                                           (20_000, 300, 136, 520, 0.0), (66_000, 5, 520, 776, 0.5)])
 def test_linear_large(dtype, n, G, K, N, skew):
-    # rows and columns that fill the largest tiles, with ends inside them; the sums in 64 bits and
-    # their absolute sums are computed on the device, leaf by leaf
+    # rows and columns that fill the largest tiles, with ends inside them
+    large_case(dtype, n, G, K, N, skew)
+
+
+def large_case(dtype, n, G, K, N, skew, shift=0):
+    # the sums in 64 bits and their absolute sums are computed on the device, leaf by leaf;
+    # shift: rows of x and dy start that many elements behind an aligned address
     g = gen(n + G)
     ids = draw_leaves(g, n, G, skew, 0.02).cuda()
-    x = torch.randn(n, K, generator=g).to(dtype).cuda()
+    x = torch.randn(n, K + shift, generator=g).to(dtype).cuda()[:, shift:]
     w = (torch.randn(G, N, K, generator=g) * K ** -0.5).to(dtype).cuda()
     b = torch.randn(G, N, generator=g).to(dtype).cuda()
-    dy = torch.randn(n, N, generator=g).to(dtype).cuda()
+    dy = torch.randn(n, N + shift, generator=g).to(dtype).cuda()[:, shift:]
     for p in (x, w, b):
         p.requires_grad_()
     y = leaf_linear(x, ids, w, b)
@@ -296,6 +301,17 @@ def test_linear_large(dtype, n, G, K, N, skew):
                 (dw[q], D.t().contiguous() @ X, Da.t().contiguous() @ Xa, len(r), "dw"),
                 (db[q], D.sum(0), Da.sum(0), len(r), "db")):
             check(got, want.cpu(), mass.cpu(), terms, (what, q))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,G,K,N,skew,shift", [
+    (12_000, 21, 1031, 1049, 0.0, 0), (12_000, 5, 777, 520, 0.5, 0),
+    (12_000, 300, 520, 777, 0.0, 0), (9000, 9, 600, 1000, 0.5, 3), (6000, 100, 201, 199, 1.0, 0),
+    (5000, 2, 1000, 601, 0.0, 8), (20_000, 7, 523, 1001, 0.0, 0), (1100, 5, 65, 67, 0.5, 0)])
+def test_linear_large_odd(dtype, n, G, K, N, skew, shift):
+    # widths and addresses that no 16-byte chunks fit
+    large_case(dtype, n, G, K, N, skew, shift)
 
 
 @pytest.mark.parametrize("device", DEVICES)
