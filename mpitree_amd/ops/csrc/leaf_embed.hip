@@ -13,6 +13,10 @@
 //
 // Sums are held in 32 bits for 16-bit types and in 64 bits for f32: a leaf may hold most of a
 // million rows, and a 64-bit add costs no more than a 32-bit one here, where memory is the bound.
+//
+// Both are bound by memory where rows are wide: 200k rows of 2048 f16 in 120000 leaves forward 261 us
+// (4.8 TB/s of a copy's 4.9), gradient 290 us (4.5 TB/s). 1M rows of 63 f32 in 64 leaves 47 and 67
+// us; 1M rows of 16 f32, random 64-byte reads, forward 22 us.
 #include "leaf.h"
 
 namespace mt {
@@ -93,9 +97,9 @@ __global__ __launch_bounds__(kLeThreads) void le_forward_kernel(
 }
 
 // the sums of the block's row groups, added in their order; group 0's lanes hold the result
-template <int W, typename A>
+template <int W, int THREADS, typename A>
 __device__ __forceinline__ void le_block_sum(A (&acc)[W], int tpr_shift, A* s_acc) {
-  const int tpr = 1 << tpr_shift, rpb = kLeThreads >> tpr_shift;
+  const int tpr = 1 << tpr_shift, rpb = THREADS >> tpr_shift;
   const int sub = threadIdx.x >> tpr_shift, lr = threadIdx.x & (tpr - 1);
   // pairwise: groups [half, 2 half) hand theirs to groups [0, half)
   for (int half = rpb >> 1; half > 0; half >>= 1) {
@@ -203,20 +207,31 @@ __global__ __launch_bounds__(kLeThreads) void le_backward_kernel(
     le_store<T, W, A>(dtable + (int64_t)cur * D + c0, scale, acc);
 }
 
-// One block (and column block) per chunk; it works if a leaf starts in the chunk and reaches out of
-// it, and adds that leaf's partial rows.
-template <typename T, int W>
-__global__ __launch_bounds__(kLeThreads) void le_join_kernel(
+// Adds the partial rows of the leaves that reach over a chunk's end. One block (and column block)
+// for each leaf (kByLeaf), or for each chunk in which such a leaf may start, whichever are fewer.
+// Few leaves have many partial rows each, so their blocks are larger (16384 rows of one leaf, 1024
+// columns of bf16: a gradient takes 35 us, 48 with 256 threads).
+template <bool kByLeaf>
+constexpr int kLeJoinThreads = kByLeaf ? 1024 : kLeThreads;
+template <typename T, int W, bool kByLeaf>
+__global__ __launch_bounds__(kLeJoinThreads<kByLeaf>) void le_join_kernel(
     const typename LeAcc<T>::type* __restrict__ part, const uint32_t* __restrict__ open,
-    const int32_t* __restrict__ off, int64_t chunks, int D, float scale, LeCols lc, int run_shift,
+    const int32_t* __restrict__ off, int64_t count, int D, float scale, LeCols lc, int run_shift,
     T* __restrict__ dtable) {
   using A = typename LeAcc<T>::type;
-  __shared__ A s_acc[W * kLeThreads / 2];
-  const int64_t blk = leaf_block(), chunk = blk / lc.col_blocks;
-  if (chunk >= chunks) return;
-  const uint32_t k = open[chunk] - 1;
-  if (k == 0xffffffffu) return;
-  const int tpr = 1 << lc.tpr_shift, rpb = kLeThreads >> lc.tpr_shift;
+  constexpr int kThreads = kLeJoinThreads<kByLeaf>;
+  __shared__ A s_acc[W * kThreads / 2];
+  const int64_t blk = leaf_block(), i = blk / lc.col_blocks;
+  if (i >= count) return;
+  int64_t k, chunk;
+  if constexpr (kByLeaf) {
+    k = i, chunk = off[k] >> run_shift;
+    if (off[k + 1] <= (chunk + 1) << run_shift) return;
+  } else {
+    chunk = i, k = (int64_t)open[chunk] - 1;
+    if (k < 0) return;
+  }
+  const int tpr = 1 << lc.tpr_shift, rpb = kThreads >> lc.tpr_shift;
   const int sub = threadIdx.x >> lc.tpr_shift, lr = threadIdx.x & (tpr - 1);
   const int c0 = ((int)(blk % lc.col_blocks) * tpr + lr) * W;
   const int64_t last = (off[k + 1] - 1) >> run_shift;
@@ -229,7 +244,7 @@ __global__ __launch_bounds__(kLeThreads) void le_join_kernel(
       for (int e = 0; e < W; ++e) acc[e] += in[e];
     }
   }
-  le_block_sum<W, A>(acc, lc.tpr_shift, s_acc);
+  le_block_sum<W, kThreads, A>(acc, lc.tpr_shift, s_acc);
   if (sub == 0 && c0 < D) le_store<T, W, A>(dtable + (int64_t)k * D + c0, scale, acc);
 }
 
@@ -347,10 +362,14 @@ static void le_backward(hipStream_t s, const T* dy, int64_t stride, const int32_
   };
   lc.tpr_shift == 6 ? go(le_backward_kernel<T, W, true>) : go(le_backward_kernel<T, W, false>);
   if (chunks > 1) {
-    hipLaunchKernelGGL((le_join_kernel<T, W>), leaf_grid((chunks - 1) * lc.col_blocks),
-                       dim3(kLeThreads), 0, s, part, open, off, chunks - 1, D, scale, lc, shift,
-                       dtable);
-    MT_HIP_CHECK(hipGetLastError());
+    const int64_t count = std::min(V, chunks - 1);
+    auto join = [&](auto kern, int threads) {
+      hipLaunchKernelGGL(kern, leaf_grid(count * lc.col_blocks), dim3(threads), 0, s, part, open,
+                         off, count, D, scale, lc, shift, dtable);
+      MT_HIP_CHECK(hipGetLastError());
+    };
+    V < chunks ? join(le_join_kernel<T, W, true>, kLeJoinThreads<true>)
+               : join(le_join_kernel<T, W, false>, kLeJoinThreads<false>);
   }
 }
 
