@@ -14,9 +14,9 @@
 // Sums are held in 32 bits for 16-bit types and in 64 bits for f32: a leaf may hold most of a
 // million rows, and a 64-bit add costs no more than a 32-bit one here, where memory is the bound.
 //
-// Both are bound by memory where rows are wide: 200k rows of 2048 f16 in 120000 leaves forward 261 us
-// (4.8 TB/s of a copy's 4.9), gradient 290 us (4.5 TB/s). 1M rows of 63 f32 in 64 leaves 47 and 67
-// us; 1M rows of 16 f32, random 64-byte reads, forward 22 us.
+// Both are bound by memory where rows are wide: 200k rows of 2048 f16 in 120000 leaves forward 261
+// us (4.8 TB/s of a copy's 4.9), gradient 290 us (4.5 TB/s). 1M rows of 63 f32 in 64 leaves 47 and
+// 67 us; 1M rows of 16 f32, random 64-byte reads, forward 22 us.
 #include "leaf.h"
 
 namespace mt {

@@ -639,9 +639,11 @@ def test_captured_and_replayed(n):
 
 
 @pytest.mark.gpu
-def test_captured_and_replayed_large():
-    # the largest tiles, in all three directions
-    n, G, K, N = 16_500, 16, 1024, 1032
+@pytest.mark.parametrize("n,G,K,N", [(16_500, 16, 1024, 1032), (16_500, 16, 1023, 1029),
+                                     (40_000, 3, 33, 600)])
+def test_captured_and_replayed_large(n, G, K, N):
+    # the largest tiles in all three directions, operands copied into whole chunks, few leaves with
+    # many partial sums
     bf = dict(device="cuda", dtype=torch.bfloat16)
 
     def make(seed):
