@@ -36,6 +36,7 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _MAX_ROWS = 2 ** 31 - 1
 _MAX_LEAVES = 2 ** 30
 _MAX_WIDTH = 2 ** 20
+_MAX_F32 = torch.finfo(torch.float32).max
 
 
 class LeafRoute:
@@ -180,6 +181,7 @@ def _sum_by_leaf_plain(dy, route: LeafRoute, scale: float) -> torch.Tensor:
     V = route.n_leaves
     out = torch.zeros((V + 1, dy.shape[1]), dtype=torch.float64)
     out.index_add_(0, route.keys.long(), dy[route.order.long()].double())
+    scale = torch.tensor(scale, dtype=torch.float32).double()  # as the forward pass has it
     return (out[:V] * scale).to(dy.dtype)
 
 
@@ -224,7 +226,8 @@ def leaf_embedding(leaves, table: torch.Tensor, *, scale: float = 1.0) -> torch.
     """``scale * table[leaves]``: one row of ``table`` [n_leaves, D] per leaf number.
 
     Returns ``leaves.shape + (D,)`` in the table's type. The gradient of ``table`` is dense: for
-    each leaf ``scale`` times the sum over its rows, zeros for a leaf that no row reached."""
+    each leaf ``scale`` times the sum over its rows, zeros for a leaf that no row reached.
+    ``scale`` is taken in float32, where it has to be finite."""
     table = _check_params("table", table, ndim=2)
     route = leaves if isinstance(leaves, LeafRoute) else None
     ids = _check_leaves(leaves if route is None else route.leaves)
@@ -234,8 +237,8 @@ def leaf_embedding(leaves, table: torch.Tensor, *, scale: float = 1.0) -> torch.
     _check_width("the table's width", table.shape[1])
     _check_device(ids, table)
     scale = float(scale)
-    if scale - scale != 0.0:
-        raise ValueError(f"scale must be finite, got {scale}")
+    if not -_MAX_F32 <= scale <= _MAX_F32:
+        raise ValueError(f"scale must be finite in float32, got {scale}")
     if table.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(table, ids, route, scale)
     return _embed_forward(ids, table, scale)
