@@ -27,6 +27,7 @@ torch). CPU tensors take a plain path of the same results.
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as fwad
 
 from . import native
 
@@ -116,6 +117,15 @@ def _check_device(first, *others):
             raise ValueError(f"operands on different devices: {first.device}, {t.device}")
 
 
+def _check_launch(*operands):
+    """The kernels take addresses, which say nothing of what torch keeps beside a tensor."""
+    if fwad._current_level >= 0:
+        for t in operands:
+            if t is not None and fwad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the leaf operators have no forward-mode derivative on CUDA "
+                                   "tensors: an operand has a tangent")
+
+
 def _stream(dev: int) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
@@ -167,6 +177,7 @@ def _embed_forward(ids: torch.Tensor, table: torch.Tensor, scale: float) -> torc
         has = (flat >= 0) & (flat < table.shape[0])
         y = table[torch.where(has, flat, 0)].float() * scale
         return torch.where(has[:, None], y, 0.0).to(table.dtype).reshape(*ids.shape, D)
+    _check_launch(table)
     y = table.new_empty((*ids.shape, D))
     if D > 1 and table.stride(1) != 1:
         table = table.contiguous()
@@ -191,6 +202,7 @@ def _embed_grad(dy, ids, route, n_leaves: int, scale: float) -> torch.Tensor:
     if not dy.is_cuda:
         route = route if route is not None else _route(ids, n_leaves)
         return _sum_by_leaf_plain(dy.reshape(-1, D), route, scale)
+    _check_launch(dy)
     hip, kind, dev = native.hip(), _TYPES[dy.dtype], dy.get_device()
     dy, ids = _rows(dy), ids.contiguous()
     n = dy.shape[0]
@@ -277,6 +289,7 @@ def _linear_forward(x, ids, route, w, b):
     if not x.is_cuda:
         route = route if route is not None else _route(ids, G)
         return _linear_plain(x, route, w, b), route
+    _check_launch(x, w, b)
     hip, kind, dev, ids = native.hip(), _TYPES[x.dtype], x.get_device(), ids.contiguous()
     wide, bias = ids.dtype == torch.int64, 0 if b is None else b.data_ptr()
     y = x.new_empty((n, N))
@@ -298,6 +311,7 @@ def _linear_forward(x, ids, route, w, b):
 
 def _linear_grad(dy, x, route, w, need_x, need_w, need_b):
     n, (G, N, K) = x.shape[0], w.shape
+    _check_launch(dy)
     hip, kind, dev, dy = native.hip(), _TYPES[x.dtype], x.get_device(), _rows(dy)
     dx = x.new_empty((n, K)) if need_x else None
     dw = x.new_empty((G, N, K)) if need_w else None

@@ -2,8 +2,10 @@
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
-from mpitree_amd import leaf_embedding
+from mpitree_amd import leaf_embedding, leaf_linear, leaf_route
+from mpitree_amd.ops import leaf_ops
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -43,3 +45,73 @@ def test_scale_is_the_same_number_in_both_directions(device):
     want = (d.double() * torch.tensor(0.1, dtype=torch.float32).double()).float()
     assert torch.equal(y.detach().cpu(), want)
     assert torch.equal(dt.cpu(), want)
+
+
+# --------------------------------------------------------------------- forward-mode tangents
+def operands(device, n=9, G=3, K=4, N=2):
+    g = torch.Generator().manual_seed(n)
+    return (torch.randint(-1, G, (n,), generator=g).to(device),
+            *(torch.randn(*s, generator=g).to(device) for s in ((n, K), (G, N, K), (G, N))))
+
+
+def forward_calls(device):
+    """(call, its operands that may have a tangent) of each operator."""
+    for n in (9, 90):  # the form for few rows and the tiles
+        ids, x, w, b = operands(device, n)
+        for leaves in (ids, leaf_route(ids, 3)):
+            yield (lambda t, leaves=leaves: leaf_embedding(leaves, t, scale=0.5)), [b]
+            yield (lambda x, w, b, leaves=leaves: leaf_linear(x, leaves, w, b)), [x, w, b]
+
+
+@pytest.mark.gpu
+def test_tangents_are_refused_on_the_gpu():
+    # the kernels know nothing of them: the derivative would read as zero
+    for call, args in forward_calls("cuda"):
+        for k in range(len(args)):
+            with fwad.dual_level():
+                dual = list(args)
+                dual[k] = fwad.make_dual(args[k], torch.ones_like(args[k]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*dual)
+                with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+                    call(*dual)
+                call(*args)  # operands without one pass
+        call(*args)
+
+
+@pytest.mark.gpu
+def test_tangents_of_an_incoming_gradient_are_refused_on_the_gpu():
+    for call, args in forward_calls("cuda"):
+        args = [a.clone().requires_grad_() for a in args]
+        y = call(*args)
+        with fwad.dual_level():
+            dy = fwad.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, args, dy)
+
+
+def test_tangents_are_refused_before_a_launch():
+    # what the calls above check first, here without a GPU
+    t = torch.randn(3, 4)
+    leaf_ops._check_launch(t, None)
+    with fwad.dual_level():
+        leaf_ops._check_launch(t, None)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            leaf_ops._check_launch(torch.arange(3), fwad.make_dual(t, t), None)
+    leaf_ops._check_launch(t, None)
+
+
+def test_tangents_on_the_cpu():
+    # plain torch operations: the operators are linear in each operand
+    for call, args in forward_calls("cpu"):
+        for k in range(len(args)):
+            with fwad.dual_level():
+                dual = list(args)
+                tangent = torch.ones_like(args[k])
+                dual[k] = fwad.make_dual(args[k], tangent)
+                got = fwad.unpack_dual(call(*dual)).tangent
+            zero = list(args)
+            zero[k] = torch.zeros_like(tangent)
+            one = list(args)
+            one[k] = tangent
+            assert torch.allclose(got, call(*one) - call(*zero), atol=1e-5)
