@@ -4,6 +4,7 @@
 #include <pybind11/pybind11.h>
 
 #include <algorithm>
+#include <initializer_list>
 
 #include "leaf.h"
 
@@ -54,6 +55,14 @@ class OnDevice {
   int dev_, was_ = 0;
 };
 
+// Operands that a launch of `n` rows reads or writes. A tensor without memory of its own (a wrapper
+// of another one) has the address 0.
+void need(int64_t n, std::initializer_list<uintptr_t> operands) {
+  if (n > 0)
+    for (const uintptr_t p : operands)
+      if (p == 0) throw std::runtime_error("leaf operator: an operand has no memory of its own");
+}
+
 // A route in one int32 buffer: order [n], keys [n], offsets [G + 2].
 struct Route {
   int32_t* order;
@@ -70,12 +79,15 @@ void bind_leaf(py::module_& m) {
   m.def("leaf_route_words", &leaf_route_words);  // ... of the scratch of its sort
   m.def("leaf_route", [](int dev, uintptr_t s, uintptr_t ids, bool wide, int64_t n, int G,
                          uintptr_t buf, uintptr_t work) {
+    need(1, {buf});
+    need(n, {ids});
     const OnDevice on(dev);
     const Route r(buf, n);
     launch_leaf_route(S(s), P<void>(ids), wide, n, G, r.order, r.keys, r.off, P<uint32_t>(work));
   });
   m.def("leaf_embed", [](int dev, uintptr_t s, int type, uintptr_t ids, bool wide, uintptr_t table,
                          int64_t stride, int64_t n, int64_t V, int D, float scale, uintptr_t y) {
+    need(n, {ids, table, y});
     const OnDevice on(dev);
     launch_leaf_embed(S(s), type, P<void>(ids), wide, P<void>(table), stride, n, V, D, scale,
                       P<void>(y));
@@ -88,6 +100,8 @@ void bind_leaf(py::module_& m) {
   m.def("leaf_embed_grad", [](int dev, uintptr_t s, int type, uintptr_t dy, int64_t dy_stride,
                               uintptr_t ids, bool wide, uintptr_t route, int64_t n, int G, int D,
                               float scale, uintptr_t dtable, uintptr_t work) {
+    need(1, {dtable, work});
+    need(n, {dy, route | ids});
     const OnDevice on(dev);
     if (route == 0) {
       route = work + pad16(4 * leaf_route_words(n, G));
@@ -100,10 +114,11 @@ void bind_leaf(py::module_& m) {
     launch_leaf_embed_grad(S(s), type, P<void>(dy), dy_stride, r.order, r.keys, r.off, n, G, D,
                            scale, P<void>(dtable), P<void>(work));
   });
-  m.def("leaf_linear_small_rows", &leaf_linear_small_rows);
+  m.attr("LEAF_LINEAR_SMALL_ROWS") = leaf_linear_small_rows();
   m.def("leaf_linear_small", [](int dev, uintptr_t s, int type, uintptr_t x, int64_t x_stride,
                                 uintptr_t ids, bool wide, int n, int G, uintptr_t w,
                                 uintptr_t bias, int K, int N, uintptr_t y) {
+    need(n, {x, ids, w, y});
     const OnDevice on(dev);
     launch_leaf_linear_small(S(s), type, P<void>(x), x_stride, P<void>(ids), wide, n, G,
                              P<void>(w), P<void>(bias), K, N, P<void>(y));
@@ -117,6 +132,7 @@ void bind_leaf(py::module_& m) {
   m.def("leaf_linear", [](int dev, uintptr_t s, int type, uintptr_t x, int64_t x_stride,
                           uintptr_t ids, bool wide, uintptr_t route, int64_t n, int G, uintptr_t w,
                           uintptr_t bias, int K, int N, uintptr_t y, uintptr_t work) {
+    need(n, {x, route, w, y});
     const OnDevice on(dev);
     const Route r(route, n);
     if (ids != 0)
@@ -136,6 +152,8 @@ void bind_leaf(py::module_& m) {
                                uintptr_t dy, int64_t dy_stride, uintptr_t route, int64_t n, int G,
                                uintptr_t w, int K, int N, uintptr_t dx, uintptr_t dw, uintptr_t db,
                                uintptr_t work) {
+    need(1, {route});
+    need(n, {x, dy, w});
     const OnDevice on(dev);
     const Route r(route, n);
     launch_leaf_linear_grad(S(s), type, P<void>(x), x_stride, P<void>(dy), dy_stride, r.order,

@@ -39,6 +39,7 @@ def leaf_numbers(est, X: torch.Tensor) -> torch.Tensor:
 
 
 def _walk(est, X: torch.Tensor, number: bool) -> torch.Tensor:
+    native.check_memory(X)
     hip = native.hip()
     if X.dtype not in (torch.float32, torch.float64):
         X = X.double()

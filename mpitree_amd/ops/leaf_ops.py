@@ -21,7 +21,9 @@ and rounded once. Gradients do not depend on the launch: the same inputs give th
 CUDA tensors run the gfx950 kernels (``ops/csrc/leaf_*.hip``) on the tensors' device and its current
 stream, without host synchronisation, so calls can be captured into a graph (one with a backward
 pass: while no eager autograd graph of the same parameters is alive, as for every operator of
-torch). CPU tensors take a plain path of the same results.
+torch). They give first derivatives in reverse mode; operands with a forward-mode tangent, tensors
+without memory of their own (fake, functional or wrapped ones) and tracing (``make_fx``,
+``torch.jit.trace``) are refused. CPU tensors take a plain path of the same results.
 """
 
 from __future__ import annotations
@@ -112,13 +114,15 @@ def _check_width(what: str, width: int):
 
 
 def _check_device(first, *others):
+    dev = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"operands on different devices: {first.device}, {t.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"operands on different devices: {dev}, {t.device}")
 
 
 def _check_launch(*operands):
     """The kernels take addresses, which say nothing of what torch keeps beside a tensor."""
+    native.check_memory(*operands)
     if fwad._current_level >= 0:
         for t in operands:
             if t is not None and fwad.unpack_dual(t).tangent is not None:
@@ -142,7 +146,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., C] as [rows, C] with unit column stride (any row stride)."""
     if t.dim() != 2:  # (a view would be one more node for autograd to walk)
         t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] == 1 and t.stride(0) >= 0 else t.contiguous()
+    stride, step = t.stride()
+    return t if step == 1 or t.shape[1] == 1 and stride >= 0 else t.contiguous()
 
 
 # -------------------------------------------------------------------------------- route
@@ -153,7 +158,7 @@ def leaf_route(leaves: torch.Tensor, n_leaves: int) -> LeafRoute:
 
 
 def _route(leaves: torch.Tensor, n_leaves: int) -> LeafRoute:
-    ids = leaves.reshape(-1)
+    ids = leaves if leaves.dim() == 1 else leaves.reshape(-1)
     n = ids.numel()
     if not ids.is_cuda:
         key = torch.where((ids >= 0) & (ids < n_leaves), ids, n_leaves).to(torch.int64)
@@ -161,6 +166,7 @@ def _route(leaves: torch.Tensor, n_leaves: int) -> LeafRoute:
         bounds = torch.arange(n_leaves + 1, dtype=torch.int64)
         offsets = torch.cat([torch.searchsorted(key, bounds), torch.tensor([n])])
         return LeafRoute(leaves, n_leaves, torch.cat([order, key, offsets]).int())
+    _check_launch(ids)
     hip, dev, ids = native.hip(), ids.get_device(), ids.contiguous()
     buf = ids.new_empty(hip.leaf_route_len(n, n_leaves), dtype=torch.int32)
     work = _scratch(4 * hip.leaf_route_words(n, n_leaves), ids)
@@ -171,20 +177,21 @@ def _route(leaves: torch.Tensor, n_leaves: int) -> LeafRoute:
 
 # ---------------------------------------------------------------------------- embedding
 def _embed_forward(ids: torch.Tensor, table: torch.Tensor, scale: float) -> torch.Tensor:
-    D = table.shape[1]
+    V, D = table.shape
     if not ids.is_cuda:
         flat = ids.reshape(-1)
-        has = (flat >= 0) & (flat < table.shape[0])
+        has = (flat >= 0) & (flat < V)
         y = table[torch.where(has, flat, 0)].float() * scale
         return torch.where(has[:, None], y, 0.0).to(table.dtype).reshape(*ids.shape, D)
-    _check_launch(table)
+    _check_launch(table, ids)
     y = table.new_empty((*ids.shape, D))
-    if D > 1 and table.stride(1) != 1:
-        table = table.contiguous()
+    stride, step = table.stride()
+    if D > 1 and step != 1:
+        table, stride = table.contiguous(), D
     ids, dev = ids.contiguous(), table.get_device()
     native.hip().leaf_embed(dev, _stream(dev), _TYPES[table.dtype], ids.data_ptr(),
-                            ids.dtype == torch.int64, table.data_ptr(), table.stride(0),
-                            ids.numel(), table.shape[0], D, scale, y.data_ptr())
+                            ids.dtype == torch.int64, table.data_ptr(), stride, ids.numel(), V, D,
+                            scale, y.data_ptr())
     return y
 
 
@@ -202,7 +209,7 @@ def _embed_grad(dy, ids, route, n_leaves: int, scale: float) -> torch.Tensor:
     if not dy.is_cuda:
         route = route if route is not None else _route(ids, n_leaves)
         return _sum_by_leaf_plain(dy.reshape(-1, D), route, scale)
-    _check_launch(dy)
+    _check_launch(dy, ids)
     hip, kind, dev = native.hip(), _TYPES[dy.dtype], dy.get_device()
     dy, ids = _rows(dy), ids.contiguous()
     n = dy.shape[0]
@@ -242,11 +249,12 @@ def leaf_embedding(leaves, table: torch.Tensor, *, scale: float = 1.0) -> torch.
     ``scale`` is taken in float32, where it has to be finite."""
     table = _check_params("table", table, ndim=2)
     route = leaves if isinstance(leaves, LeafRoute) else None
-    ids = _check_leaves(leaves if route is None else route.leaves)
-    n_leaves = _check_n_leaves(table.shape[0])
+    ids = _check_leaves(leaves) if route is None else route.leaves
+    n_leaves, D = table.shape
+    _check_n_leaves(n_leaves)
     if route is not None and route.n_leaves != n_leaves:
         raise ValueError(f"table has {n_leaves} rows, the route {route.n_leaves} leaves")
-    _check_width("the table's width", table.shape[1])
+    _check_width("the table's width", D)
     _check_device(ids, table)
     scale = float(scale)
     if not -_MAX_F32 <= scale <= _MAX_F32:
@@ -289,11 +297,11 @@ def _linear_forward(x, ids, route, w, b):
     if not x.is_cuda:
         route = route if route is not None else _route(ids, G)
         return _linear_plain(x, route, w, b), route
-    _check_launch(x, w, b)
+    _check_launch(x, w, b, ids)
     hip, kind, dev, ids = native.hip(), _TYPES[x.dtype], x.get_device(), ids.contiguous()
     wide, bias = ids.dtype == torch.int64, 0 if b is None else b.data_ptr()
     y = x.new_empty((n, N))
-    if n <= hip.leaf_linear_small_rows():
+    if n <= hip.LEAF_LINEAR_SMALL_ROWS:
         hip.leaf_linear_small(dev, _stream(dev), kind, x.data_ptr(), x.stride(0), ids.data_ptr(),
                               wide, n, G, w.data_ptr(), bias, K, N, y.data_ptr())
         return y, route
@@ -360,7 +368,7 @@ def leaf_linear(inputs: torch.Tensor, leaves, weight: torch.Tensor, bias=None) -
     weight = _check_params("weight", weight, ndim=3)
     inputs = _check_params("inputs", inputs, like=weight)
     route = leaves if isinstance(leaves, LeafRoute) else None
-    ids = _check_leaves(leaves if route is None else route.leaves)
+    ids = _check_leaves(leaves) if route is None else route.leaves
     G, N, K = weight.shape
     _check_n_leaves(G)
     _check_width("weight's rows", N)
@@ -378,10 +386,11 @@ def leaf_linear(inputs: torch.Tensor, leaves, weight: torch.Tensor, bias=None) -
         bias = bias.contiguous()
     _check_device(inputs, ids, weight, bias)
     x, weight = _rows(inputs), weight.contiguous()
-    flat = ids if ids.dim() == 1 else ids.reshape(-1)
+    one = ids.dim() == 1
+    flat = ids if one else ids.reshape(-1)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                     or bias is not None and bias.requires_grad):
         y = _Linear.apply(x, weight, bias, flat, route)
     else:
         y = _linear_forward(x, flat, route, weight, bias)[0]
-    return y if ids.dim() == 1 else y.reshape(*ids.shape, N)
+    return y if one else y.reshape(*ids.shape, N)

@@ -3,9 +3,12 @@
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils.flop_counter import FlopCounterMode
 
-from mpitree_amd import leaf_embedding, leaf_linear, leaf_route
-from mpitree_amd.ops import leaf_ops
+from mpitree_amd import DecisionTreeClassifier, leaf_embedding, leaf_linear, leaf_route
+from mpitree_amd.ops import leaf_ops, native
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -115,3 +118,125 @@ def test_tangents_on_the_cpu():
             one = list(args)
             one[k] = tangent
             assert torch.allclose(got, call(*one) - call(*zero), atol=1e-5)
+
+
+# ------------------------------------------- tensors without memory of their own, and tracing
+def all_calls(device):
+    ids = operands(device)[0]
+    yield (lambda ids: leaf_route(ids, 3)), [ids]
+    for call, args in forward_calls(device):
+        yield call, args
+
+
+class Wrapped(torch.Tensor):
+    """A tensor whose operations are answered by its class."""
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        return NotImplemented
+
+
+def test_fake_tensors_of_the_gpu_are_refused():
+    # their address is 0
+    with FakeTensorMode():
+        ids = torch.zeros(100, dtype=torch.int64, device="cuda")
+        x, w, b = (torch.zeros(*s, device="cuda") for s in ((100, 4), (3, 2, 4), (3, 2)))
+        for call in (lambda: leaf_route(ids, 3), lambda: leaf_embedding(ids, b),
+                     lambda: leaf_embedding(ids, b.requires_grad_()),
+                     lambda: leaf_linear(x, ids, w, b), lambda: leaf_linear(x[:9], ids[:9], w)):
+            with pytest.raises(TypeError, match="plain tensors"):
+                call()
+    for call in (lambda: leaf_embedding(ids, b), lambda: leaf_linear(x, ids, w)):
+        with pytest.raises(TypeError, match="plain tensors"):
+            call()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_what_a_launch_would_do_wrongly_is_refused(device):
+    t = torch.zeros(3, 4, device=device)
+    native.check_memory(t, None, torch.nn.Parameter(t))
+    with pytest.raises(TypeError, match="plain tensors"):
+        native.check_memory(t, t.as_subclass(Wrapped))
+    with FakeTensorMode(), pytest.raises(RuntimeError, match="traced"):
+        native.check_memory(t)
+    for mode in ("real", "fake", "symbolic"):
+        with pytest.raises((RuntimeError, TypeError), match="traced|plain tensors"):
+            make_fx(lambda x: (native.check_memory(x), x + 1)[1], tracing_mode=mode)(t)
+    with pytest.raises(RuntimeError, match="jit.trace"):
+        torch.jit.trace(lambda x: (native.check_memory(x), x + 1)[1], (t,))
+    with FlopCounterMode(display=False):  # it watches and changes nothing
+        native.check_memory(t)
+    native.check_memory(t.as_subclass(type("Named", (torch.Tensor,), {})))
+
+
+def test_null_addresses_are_refused():
+    hip = native.hip()
+    for call in (lambda: hip.leaf_route(0, 0, 0, True, 5, 3, 64, 0),
+                 lambda: hip.leaf_route(0, 0, 64, True, 5, 3, 0, 0),
+                 lambda: hip.leaf_embed(0, 0, 0, 64, True, 0, 4, 5, 3, 4, 1.0, 64),
+                 lambda: hip.leaf_embed(0, 0, 0, 64, True, 64, 4, 5, 3, 4, 1.0, 0),
+                 lambda: hip.leaf_embed_grad(0, 0, 0, 0, 4, 64, True, 0, 5, 3, 4, 1.0, 64, 64),
+                 lambda: hip.leaf_embed_grad(0, 0, 0, 64, 4, 0, True, 0, 5, 3, 4, 1.0, 64, 64),
+                 lambda: hip.leaf_linear_small(0, 0, 0, 0, 4, 64, True, 5, 3, 64, 0, 4, 2, 64),
+                 lambda: hip.leaf_linear(0, 0, 0, 64, 4, 0, True, 64, 99, 3, 64, 0, 4, 2, 0, 64),
+                 lambda: hip.leaf_linear_grad(0, 0, 0, 64, 4, 0, 2, 64, 99, 3, 64, 4, 2, 64, 64, 0,
+                                              64)):
+        with pytest.raises(RuntimeError, match="no memory of its own"):
+            call()
+
+
+@pytest.mark.gpu
+def test_traced_and_wrapped_calls_are_refused_on_the_gpu():
+    for call, args in all_calls("cuda"):
+        want = call(*args)
+        for mode in ("real", "fake", "symbolic"):
+            with pytest.raises((RuntimeError, TypeError), match="traced|plain tensors"):
+                make_fx(call, tracing_mode=mode)(*args)
+        with pytest.raises(RuntimeError, match="jit.trace"):
+            torch.jit.trace(call, tuple(args))
+        # (wrappers that torch itself makes: an address of 0, or no address)
+        with pytest.raises(RuntimeError, match="memory|storage"):
+            torch.func.functionalize(call)(*args)
+        with pytest.raises(RuntimeError, match="memory|storage"):
+            torch.func.vmap(call)(*(a[None] for a in args))
+        with FlopCounterMode(display=False):
+            got = call(*args)
+        if isinstance(want, torch.Tensor):
+            assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_traced_and_faked_gradients_are_refused_on_the_gpu():
+    for call, args in forward_calls("cuda"):
+        args = [a.clone().requires_grad_() for a in args]
+        y = call(*args)
+        dy = torch.ones_like(y)
+        want = torch.autograd.grad(y, args, dy, retain_graph=True)
+        with pytest.raises((RuntimeError, TypeError), match="traced|plain tensors"):
+            make_fx(lambda d: torch.autograd.grad(y, args, d, retain_graph=True))(dy)
+        for a, b in zip(want, torch.autograd.grad(y, args, dy)):
+            assert torch.equal(a, b)
+
+
+def test_an_estimator_refuses_fake_rows():
+    X = torch.randn(80, 3, generator=torch.Generator().manual_seed(0))
+    est = DecisionTreeClassifier(max_depth=3, device="cpu").fit(X.numpy(), (X[:, 0] > 0).long())
+    with FakeTensorMode(), pytest.raises(TypeError, match="plain tensors"):
+        est.leaf_route(torch.zeros(4, 3, device="cuda"))
+    assert est.leaf_route(X).leaves.shape == (80,)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_inside_a_compiled_function(device):
+    # torch.compile breaks its graph at the launches and calls them as they are
+    for call, args in forward_calls(device):
+        args = [a.clone().requires_grad_() for a in args]
+
+        def step(*args):
+            return call(*(a * 2 for a in args)) + 1
+
+        y, want = torch.compile(step, backend="eager")(*args), step(*args)
+        assert torch.equal(y, want)
+        for a, b in zip(*(torch.autograd.grad(out.sum(), args) for out in (y, want))):
+            assert torch.equal(a, b)
+        torch._dynamo.reset()
