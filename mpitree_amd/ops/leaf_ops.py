@@ -105,7 +105,7 @@ def _check_params(what: str, t, like=None, ndim=None) -> torch.Tensor:
         raise ValueError(f"{what} must have {ndim} dimensions, got shape {tuple(t.shape)}")
     if like is not None and t.dtype != like.dtype:
         raise TypeError(f"{what} is {t.dtype}, expected {like.dtype} as the other operands")
-    return t
+    return t.resolve_neg() if t.is_neg() else t
 
 
 def _check_width(what: str, width: int):
@@ -143,7 +143,10 @@ def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """[..., C] as [rows, C] with unit column stride (any row stride)."""
+    """[..., C] as [rows, C] with unit column stride (any row stride), and no sign that only the
+    tensor knows of (the imaginary part of a conjugate)."""
+    if t.is_neg():
+        t = t.resolve_neg()
     if t.dim() != 2:  # (a view would be one more node for autograd to walk)
         t = t.reshape(-1, t.shape[-1])
     stride, step = t.stride()

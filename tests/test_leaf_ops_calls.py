@@ -240,3 +240,43 @@ def test_inside_a_compiled_function(device):
         for a, b in zip(*(torch.autograd.grad(out.sum(), args) for out in (y, want))):
             assert torch.equal(a, b)
         torch._dynamo.reset()
+
+
+# --------------------------------------------------------- views that torch negates when read
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [9, 90])
+def test_lazily_negated_operands(device, n):
+    # the imaginary part of a conjugate holds the other sign in memory
+    g = torch.Generator().manual_seed(3)
+    ids = torch.randint(-1, 3, (n,), generator=g).to(device)
+
+    def pair(*shape):
+        z = torch.randn(*shape, dtype=torch.complex64, generator=g).to(device)
+        view = z.conj().imag
+        assert view.is_neg()
+        return view, view.clone()
+
+    for K, N in ((1, 1), (1, 6), (6, 1), (6, 6)):
+        (x, x0), (w, w0), (b, b0) = pair(n, K), pair(3, N, K), pair(3, N)
+        dy, dy0 = pair(n, N)
+        w1, b1 = torch._neg_view(-w0), torch._neg_view(-b0)  # (contiguous ones)
+        assert torch.equal(w1, w0) and w1.is_contiguous()
+        want = leaf_linear(x0, ids, w0, b0)
+        assert torch.equal(leaf_linear(x, ids, w, b), want)
+        assert torch.equal(leaf_linear(torch._neg_view(-x0), ids, w1, b1), want)
+        assert torch.equal(leaf_embedding(ids, b), leaf_embedding(ids, b0))
+        assert torch.equal(leaf_embedding(ids, b1), leaf_embedding(ids, b0))
+        args = [a.requires_grad_() for a in (x0, w0, b0)]
+        for op, wrt in ((lambda: leaf_linear(args[0], ids, *args[1:]), args),
+                        (lambda: leaf_embedding(ids, args[2]), args[2:])):
+            for got, ref in zip(torch.autograd.grad(op(), wrt, dy),
+                                torch.autograd.grad(op(), wrt, dy0)):
+                assert torch.equal(got, ref)
+
+
+def test_rows_and_parameters_of_negated_views_are_materialised():
+    # what reaches a launch, here without a GPU
+    v = torch.randn(5, 1, dtype=torch.complex64).conj().imag
+    assert v.is_neg() and not leaf_ops._rows(v).is_neg()
+    assert torch.equal(leaf_ops._rows(v), v)
+    assert not leaf_ops._check_params("table", v, ndim=2).is_neg()
