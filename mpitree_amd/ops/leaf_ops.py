@@ -90,7 +90,14 @@ def _check_leaves(leaves) -> torch.Tensor:
 
 
 def _check_n_leaves(n_leaves) -> int:
-    n_leaves = int(n_leaves)
+    if type(n_leaves) is not int:
+        try:
+            whole = int(n_leaves) == n_leaves
+        except (TypeError, ValueError, OverflowError):
+            whole = False
+        if not whole:
+            raise TypeError(f"n_leaves must be a whole number, got {n_leaves!r}")
+        n_leaves = int(n_leaves)
     if not 1 <= n_leaves <= _MAX_LEAVES:
         raise ValueError(f"n_leaves must be in [1, {_MAX_LEAVES}], got {n_leaves}")
     return n_leaves

@@ -1,5 +1,6 @@
 """Calls of the operators over a tree's leaves that have to be right or refused."""
 
+import numpy as np
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
@@ -280,3 +281,16 @@ def test_rows_and_parameters_of_negated_views_are_materialised():
     assert v.is_neg() and not leaf_ops._rows(v).is_neg()
     assert torch.equal(leaf_ops._rows(v), v)
     assert not leaf_ops._check_params("table", v, ndim=2).is_neg()
+
+
+# ------------------------------------------------------------------------- whole numbers
+@pytest.mark.parametrize("n_leaves", [2.5, 0.9, "3", None, float("nan"), float("inf")])
+def test_the_number_of_leaves_is_whole(n_leaves):
+    with pytest.raises((TypeError, ValueError), match="n_leaves"):
+        leaf_route(torch.zeros(4, dtype=torch.int64), n_leaves)
+
+
+@pytest.mark.parametrize("n_leaves", [3, 3.0, np.int32(3), torch.tensor(3)])
+def test_whole_numbers_of_any_type(n_leaves):
+    r = leaf_route(torch.tensor([2, 0]), n_leaves)
+    assert r.n_leaves == 3 and type(r.n_leaves) is int
