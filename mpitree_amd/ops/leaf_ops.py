@@ -149,25 +149,30 @@ def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
     return like.new_empty(nbytes, dtype=torch.uint8)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """[..., C] as [rows, C] with unit column stride (any row stride), and no sign that only the
-    tensor knows of (the imaginary part of a conjugate)."""
-    if t.is_neg():
-        t = t.resolve_neg()
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """[..., C] as [rows, C] with unit column stride (any row stride)."""
     if t.dim() != 2:  # (a view would be one more node for autograd to walk)
         t = t.reshape(-1, t.shape[-1])
     stride, step = t.stride()
     return t if step == 1 or t.shape[1] == 1 and stride >= 0 else t.contiguous()
 
 
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """The same of an incoming gradient, whose sign may be known to the tensor only (the imaginary
+    part of a conjugate)."""
+    return _flat(t.resolve_neg() if t.is_neg() else t)
+
+
 # -------------------------------------------------------------------------------- route
 def leaf_route(leaves: torch.Tensor, n_leaves: int) -> LeafRoute:
     """Sort the rows by leaf (stable). ``leaves``: int32 or int64 of any shape."""
-    return _route(_check_leaves(leaves).clone(memory_format=torch.contiguous_format),
-                  _check_n_leaves(n_leaves))
+    leaves = _check_leaves(leaves).clone(memory_format=torch.contiguous_format)
+    n_leaves = _check_n_leaves(n_leaves)
+    return LeafRoute(leaves, n_leaves, _sort(leaves, n_leaves))
 
 
-def _route(leaves: torch.Tensor, n_leaves: int) -> LeafRoute:
+def _sort(leaves: torch.Tensor, n_leaves: int) -> torch.Tensor:
+    """A route's buffer: order [n], keys [n], offsets [n_leaves + 2], int32."""
     ids = leaves if leaves.dim() == 1 else leaves.reshape(-1)
     n = ids.numel()
     if not ids.is_cuda:
@@ -175,14 +180,14 @@ def _route(leaves: torch.Tensor, n_leaves: int) -> LeafRoute:
         key, order = torch.sort(key, stable=True)
         bounds = torch.arange(n_leaves + 1, dtype=torch.int64)
         offsets = torch.cat([torch.searchsorted(key, bounds), torch.tensor([n])])
-        return LeafRoute(leaves, n_leaves, torch.cat([order, key, offsets]).int())
+        return torch.cat([order, key, offsets]).int()
     _check_launch(ids)
     hip, dev, ids = native.hip(), ids.get_device(), ids.contiguous()
     buf = ids.new_empty(hip.leaf_route_len(n, n_leaves), dtype=torch.int32)
     work = _scratch(4 * hip.leaf_route_words(n, n_leaves), ids)
     hip.leaf_route(dev, _stream(dev), ids.data_ptr(), ids.dtype == torch.int64, n, n_leaves,
                    buf.data_ptr(), work.data_ptr())
-    return LeafRoute(leaves, n_leaves, buf)
+    return buf
 
 
 # ---------------------------------------------------------------------------- embedding
@@ -205,43 +210,49 @@ def _embed_forward(ids: torch.Tensor, table: torch.Tensor, scale: float) -> torc
     return y
 
 
-def _sum_by_leaf_plain(dy, route: LeafRoute, scale: float) -> torch.Tensor:
-    V = route.n_leaves
+def _sum_by_leaf_plain(dy, buf, V: int, scale: float) -> torch.Tensor:
+    n = dy.shape[0]
     out = torch.zeros((V + 1, dy.shape[1]), dtype=torch.float64)
-    out.index_add_(0, route.keys.long(), dy[route.order.long()].double())
+    out.index_add_(0, buf[n : 2 * n].long(), dy[buf[:n].long()].double())
     scale = torch.tensor(scale, dtype=torch.float32).double()  # as the forward pass has it
     return (out[:V] * scale).to(dy.dtype)
 
 
-def _embed_grad(dy, ids, route, n_leaves: int, scale: float) -> torch.Tensor:
-    """scale * the sum of dy's rows of each leaf, [n_leaves, D]."""
+def _embed_grad(dy, ids, buf, n_leaves: int, scale: float) -> torch.Tensor:
+    """scale * the sum of dy's rows of each leaf, [n_leaves, D], from the leaf numbers or a route's
+    buffer."""
     D = dy.shape[-1]
     if not dy.is_cuda:
-        route = route if route is not None else _route(ids, n_leaves)
-        return _sum_by_leaf_plain(dy.reshape(-1, D), route, scale)
+        buf = buf if buf is not None else _sort(ids, n_leaves)
+        return _sum_by_leaf_plain(dy.reshape(-1, D), buf, n_leaves, scale)
     _check_launch(dy, ids)
-    hip, kind, dev = native.hip(), _TYPES[dy.dtype], dy.get_device()
-    dy, ids = _rows(dy), ids.contiguous()
+    _check_device(dy, ids, buf)  # (saved tensors come back as their hooks leave them)
+    hip, kind, dev, dy = native.hip(), _TYPES[dy.dtype], dy.get_device(), _rows(dy)
     n = dy.shape[0]
     out = dy.new_empty((n_leaves, D))
-    work = _scratch(hip.leaf_embed_grad_bytes(kind, n, n_leaves, D, route is not None), dy)
-    hip.leaf_embed_grad(dev, _stream(dev), kind, dy.data_ptr(), dy.stride(0), ids.data_ptr(),
-                        ids.dtype == torch.int64, 0 if route is None else route._buf.data_ptr(), n,
+    work = _scratch(hip.leaf_embed_grad_bytes(kind, n, n_leaves, D, buf is not None), dy)
+    if buf is None:
+        ids = ids.contiguous()
+        at, wide, sorted_ = ids.data_ptr(), ids.dtype == torch.int64, 0
+    else:
+        at, wide, sorted_ = 0, False, buf.data_ptr()
+    hip.leaf_embed_grad(dev, _stream(dev), kind, dy.data_ptr(), dy.stride(0), at, wide, sorted_, n,
                         n_leaves, D, scale, out.data_ptr(), work.data_ptr())
     return out
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, ids, route, scale):
-        ctx.route, ctx.scale, ctx.n_leaves = route, scale, table.shape[0]
-        ctx.save_for_backward(ids)
+    def forward(ctx, table, ids, buf, scale):
+        ctx.routed, ctx.scale, ctx.n_leaves = buf is not None, scale, table.shape[0]
+        ctx.save_for_backward(ids if buf is None else buf)
         return _embed_forward(ids, table, scale)
 
     @staticmethod
     def _first(ctx, dy):
-        (ids,) = ctx.saved_tensors
-        return _embed_grad(dy, ids, ctx.route, ctx.n_leaves, ctx.scale), None, None, None
+        (kept,) = ctx.saved_tensors
+        ids, buf = (None, kept) if ctx.routed else (kept, None)
+        return _embed_grad(dy, ids, buf, ctx.n_leaves, ctx.scale), None, None, None
 
     _marked = torch.autograd.function.once_differentiable(_first.__func__)
 
@@ -270,66 +281,68 @@ def leaf_embedding(leaves, table: torch.Tensor, *, scale: float = 1.0) -> torch.
     if not -_MAX_F32 <= scale <= _MAX_F32:
         raise ValueError(f"scale must be finite in float32, got {scale}")
     if table.requires_grad and torch.is_grad_enabled():
-        return _Embedding.apply(table, ids, route, scale)
+        return _Embedding.apply(table, ids, None if route is None else route._buf, scale)
     return _embed_forward(ids, table, scale)
 
 
 # ------------------------------------------------------------------------------- linear
-def _linear_plain(x, route, w, b):
+def _leaf_rows(buf, n: int, G: int):
+    """(leaf, its rows) of the leaves that have rows."""
+    order, bounds = buf[:n].long(), buf[2 * n :].tolist()
+    for g in torch.unique(buf[n : 2 * n]).tolist():
+        if g < G:
+            yield g, order[bounds[g] : bounds[g + 1]]
+
+
+def _linear_plain(x, buf, w, b):
     y = torch.zeros((x.shape[0], w.shape[1]), dtype=torch.float32)
-    bounds = route.offsets.tolist()
-    for g in torch.unique(route.keys).tolist():
-        if g < route.n_leaves:
-            rows = route.order[bounds[g] : bounds[g + 1]].long()
-            out = x[rows].float() @ w[g].float().t()
-            y[rows] = out if b is None else out + b[g].float()
+    for g, rows in _leaf_rows(buf, x.shape[0], w.shape[0]):
+        out = x[rows].float() @ w[g].float().t()
+        y[rows] = out if b is None else out + b[g].float()
     return y.to(x.dtype)
 
 
-def _linear_plain_grad(dy, x, route, w, need_x, need_w):
+def _linear_plain_grad(dy, x, buf, w, need_x, need_w):
     dx = torch.zeros(x.shape, dtype=torch.float32) if need_x else None
     dw = torch.zeros(w.shape, dtype=torch.float32) if need_w else None
-    bounds = route.offsets.tolist()
-    for g in torch.unique(route.keys).tolist():
-        if g < route.n_leaves:
-            rows = route.order[bounds[g] : bounds[g + 1]].long()
-            d = dy[rows].float()
-            if need_x:
-                dx[rows] = d @ w[g].float()
-            if need_w:
-                dw[g] = d.t() @ x[rows].float()
+    for g, rows in _leaf_rows(buf, x.shape[0], w.shape[0]):
+        d = dy[rows].float()
+        if need_x:
+            dx[rows] = d @ w[g].float()
+        if need_w:
+            dw[g] = d.t() @ x[rows].float()
     return (dx.to(x.dtype) if need_x else None), (dw.to(w.dtype) if need_w else None)
 
 
-def _linear_forward(x, ids, route, w, b):
-    """Returns (y, route): the route is made where the kernel needs one."""
-    n, (G, N, K) = x.shape[0], w.shape
+def _linear_forward(x, ids, buf, w, b):
+    """Returns (y, the route's buffer); it is made where the kernel needs one and none is given."""
+    (n, K), (G, N, _) = x.shape, w.shape
     if not x.is_cuda:
-        route = route if route is not None else _route(ids, G)
-        return _linear_plain(x, route, w, b), route
+        buf = buf if buf is not None else _sort(ids, G)
+        return _linear_plain(x, buf, w, b), buf
     _check_launch(x, w, b, ids)
     hip, kind, dev, ids = native.hip(), _TYPES[x.dtype], x.get_device(), ids.contiguous()
     wide, bias = ids.dtype == torch.int64, 0 if b is None else b.data_ptr()
-    y = x.new_empty((n, N))
+    y, (stride, _) = x.new_empty((n, N)), x.stride()
     if n <= hip.LEAF_LINEAR_SMALL_ROWS:
-        hip.leaf_linear_small(dev, _stream(dev), kind, x.data_ptr(), x.stride(0), ids.data_ptr(),
-                              wide, n, G, w.data_ptr(), bias, K, N, y.data_ptr())
-        return y, route
-    work = _scratch(hip.leaf_linear_bytes(kind, x.data_ptr(), x.stride(0), w.data_ptr(), n, G, K,
-                                          N), x)
+        hip.leaf_linear_small(dev, _stream(dev), kind, x.data_ptr(), stride, ids.data_ptr(), wide,
+                              n, G, w.data_ptr(), bias, K, N, y.data_ptr())
+        return y, buf
+    work = _scratch(hip.leaf_linear_bytes(kind, x.data_ptr(), stride, w.data_ptr(), n, G, K, N), x)
     sort = 0
-    if route is None:
+    if buf is None:
         sort = ids.data_ptr()
-        route = LeafRoute(ids, G, ids.new_empty(hip.leaf_route_len(n, G), dtype=torch.int32))
-    hip.leaf_linear(dev, _stream(dev), kind, x.data_ptr(), x.stride(0), sort, wide,
-                    route._buf.data_ptr(), n, G, w.data_ptr(), bias, K, N, y.data_ptr(),
-                    work.data_ptr())
-    return y, route
+        buf = ids.new_empty(hip.leaf_route_len(n, G), dtype=torch.int32)
+    hip.leaf_linear(dev, _stream(dev), kind, x.data_ptr(), stride, sort, wide, buf.data_ptr(), n,
+                    G, w.data_ptr(), bias, K, N, y.data_ptr(), work.data_ptr())
+    return y, buf
 
 
-def _linear_grad(dy, x, route, w, need_x, need_w, need_b):
+def _linear_grad(dy, x, buf, w, need_x, need_w, need_b):
     n, (G, N, K) = x.shape[0], w.shape
-    _check_launch(dy)
+    _check_launch(dy, x, w)
+    _check_device(dy, x, w, buf)  # (saved tensors come back as their hooks leave them)
+    x, w = _flat(x), w.contiguous()
     hip, kind, dev, dy = native.hip(), _TYPES[x.dtype], x.get_device(), _rows(dy)
     dx = x.new_empty((n, K)) if need_x else None
     dw = x.new_empty((G, N, K)) if need_w else None
@@ -338,7 +351,7 @@ def _linear_grad(dy, x, route, w, need_x, need_w, need_b):
                                                dy.stride(0), w.data_ptr(), n, G, K, N, need_x,
                                                need_w), x)
     hip.leaf_linear_grad(dev, _stream(dev), kind, x.data_ptr(), x.stride(0), dy.data_ptr(),
-                         dy.stride(0), route._buf.data_ptr(), n, G, w.data_ptr(), K, N,
+                         dy.stride(0), buf.data_ptr(), n, G, w.data_ptr(), K, N,
                          *(0 if t is None else t.data_ptr() for t in (dx, dw, db)),
                          work.data_ptr())
     return dx, dw, db
@@ -346,21 +359,22 @@ def _linear_grad(dy, x, route, w, need_x, need_w, need_b):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, b, ids, route):
-        y, ctx.route = _linear_forward(x, ids, route, w, b)
-        ctx.save_for_backward(x, w, ids)
+    def forward(ctx, x, w, b, ids, buf):
+        y, buf = _linear_forward(x, ids, buf, w, b)
+        ctx.routed = buf is not None
+        ctx.save_for_backward(x, w, buf if ctx.routed else ids)
         return y
 
     @staticmethod
     def _first(ctx, dy):
-        x, w, ids = ctx.saved_tensors
+        x, w, kept = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        route = ctx.route if ctx.route is not None else _route(ids, w.shape[0])
+        buf = kept if ctx.routed else _sort(kept, w.shape[0])
         if x.is_cuda:
-            grads = _linear_grad(dy, x, route, w, need_x, need_w, need_b)
+            grads = _linear_grad(dy, x, buf, w, need_x, need_w, need_b)
         else:
-            grads = _linear_plain_grad(dy, x, route, w, need_x, need_w)
-            grads += (_sum_by_leaf_plain(dy, route, 1.0) if need_b else None,)
+            grads = _linear_plain_grad(dy, x, buf, w, need_x, need_w)
+            grads += (_sum_by_leaf_plain(dy, buf, w.shape[0], 1.0) if need_b else None,)
         return (*grads, None, None)
 
     _marked = torch.autograd.function.once_differentiable(_first.__func__)
@@ -395,12 +409,13 @@ def leaf_linear(inputs: torch.Tensor, leaves, weight: torch.Tensor, bias=None) -
             raise ValueError(f"bias has shape {tuple(bias.shape)}, expected {(G, N)}")
         bias = bias.contiguous()
     _check_device(inputs, ids, weight, bias)
-    x, weight = _rows(inputs), weight.contiguous()
+    x, weight = _flat(inputs), weight.contiguous()
+    buf = None if route is None else route._buf
     one = ids.dim() == 1
     flat = ids if one else ids.reshape(-1)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                     or bias is not None and bias.requires_grad):
-        y = _Linear.apply(x, weight, bias, flat, route)
+        y = _Linear.apply(x, weight, bias, flat, buf)
     else:
-        y = _linear_forward(x, flat, route, weight, bias)[0]
+        y = _linear_forward(x, flat, buf, weight, bias)[0]
     return y if one else y.reshape(*ids.shape, N)

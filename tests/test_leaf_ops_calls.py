@@ -1,5 +1,7 @@
 """Calls of the operators over a tree's leaves that have to be right or refused."""
 
+import gc
+
 import numpy as np
 import pytest
 import torch
@@ -8,7 +10,8 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils.flop_counter import FlopCounterMode
 
-from mpitree_amd import DecisionTreeClassifier, leaf_embedding, leaf_linear, leaf_route
+from mpitree_amd import (DecisionTreeClassifier, LeafRoute, leaf_embedding, leaf_linear,
+                         leaf_route)
 from mpitree_amd.ops import leaf_ops, native
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -294,3 +297,70 @@ def test_the_number_of_leaves_is_whole(n_leaves):
 def test_whole_numbers_of_any_type(n_leaves):
     r = leaf_route(torch.tensor([2, 0]), n_leaves)
     assert r.n_leaves == 3 and type(r.n_leaves) is int
+
+
+# ----------------------------------------------------------------- what a graph keeps
+def kept_by_hooks(call, args, device):
+    """Runs call with its saved tensors moved to the host; their types and shapes, the gradients."""
+    seen = []
+
+    def pack(t):
+        seen.append((t.dtype, t.numel()))
+        return t.cpu().clone()
+
+    args = [a.detach().clone().requires_grad_() for a in args]
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.to(device)):
+        y = call(*args)
+    routes = sum(isinstance(o, LeafRoute) for o in gc.get_objects())
+    return seen, routes, [y, *torch.autograd.grad(y.sum(), args)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_saved_tensors_are_all_that_a_graph_keeps(device):
+    # a route made inside a call too: hooks see it, and it goes with the saved tensors
+    gc.collect()
+    before = sum(isinstance(o, LeafRoute) for o in gc.get_objects())
+    ids, x, w, b = operands(device, 90)
+    route = leaf_route(ids, 3)
+    size = 2 * 90 + 3 + 2
+    for leaves in (ids, route):
+        for call, args, want in (
+                (lambda t: leaf_embedding(leaves, t), [b],
+                 [(torch.int32, size) if leaves is route else (torch.int64, 90)]),
+                (lambda x, w, b: leaf_linear(x, leaves, w, b), [x, w, b],
+                 [(torch.float32, x.numel()), (torch.float32, w.numel()), (torch.int32, size)])):
+            seen, routes, got = kept_by_hooks(call, args, device)
+            assert seen == want and routes == before + 1
+            args = [a.detach().clone().requires_grad_() for a in args]
+            y = call(*args)
+            for p, q in zip(got, (y, *torch.autograd.grad(y.sum(), args))):
+                assert torch.equal(p, q)
+
+
+def test_a_rewritten_route_is_noticed():
+    ids, x, w, b = operands("cpu", 90)
+    route, b = leaf_route(ids, 3), b.requires_grad_()
+    y, z = leaf_embedding(route, b), leaf_linear(x, route, w, b)
+    route.order.zero_()
+    for out in (y, z):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+
+
+@pytest.mark.gpu
+def test_saved_tensors_that_come_back_elsewhere():
+    # a hook that leaves them on the host is refused, one that returns other strides is not
+    ids, x, w, b = operands("cuda", 90)
+    for call, args in ((lambda t: leaf_embedding(ids, t), [b]),
+                       (lambda x, w, b: leaf_linear(x, ids, w, b), [x, w, b])):
+        args = [a.detach().clone().requires_grad_() for a in args]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t):
+            y = call(*args)
+        with pytest.raises((ValueError, RuntimeError), match="device"):
+            torch.autograd.grad(y.sum(), args)
+        with torch.autograd.graph.saved_tensors_hooks(
+                lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t):
+            y = call(*args)
+        got = torch.autograd.grad(y.sum(), args)
+        for p, q in zip(got, torch.autograd.grad(call(*args).sum(), args)):
+            assert torch.equal(p, q)
