@@ -27,7 +27,7 @@ int64_t leaf_linear_bytes(int, const void*, int64_t, const void*, int64_t, int, 
 void launch_leaf_linear(hipStream_t, int, const void*, int64_t, const int32_t*, const int32_t*,
                         int64_t, int, const void*, const void*, int, int, void*, void*);
 int64_t leaf_linear_grad_bytes(int, const void*, int64_t, const void*, int64_t, const void*,
-                               int64_t, int, int, int, bool, bool);
+                               int64_t, int, int, int, bool, bool, bool);
 void launch_leaf_linear_grad(hipStream_t, int, const void*, int64_t, const void*, int64_t,
                              const int32_t*, const uint32_t*, const int32_t*, int64_t, int,
                              const void*, int, int, void*, void*, void*, void*);
@@ -123,10 +123,10 @@ void bind_leaf(py::module_& m) {
     launch_leaf_linear_small(S(s), type, P<void>(x), x_stride, P<void>(ids), wide, n, G,
                              P<void>(w), P<void>(bias), K, N, P<void>(y));
   });
-  // ids != 0: the rows are sorted into `route` first; else it holds the sort
+  // ids != 0: the rows are sorted into `route` first; else it holds the sort (routed)
   m.def("leaf_linear_bytes", [](int type, uintptr_t x, int64_t x_stride, uintptr_t w, int64_t n,
-                                int G, int K, int N) {
-    return std::max(4 * leaf_route_words(n, G),
+                                int G, int K, int N, bool routed) {
+    return std::max(routed ? 0 : 4 * leaf_route_words(n, G),
                     leaf_linear_bytes(type, P<void>(x), x_stride, P<void>(w), n, G, K, N));
   });
   m.def("leaf_linear", [](int dev, uintptr_t s, int type, uintptr_t x, int64_t x_stride,
@@ -144,9 +144,9 @@ void bind_leaf(py::module_& m) {
   // dx, dw and db, each where its address is not 0
   m.def("leaf_linear_grad_bytes", [](int type, uintptr_t x, int64_t x_stride, uintptr_t dy,
                                      int64_t dy_stride, uintptr_t w, int64_t n, int G, int K, int N,
-                                     bool dx, bool dw) {
+                                     bool dx, bool dw, bool db) {
     return leaf_linear_grad_bytes(type, P<void>(x), x_stride, P<void>(dy), dy_stride, P<void>(w), n,
-                                  G, K, N, dx, dw);
+                                  G, K, N, dx, dw, db);
   });
   m.def("leaf_linear_grad", [](int dev, uintptr_t s, int type, uintptr_t x, int64_t x_stride,
                                uintptr_t dy, int64_t dy_stride, uintptr_t route, int64_t n, int G,

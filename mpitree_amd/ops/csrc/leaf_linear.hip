@@ -1717,11 +1717,11 @@ void launch_leaf_linear(hipStream_t s, int type, const void* x, int64_t x_stride
 
 int64_t leaf_linear_grad_bytes(int type, const void* x, int64_t x_stride, const void* dy,
                                int64_t dy_stride, const void* w, int64_t n, int G, int K, int N,
-                               bool dx, bool dw) {
+                               bool dx, bool dw, bool db) {
   const LlPacks p = ll_grad_packs(type, x, x_stride, dy, dy_stride, w, n, G, K, N, dx, dw);
-  return p.bytes(type, n, G, K, N) + std::max({ll_plan_bytes(n, G),
-                                               ll_part_bytes(type, n, G, K, N),
-                                               leaf_embed_grad_bytes(type, n, N)});
+  return p.bytes(type, n, G, K, N) + std::max({dx ? ll_plan_bytes(n, G) : 0,
+                                               dw ? ll_part_bytes(type, n, G, K, N) : 0,
+                                               db ? leaf_embed_grad_bytes(type, n, N) : 0});
 }
 
 // dx, dw and db, each where it is not null; their scratch is used by one after the other

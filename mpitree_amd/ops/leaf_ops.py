@@ -328,7 +328,8 @@ def _linear_forward(x, ids, buf, w, b):
         hip.leaf_linear_small(dev, _stream(dev), kind, x.data_ptr(), stride, ids.data_ptr(), wide,
                               n, G, w.data_ptr(), bias, K, N, y.data_ptr())
         return y, buf
-    work = _scratch(hip.leaf_linear_bytes(kind, x.data_ptr(), stride, w.data_ptr(), n, G, K, N), x)
+    work = _scratch(hip.leaf_linear_bytes(kind, x.data_ptr(), stride, w.data_ptr(), n, G, K, N,
+                                          buf is not None), x)
     sort = 0
     if buf is None:
         sort = ids.data_ptr()
@@ -349,7 +350,7 @@ def _linear_grad(dy, x, buf, w, need_x, need_w, need_b):
     db = x.new_empty((G, N)) if need_b else None
     work = _scratch(hip.leaf_linear_grad_bytes(kind, x.data_ptr(), x.stride(0), dy.data_ptr(),
                                                dy.stride(0), w.data_ptr(), n, G, K, N, need_x,
-                                               need_w), x)
+                                               need_w, need_b), x)
     hip.leaf_linear_grad(dev, _stream(dev), kind, x.data_ptr(), x.stride(0), dy.data_ptr(),
                          dy.stride(0), buf.data_ptr(), n, G, w.data_ptr(), K, N,
                          *(0 if t is None else t.data_ptr() for t in (dx, dw, db)),
@@ -370,7 +371,7 @@ class _Linear(torch.autograd.Function):
         x, w, kept = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         buf = kept if ctx.routed else _sort(kept, w.shape[0])
-        if x.is_cuda:
+        if dy.is_cuda:
             grads = _linear_grad(dy, x, buf, w, need_x, need_w, need_b)
         else:
             grads = _linear_plain_grad(dy, x, buf, w, need_x, need_w)

@@ -364,3 +364,54 @@ def test_saved_tensors_that_come_back_elsewhere():
         got = torch.autograd.grad(y.sum(), args)
         for p, q in zip(got, torch.autograd.grad(call(*args).sum(), args)):
             assert torch.equal(p, q)
+
+
+# ----------------------------------------------------------------------------- scratch
+def test_scratch_is_of_what_a_call_makes():
+    # 65536 rows, 64 leaves, 2048 -> 2048 bf16: partial matrices with a weight gradient only
+    h, at = native.hip(), 1 << 20
+    n, G, K, N = 65_536, 64, 2048, 2048
+
+    def grad(dx, dw, db):
+        return h.leaf_linear_grad_bytes(2, at, K, at, N, at, n, G, K, N, dx, dw, db)
+
+    assert grad(True, False, False) < 2 ** 14  # the tile list: 8 bytes for each 256 rows and leaf
+    assert grad(False, False, False) == 0
+    assert 0 < grad(False, False, True) == h.leaf_embed_grad_bytes(2, n, G, N, True)
+    assert grad(True, True, False) >= 2 * N * K * 4
+    assert grad(True, False, True) == max(grad(True, False, False), grad(False, False, True))
+    assert grad(True, True, True) == max(grad(True, True, False), grad(False, False, True))
+
+    def forward(n, K, N, routed):
+        return h.leaf_linear_bytes(0, at, K, at, n, 4096, K, N, routed)
+
+    assert forward(10 ** 6, 64, 64, True) == 0  # nothing is sorted, no tiles listed
+    assert forward(10 ** 6, 64, 64, False) == 4 * h.leaf_route_words(10 ** 6, 4096)
+    # operands that are copied into whole chunks are so in every call
+    odd = [h.leaf_linear_grad_bytes(2, at, 2047, at, 2049, at, n, G, 2047, 2049, dx, dw, False)
+           for dx, dw in ((True, False), (False, True))]
+    assert odd[0] >= n * 2056 * 2 + G * 2049 * 2048 * 2 and odd[1] >= n * (2048 + 2056) * 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,G,K,N", [(90, 3, 6, 5), (5000, 4, 24, 40), (9000, 3, 200, 129),
+                                     (9000, 3, 1032, 520), (1000, 2500, 64, 64)])
+def test_every_subset_of_the_gradients(dtype, n, G, K, N):
+    # each with the scratch that is its own; from leaf numbers and from a route
+    g = torch.Generator().manual_seed(n + K)
+    ids = torch.randint(-1, G, (n,), generator=g).cuda()
+    # whole numbers of few bits: sums in any order are exact
+    x, w, b, dy = (torch.randint(-2, 3, s, generator=g).to(dtype).cuda()
+                   for s in ((n, K), (G, N, K), (G, N), (n, N)))
+    for leaves in (ids, leaf_route(ids, G)):
+        full = None
+        for need in ("xwb", "x", "w", "b", "xw", "wb", "xb"):
+            args = {k: t.detach().clone().requires_grad_(k in need)
+                    for k, t in zip("xwb", (x, w, b))}
+            y = leaf_linear(args["x"], leaves, args["w"], args["b"])
+            got = dict(zip(need, torch.autograd.grad(y, [args[k] for k in need], dy)))
+            full = full or (y, got)
+            assert torch.equal(y, full[0])
+            for k in need:
+                assert torch.equal(got[k], full[1][k]), (need, k)
