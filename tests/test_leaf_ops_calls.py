@@ -65,9 +65,13 @@ def forward_calls(device):
     """(call, its operands that may have a tangent) of each operator."""
     for n in (9, 90):  # the form for few rows and the tiles
         ids, x, w, b = operands(device, n)
-        for leaves in (ids, leaf_route(ids, 3)):
-            yield (lambda t, leaves=leaves: leaf_embedding(leaves, t, scale=0.5)), [b]
-            yield (lambda x, w, b, leaves=leaves: leaf_linear(x, leaves, w, b)), [x, w, b]
+        yield from calls_of(ids, x, w, b)
+        yield from calls_of(leaf_route(ids, 3), x, w, b)
+
+
+def calls_of(leaves, x, w, b):
+    yield (lambda t: leaf_embedding(leaves, t, scale=0.5)), [b]
+    yield (lambda x, w, b: leaf_linear(x, leaves, w, b)), [x, w, b]
 
 
 @pytest.mark.gpu
@@ -311,7 +315,7 @@ def kept_by_hooks(call, args, device):
     args = [a.detach().clone().requires_grad_() for a in args]
     with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.to(device)):
         y = call(*args)
-    routes = sum(isinstance(o, LeafRoute) for o in gc.get_objects())
+    routes = sum(type(o) is LeafRoute for o in gc.get_objects())
     return seen, routes, [y, *torch.autograd.grad(y.sum(), args)]
 
 
@@ -319,7 +323,7 @@ def kept_by_hooks(call, args, device):
 def test_saved_tensors_are_all_that_a_graph_keeps(device):
     # a route made inside a call too: hooks see it, and it goes with the saved tensors
     gc.collect()
-    before = sum(isinstance(o, LeafRoute) for o in gc.get_objects())
+    before = sum(type(o) is LeafRoute for o in gc.get_objects())
     ids, x, w, b = operands(device, 90)
     route = leaf_route(ids, 3)
     size = 2 * 90 + 3 + 2
