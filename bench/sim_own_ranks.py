@@ -21,7 +21,7 @@ finisher share, exchange stand-in, assembly + the full tree's D2H):
 * ``rows_owned`` / ``units`` -- the LPT's per-rank rows and the unit count.
 
     python bench/sim_own_ranks.py [--n 1000000] [--features 64] [--ranks 1,2,4,8]
-                                  [--regression] [--continuous]
+                                  [--regression] [--registered]
 
 ``--regression``: the 1M x 64 MSE regression tree, whose
 exchange rows carry int64 {count, sum} statistics.
@@ -41,14 +41,18 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 from mpitree_amd.core.levelwise import LocalComm  # noqa: E402
-from mpitree_amd.parallel.shared_tree import GATHER_HDR  # noqa: E402
+from mpitree_amd.parallel.shared_tree import GATHER_HDR, _Slot  # noqa: E402
 
 
 class SimSlot:
     """The shared tree buffer stand-in: mapped pinned host memory holding the
-    reference tree's packed columns (the other ranks' nodes) before each fit."""
+    reference tree's packed columns (the other ranks' nodes) before each fit.
+    ``registered``: kernels store into it; else nodes are copied into it."""
 
-    def __init__(self, ref_bytes: np.ndarray):
+    copy_nodes = _Slot.copy_nodes
+    column_widths = staticmethod(_Slot.column_widths)
+
+    def __init__(self, ref_bytes: np.ndarray, registered: bool = False):
         import ctypes
 
         from mpitree_amd.ops import native
@@ -58,7 +62,7 @@ class SimSlot:
         size = HEADER + ref_bytes.size
         self.host = int(hip.host_alloc(size, coherent=False))
         self.nd = np.ctypeslib.as_array((ctypes.c_uint8 * size).from_address(self.host))
-        self.dev = int(hip.host_device_ptr(self.host))
+        self.dev = int(hip.host_device_ptr(self.host)) if registered else 0
         self.nbytes = size
         self.ref = ref_bytes
         self.header = HEADER
@@ -190,6 +194,9 @@ def main():
                     help="force the feature-parallel prefix levels off / on")
     ap.add_argument("--no-shared", action="store_true",
                     help="node exchange + full-tree copy instead of the shared-host assembly")
+    ap.add_argument("--registered", action="store_true",
+                    help="kernels store into the shared buffer (MPITREE_SHM_REGISTER=1); the "
+                         "default copies each rank's nodes into it")
     ap.add_argument("--cprofile", default=None,
                     help="write a cProfile of the timed fits' host code to this file")
     a = ap.parse_args()
@@ -225,7 +232,7 @@ def main():
     ref_pos = ref_rows[:, 0].long().contiguous()  # live positions, ascending
     pool = None
     if not a.no_shared:
-        pool = SimPool(SimSlot(packed_bytes(ref.arrays)))
+        pool = SimPool(SimSlot(packed_bytes(ref.arrays), a.registered))
     for P in [int(v) for v in a.ranks.replace("+", ",").split(",")]:
         per_rank = []
         for r in range(P) if a.only_rank is None else [a.only_rank]:

@@ -524,13 +524,18 @@ int shm_max_segs() { return kShmMaxSegs; }
 
 // One workgroup: every segment's count (summed over the gathered rows: one owner
 // each), the segments sorted by lo (bitonic, LDS), the running count of other
-// ranks' nodes -> tab [S][4]; unused entries get lo = INT64_MAX (sorted last).
+// ranks' nodes -> tab [S][4]; unused entries get lo = INT64_MAX (sorted last). runs [S][3], in
+// the same order: the ids of a segment's nodes in the whole tree, {first, count, owner}.
 // total becomes the whole tree's {nodes, depth}.
 __global__ __launch_bounds__(1024) void shm_seg_prefix_kernel(const int64_t* __restrict__ gall,
                                                               int nranks, int W,
                                                               const int64_t* __restrict__ segs,
-                                                              int S, int me, int64_t* __restrict__ total,
-                                                              int64_t* __restrict__ tab) {
+                                                              int S, int me,
+                                                              const int32_t* __restrict__ rank,
+                                                              int64_t P,
+                                                              int64_t* __restrict__ total,
+                                                              int64_t* __restrict__ tab,
+                                                              int64_t* __restrict__ runs) {
   __shared__ uint64_t key[kShmMaxSegs];
   __shared__ int32_t idx[kShmMaxSegs];
   __shared__ int64_t wsum[1024 / kWave];
@@ -571,15 +576,16 @@ __global__ __launch_bounds__(1024) void shm_seg_prefix_kernel(const int64_t* __r
   __syncthreads();
   for (int b0 = 0; b0 < S; b0 += 1024) {
     const int k = b0 + tid;
-    int64_t v = 0, lo = INT64_MAX, hi = INT64_MAX, owner = -1;
+    int64_t v = 0, lo = INT64_MAX, hi = INT64_MAX, owner = -1, c = 0, before = 0;
     if (k < S && key[k] != ~0ull) {
       const int s = idx[k];
       lo = segs[(int64_t)s * 3 + 0];
       hi = segs[(int64_t)s * 3 + 1];
       owner = segs[(int64_t)s * 3 + 2];
-      int64_t c = 0;
       for (int r = 0; r < nranks; ++r) c += gall[(int64_t)r * W + kShmHdr + s];
       v = owner != me ? c : 0;
+      const int64_t j = lo < P ? (int64_t)rank[lo] : total[0];  // (as in shm_seg_count_kernel)
+      before = j >= 0 ? j : ~j;
     }
     // inclusive block scan of v
     int64_t x = v;
@@ -596,6 +602,9 @@ __global__ __launch_bounds__(1024) void shm_seg_prefix_kernel(const int64_t* __r
       tab[(int64_t)k * 4 + 1] = hi;
       tab[(int64_t)k * 4 + 2] = owner;
       tab[(int64_t)k * 4 + 3] = off + x;
+      runs[(int64_t)k * 3 + 0] = before + off + x - v;
+      runs[(int64_t)k * 3 + 1] = c;
+      runs[(int64_t)k * 3 + 2] = owner;
     }
     __syncthreads();
     if (tid == 1023) carry = off + x;
@@ -617,10 +626,11 @@ void launch_shm_seg_count(hipStream_t stream, const int64_t* segs, int S, int me
 }
 
 void launch_shm_seg_prefix(hipStream_t stream, const int64_t* gall, int nranks, int W,
-                           const int64_t* segs, int S, int me, int64_t* total, int64_t* tab) {
+                           const int64_t* segs, int S, int me, const int32_t* rank,
+                           int64_t P, int64_t* total, int64_t* tab, int64_t* runs) {
   if (S > kShmMaxSegs) throw std::runtime_error("shared-host assembly: too many segments");
   hipLaunchKernelGGL(shm_seg_prefix_kernel, dim3(1), dim3(1024), 0, stream, gall, nranks, W, segs,
-                     S, me, total, tab);
+                     S, me, rank, P, total, tab, runs);
   MT_HIP_CHECK(hipGetLastError());
 }
 

@@ -107,7 +107,7 @@ void launch_shm_seg_count(hipStream_t, const int64_t*, int, int, const int32_t*,
                           const int64_t*, int64_t*);
 int shm_max_segs();
 void launch_shm_seg_prefix(hipStream_t, const int64_t*, int, int, const int64_t*, int, int,
-                           int64_t*, int64_t*);
+                           const int32_t*, int64_t, int64_t*, int64_t*, int64_t*);
 }  // namespace mt
 
 template <typename T>
@@ -459,9 +459,11 @@ PYBIND11_MODULE(_hip, m) {
   });
   m.def("shm_max_segs", &mt::shm_max_segs);  // segments one shared assembly can sort
   m.def("shm_seg_prefix", [](uintptr_t s, uintptr_t gall, int nranks, int W, uintptr_t segs,
-                             int S_, int me, uintptr_t total, uintptr_t tab) {
+                             int S_, int me, uintptr_t rank, int64_t n_pos, uintptr_t total,
+                             uintptr_t tab, uintptr_t runs) {
     mt::launch_shm_seg_prefix(S(s), P<int64_t>(gall), nranks, W, P<int64_t>(segs), S_, me,
-                              P<int64_t>(total), P<int64_t>(tab));
+                              P<int32_t>(rank), n_pos, P<int64_t>(total), P<int64_t>(tab),
+                              P<int64_t>(runs));
   });
   // pin (and map for device access) host memory the process did not allocate
   // through HIP, e.g. a /dev/shm mapping several ranks share

@@ -804,29 +804,35 @@ class HipBackend:
         prefix) into one shared host buffer (``parallel/shared_tree.py``). None
         (on every rank alike) when the node's /dev/shm cannot hold a new buffer
         for the tree: the caller falls back to the node exchange."""
-        from ..parallel.shared_tree import GATHER_HDR, HEADER, shm_free_bytes
+        from ..parallel.shared_tree import GATHER_HDR, HEADER, own_runs, shm_free_bytes
 
         comm, pool, segs, S = sh["comm"], sh["pool"], sh["segs"], int(sh["S"])
         hip = self.hip
         s = _stream()
         Pn, me = int(comm.world_size), int(comm.rank)
         W = GATHER_HDR + int(segs.shape[0])
-        nw = W * (Pn + 1) + 4 * int(segs.shape[0])
+        o_tab = W * (Pn + 1)
+        o_runs = o_tab + 4 * int(segs.shape[0])
+        nw = o_runs + 3 * S
         g = _workspace(self.device, "shm.seg", nw * 8)[: nw * 8].view(torch.int64)
-        gvec, gall, tab = g[:W], g[W : W * (Pn + 1)], g[W * (Pn + 1) :]
+        gvec, gall, tab, runs = g[:W], g[W:o_tab], g[o_tab:o_runs], g[o_runs:]
         hip.shm_seg_count(s, segs.data_ptr(), S, me, rank_ptr, self.P, total.data_ptr(),
                           gvec.data_ptr())
         gvec[1].fill_(pool.free_mask())
         gvec[2].fill_(shm_free_bytes())
         comm.all_gather_seg_counts(gall, gvec, segs, S)
-        hip.shm_seg_prefix(s, gall.data_ptr(), Pn, W, segs.data_ptr(), S, me, total.data_ptr(),
-                           tab.data_ptr())
+        hip.shm_seg_prefix(s, gall.data_ptr(), Pn, W, segs.data_ptr(), S, me, rank_ptr,
+                           self.P, total.data_ptr(), tab.data_ptr(), runs.data_ptr())
         kw = dict(tab=tab.data_ptr(), n_tab=S, me=me, emit_prefix=me == 0)
         slot = pool.take_next()  # (agreed last fit: emit before the host wait)
-        if slot is not None and slot.dev:
-            emit(slot.dev + HEADER, (slot.nbytes - HEADER) // bpn, **kw)
+        stage = None  # (not registered: this rank's nodes go through its own pinned memory)
+        if slot is not None:
+            dptr = slot.dev + HEADER
+            if not slot.dev:
+                stage, dptr = _zc_out(slot.nbytes - HEADER)
+            emit(dptr, (slot.nbytes - HEADER) // bpn, **kw)
         gv = gall.view(Pn, W)
-        h = _pinned_copy(torch.cat([total, gv[:, 1], gv[:, 2]]), "shm.total")
+        h = _pinned_copy(torch.cat([total, gv[:, 1], gv[:, 2], runs]), "shm.total")
         torch.cuda.current_stream(self.device).synchronize()
         self._check_finisher_watch()
         N, max_depth = int(h[0]), int(h[1])
@@ -837,15 +843,13 @@ class HipBackend:
             slot = pool.choose(masks, nbytes, shm_free=free)
             if slot is None:
                 return None
-            if slot.dev:
-                emit(slot.dev + HEADER, 0, **kw)
-                torch.cuda.current_stream(self.device).synchronize()
-        if not slot.dev:  # (not registered: through this rank's own pinned memory)
-            stage, dptr = _zc_out(nbytes)
-            stage[nbytes - 4 * N : nbytes].view(np.int32)[:] = -1
+            dptr = slot.dev + HEADER
+            if not slot.dev:
+                stage, dptr = _zc_out(nbytes)
             emit(dptr, 0, **kw)
             torch.cuda.current_stream(self.device).synchronize()
-            slot.copy_nodes(stage[:nbytes], N)
+        if not slot.dev:
+            slot.copy_nodes(stage[:nbytes], N, own_runs(h[2 + 2 * Pn :].reshape(S, 3), N, me))
         pool.barrier(slot)
         pool.plan_next(masks, slot, nbytes, shm_free=free)
         self.pos_rec = self.pos_st = None

@@ -165,3 +165,41 @@ def test_two_ranks_nodes_make_one_tree(C, scattered):
         slot.copy_nodes(stage, N)
     assert np.array_equal(slot.nd[st.HEADER : st.HEADER + N * width], tree)
     slot.close()
+
+
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("many", [False, True])
+def test_runs_of_ids_make_one_tree(seed, many):
+    """Segments in ascending order with prefix nodes between some of them, empty ones and
+    neighbours: every id is written by one rank, and the copied nodes are the tree."""
+    rng = np.random.default_rng(seed)
+    P, S = 4, 900 if many else 30
+    count = rng.integers(0, 4 if many else 60, size=S)
+    gap = rng.integers(0, 3, size=S + 1) * (rng.random(S + 1) < 0.5)
+    first = np.cumsum(gap[:-1]) + np.concatenate([[0], np.cumsum(count)[:-1]])
+    N = int(gap.sum() + count.sum())
+    segs = np.stack([first, count, rng.integers(0, P, size=S)], 1).astype(np.int64)
+    segs = np.concatenate([segs, [[2 ** 63 - 1, 0, -1]]])  # (unused entries come last)
+    owner = np.zeros(N, dtype=int)
+    for a, c, r in segs[:-1].tolist():
+        owner[a : a + c] = r
+    C, width = 3, 3 * 8 + 4 * 3 + 5 * 4
+    tree = rng.integers(0, 255, size=N * width, dtype=np.uint8)
+    pool = _pool(uid=0x5EED500 + seed + 100 * many)
+    slot = pool.choose([0, 0], N * width)
+    for me in range(P):
+        runs = st.own_runs(segs, N, me)
+        mine = np.zeros(N, dtype=bool)
+        for a, b in runs:
+            assert a < b and not mine[a:b].any()
+            mine[a:b] = True
+        assert np.array_equal(mine, owner == me)
+        assert all(b < a for (_, b), (a, _) in zip(runs, runs[1:]))  # (neighbours joined)
+        stage, at = rng.integers(0, 255, size=N * width, dtype=np.uint8), 0
+        for w in st._Slot.column_widths(width):
+            part = slice(at, at + N * w)
+            stage[part].reshape(N, w)[mine] = tree[part].reshape(N, w)[mine]
+            at += N * w
+        slot.copy_nodes(stage, N, runs)
+    assert np.array_equal(slot.nd[st.HEADER : st.HEADER + N * width], tree)
+    slot.close()
