@@ -217,7 +217,10 @@ class _BaseTree(BaseEstimator):
         if inputs is None:
             if isinstance(X, LeafRoute):
                 raise ValueError("a LeafRoute holds no features: pass inputs")
-            rows = X if isinstance(X, torch.Tensor) else torch.from_numpy(_as_numpy_X(X))
+            rows = X
+            if not isinstance(X, torch.Tensor):  # (torch takes no reversed or foreign-endian ones)
+                rows = _as_numpy_X(X)
+                rows = torch.from_numpy(np.require(rows, rows.dtype.newbyteorder("="), "CW"))
             inputs = rows.to(device=weight.device, dtype=weight.dtype)
         return leaf_linear(inputs, leaves, weight, bias)
 

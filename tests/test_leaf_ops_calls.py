@@ -1,6 +1,7 @@
 """Calls of the operators over a tree's leaves that have to be right or refused."""
 
 import gc
+import warnings
 
 import numpy as np
 import pytest
@@ -419,3 +420,28 @@ def test_every_subset_of_the_gradients(dtype, n, G, K, N):
             assert torch.equal(y, full[0])
             for k in need:
                 assert torch.equal(got[k], full[1][k]), (need, k)
+
+
+# ------------------------------------------------------------------ rows of an estimator
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_estimator_takes_rows_of_any_layout(device):
+    # what apply() takes: reversed, read-only, strided, lists, other types
+    X = np.random.default_rng(0).normal(size=(90, 3)).astype(np.float32)
+    est = DecisionTreeClassifier(max_depth=3, device="cpu").fit(X, X[:, 0] + X[:, 1] > 0)
+    w = torch.randn(est.get_n_leaves(), 2, 3, device=device)
+    fixed = X.copy()
+    fixed.flags.writeable = False
+    wide = np.zeros((90, 6), np.float32)
+    wide[:, ::2] = X
+    want = est.leaf_linear(X, w)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        assert torch.equal(est.leaf_linear(X[::-1], w), want.flip(0))
+        assert torch.equal(est.leaf_linear(fixed, w), want)
+        assert torch.equal(est.leaf_linear(np.asfortranarray(X), w), want)
+        assert torch.equal(est.leaf_linear(wide[:, ::2], w), want)
+        assert torch.equal(est.leaf_linear(X.tolist(), w), want)
+        assert torch.equal(est.leaf_linear(X.astype(object), w), want)
+        assert torch.equal(est.leaf_linear(torch.from_numpy(X), w), want)
+        # (numpy's own bytes the other way round)
+        assert torch.equal(est.leaf_linear(X.astype(">f4"), w), want)
