@@ -121,10 +121,10 @@ def _check_width(what: str, width: int):
 
 
 def _check_device(first, *others):
-    dev = first.device
+    dev = first.get_device()  # (numbers: a third of the time; the same one for all but GPUs)
     for t in others:
-        if t is not None and t.device != dev:
-            raise ValueError(f"operands on different devices: {dev}, {t.device}")
+        if t is not None and (t.get_device() != dev or dev < 0 and t.device != first.device):
+            raise ValueError(f"operands on different devices: {first.device}, {t.device}")
 
 
 def _check_launch(*operands):
@@ -199,14 +199,15 @@ def _embed_forward(ids: torch.Tensor, table: torch.Tensor, scale: float) -> torc
         y = table[torch.where(has, flat, 0)].float() * scale
         return torch.where(has[:, None], y, 0.0).to(table.dtype).reshape(*ids.shape, D)
     _check_launch(table, ids)
-    y = table.new_empty((*ids.shape, D))
+    n = ids.numel()
+    y = table.new_empty((n, D) if ids.dim() == 1 else (*ids.shape, D))
     stride, step = table.stride()
     if D > 1 and step != 1:
         table, stride = table.contiguous(), D
     ids, dev = ids.contiguous(), table.get_device()
     native.hip().leaf_embed(dev, _stream(dev), _TYPES[table.dtype], ids.data_ptr(),
-                            ids.dtype == torch.int64, table.data_ptr(), stride, ids.numel(), V, D,
-                            scale, y.data_ptr())
+                            ids.dtype == torch.int64, table.data_ptr(), stride, n, V, D, scale,
+                            y.data_ptr())
     return y
 
 
@@ -221,14 +222,13 @@ def _sum_by_leaf_plain(dy, buf, V: int, scale: float) -> torch.Tensor:
 def _embed_grad(dy, ids, buf, n_leaves: int, scale: float) -> torch.Tensor:
     """scale * the sum of dy's rows of each leaf, [n_leaves, D], from the leaf numbers or a route's
     buffer."""
-    D = dy.shape[-1]
+    n, D = dy.shape if dy.dim() == 2 else (dy.numel() // dy.shape[-1], dy.shape[-1])
     if not dy.is_cuda:
         buf = buf if buf is not None else _sort(ids, n_leaves)
         return _sum_by_leaf_plain(dy.reshape(-1, D), buf, n_leaves, scale)
-    _check_launch(dy, ids)
+    _check_launch(dy)
     _check_device(dy, ids, buf)  # (saved tensors come back as their hooks leave them)
     hip, kind, dev, dy = native.hip(), _TYPES[dy.dtype], dy.get_device(), _rows(dy)
-    n = dy.shape[0]
     out = dy.new_empty((n_leaves, D))
     work = _scratch(hip.leaf_embed_grad_bytes(kind, n, n_leaves, D, buf is not None), dy)
     if buf is None:
@@ -236,23 +236,23 @@ def _embed_grad(dy, ids, buf, n_leaves: int, scale: float) -> torch.Tensor:
         at, wide, sorted_ = ids.data_ptr(), ids.dtype == torch.int64, 0
     else:
         at, wide, sorted_ = 0, False, buf.data_ptr()
-    hip.leaf_embed_grad(dev, _stream(dev), kind, dy.data_ptr(), dy.stride(0), at, wide, sorted_, n,
-                        n_leaves, D, scale, out.data_ptr(), work.data_ptr())
+    hip.leaf_embed_grad(dev, _stream(dev), kind, dy.data_ptr(), dy.stride()[0], at, wide, sorted_,
+                        n, n_leaves, D, scale, out.data_ptr(), work.data_ptr())
     return out
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, buf, scale):
-        ctx.routed, ctx.scale, ctx.n_leaves = buf is not None, scale, table.shape[0]
+        ctx.rest = buf is not None, table.shape[0], scale
         ctx.save_for_backward(ids if buf is None else buf)
         return _embed_forward(ids, table, scale)
 
     @staticmethod
     def _first(ctx, dy):
-        (kept,) = ctx.saved_tensors
-        ids, buf = (None, kept) if ctx.routed else (kept, None)
-        return _embed_grad(dy, ids, buf, ctx.n_leaves, ctx.scale), None, None, None
+        (kept,), (routed, n_leaves, scale) = ctx.saved_tensors, ctx.rest
+        ids, buf = (None, kept) if routed else (kept, None)
+        return _embed_grad(dy, ids, buf, n_leaves, scale), None, None, None
 
     _marked = torch.autograd.function.once_differentiable(_first.__func__)
 
@@ -340,21 +340,22 @@ def _linear_forward(x, ids, buf, w, b):
 
 
 def _linear_grad(dy, x, buf, w, need_x, need_w, need_b):
-    n, (G, N, K) = x.shape[0], w.shape
     _check_launch(dy, x, w)
     _check_device(dy, x, w, buf)  # (saved tensors come back as their hooks leave them)
-    x, w = _flat(x), w.contiguous()
-    hip, kind, dev, dy = native.hip(), _TYPES[x.dtype], x.get_device(), _rows(dy)
+    if not x.dtype == w.dtype == dy.dtype:
+        raise TypeError(f"saved tensors are {x.dtype} and {w.dtype}, the gradient {dy.dtype}")
+    dy, x, w = _rows(dy), _flat(x), w.contiguous()
+    (n, K), (G, N, _) = x.shape, w.shape
+    hip, kind, dev = native.hip(), _TYPES[x.dtype], x.get_device()
     dx = x.new_empty((n, K)) if need_x else None
     dw = x.new_empty((G, N, K)) if need_w else None
     db = x.new_empty((G, N)) if need_b else None
-    work = _scratch(hip.leaf_linear_grad_bytes(kind, x.data_ptr(), x.stride(0), dy.data_ptr(),
-                                               dy.stride(0), w.data_ptr(), n, G, K, N, need_x,
-                                               need_w, need_b), x)
-    hip.leaf_linear_grad(dev, _stream(dev), kind, x.data_ptr(), x.stride(0), dy.data_ptr(),
-                         dy.stride(0), buf.data_ptr(), n, G, w.data_ptr(), K, N,
-                         *(0 if t is None else t.data_ptr() for t in (dx, dw, db)),
-                         work.data_ptr())
+    ops = kind, x.data_ptr(), x.stride()[0], dy.data_ptr(), dy.stride()[0]
+    at = w.data_ptr()
+    work = _scratch(hip.leaf_linear_grad_bytes(*ops, at, n, G, K, N, need_x, need_w, need_b), x)
+    hip.leaf_linear_grad(dev, _stream(dev), *ops, buf.data_ptr(), n, G, at, K, N,
+                         0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
+                         0 if db is None else db.data_ptr(), work.data_ptr())
     return dx, dw, db
 
 

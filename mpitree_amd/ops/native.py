@@ -14,7 +14,7 @@ import torch
 
 _cache: dict = {}
 
-_Tensor = torch.Tensor
+_PLAIN = {torch.Tensor, torch.nn.Parameter, type(None)}
 _no_dispatch = torch._C._disabled_torch_dispatch_impl
 _modes = torch._C._len_torch_dispatch_stack
 _tracing = torch._C._is_tracing
@@ -27,9 +27,8 @@ def check_memory(*tensors) -> None:
     or wrapped tensors), and calls whose torch operations are recorded or faked, where the launch
     itself would leave no trace. (Modes that only watch the operations pass.)"""
     for t in tensors:
-        if type(t) is not _Tensor and t is not None:
-            if type(t).__torch_dispatch__ is not _no_dispatch:
-                raise TypeError(f"native kernels take plain tensors, got {type(t).__name__}")
+        if type(t) not in _PLAIN and type(t).__torch_dispatch__ is not _no_dispatch:
+            raise TypeError(f"native kernels take plain tensors, got {type(t).__name__}")
     if _modes() and any(torch._C._get_dispatch_mode(k) is not None
                         for k in (_Mode.PROXY, _Mode.FAKE, _Mode.FUNCTIONAL)):
         raise RuntimeError("native kernels cannot be traced or run on fake tensors")
