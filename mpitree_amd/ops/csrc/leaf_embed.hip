@@ -14,20 +14,27 @@
 // Sums are held in 32 bits for 16-bit types and in 64 bits for f32: a leaf may hold most of a
 // million rows, and a 64-bit add costs no more than a 32-bit one here, where memory is the bound.
 //
-// Both are bound by memory where rows are wide: 200k rows of 2048 f16 in 120000 leaves forward 261
-// us (4.8 TB/s of a copy's 4.9), gradient 290 us (4.5 TB/s). 1M rows of 63 f32 in 64 leaves 47 and
-// 67 us; 1M rows of 16 f32, random 64-byte reads, forward 22 us.
+// Both are bound by memory where rows are wide. Launches on four sets of operands in turn, where a
+// copy reaches 4.9 TB/s: 200k rows of 2048 f16 in 120000 leaves (87000 of them met) forward 264 us
+// (4.45 TB/s), gradient 291 us (4.5 TB/s). 1M rows of 63 f32 in 64 leaves 57 us (4.5 TB/s) and 70
+// us (3.7 TB/s); on one set, which the last-level cache holds in part, 45 and 65; inside a training
+// pass, where the gradient comes behind the forward pass's writes, 60 and 95. 1M rows of 16 f32 in
+// 93500 leaves, random 64-byte reads, 22 us (3.5 TB/s) and 100 us.
 #include "leaf.h"
 
 namespace mt {
 
 constexpr int kLeThreads = 256;
 // Rows of a group in flight, in the forward pass and in the gradient. Each takes dependent loads
-// (number, row), so narrow vectors need more of them (63 columns of f32 forward: 86 us with 4, 80
-// with 16).
+// (number, row), so narrow vectors need more of them. us, 1M rows of 63 columns of f32 with 4 / 16
+// / 32 forward 62 / 57 / 83, gradient 80 / 70 / 76; 200k rows of 2048 columns of f16 with 4 / 8
+// forward 264 / 269, with 4 / 8 / 16 gradient 294 / 291 / 290.
 constexpr int le_unroll(int bytes) { return bytes >= 16 ? 4 : 16; }
 constexpr int le_batch(int bytes) { return bytes >= 16 ? 8 : 16; }
-constexpr int kLeEmpty = 16;  // leaves that a group looks over for missing rows
+// Leaves that a group looks over for missing rows; a gradient's us with 4 / 16 / 32: 16384 rows, 1M
+// leaves, 63 columns of f32 75 / 59 / 60, 16 columns 15.7 / 16.7 / 17.3; 2000 rows, 200k leaves, 64
+// columns 13.4 / 14.9 / 15.4.
+constexpr int kLeEmpty = 16;
 
 template <typename T>
 struct LeAcc {
@@ -210,7 +217,8 @@ __global__ __launch_bounds__(kLeThreads) void le_backward_kernel(
 // Adds the partial rows of the leaves that reach over a chunk's end. One block (and column block)
 // for each leaf (kByLeaf), or for each chunk in which such a leaf may start, whichever are fewer.
 // Few leaves have many partial rows each, so their blocks are larger (16384 rows of one leaf, 1024
-// columns of bf16: a gradient takes 35 us, 48 with 256 threads).
+// columns of bf16: a gradient takes 36 us, 48 with 256 threads; 1M rows, 64 columns of f32 222 and
+// 677).
 template <bool kByLeaf>
 constexpr int kLeJoinThreads = kByLeaf ? 1024 : kLeThreads;
 template <typename T, int W, bool kByLeaf>
@@ -325,8 +333,8 @@ void launch_leaf_embed(hipStream_t s, int type, const void* ids, bool wide, cons
 
 // Sorted positions of a chunk: 16 to 256, so few that the chunks make about 4096 waves (16 on each
 // CU) of 16-byte vectors, 2048 of narrower ones; longer chunks leave fewer partial rows. us with
-// 1024 or 2048 / 4096 / 8192 or 16384 waves: 1M rows, 63 columns of f32 66 / 79 / 111; 200k rows,
-// 2048 columns of f16 302 / 290 / 303.
+// half / these / two / four times as many: 1M rows, 63 columns of f32 70 / 70 / 78 / 80, 300k rows
+// 47 / 32 / 31 / 32; 200k rows, 2048 columns of f16 302 / 291 / 293 / 302.
 static int le_run_shift(int64_t n, const LeCols& lc, int bytes) {
   const int64_t waves = bytes >= 16 ? 4096 : 2048;
   int shift = 8;

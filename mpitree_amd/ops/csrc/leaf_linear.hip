@@ -1,6 +1,7 @@
 // Products grouped by leaf: y[i] = W[g] x[i] + b[g] for the leaf g of row i, and the gradients
 //   dx[i] = W[g]^T dy[i],   dW[g] = sum over g's rows of dy[i] x[i]^T.
-// (db[g], the sum of dy over g's rows, is the embedding's gradient: leaf_embed.hip.)
+// and db[g], the sum of dy over g's rows: of the same tiles of dy as dW, except the largest, where
+// it is the embedding's gradient (leaf_embed.hip), as it is without dW.
 //
 // x is [n, K], W is [G, N, K], rows of a leaf are found through the route's `order` and `offsets`
 // (leaf_route.hip). Rows are gathered while a tile is loaded and scattered when it is stored, so
@@ -19,6 +20,9 @@ void launch_leaf_embed_grad(hipStream_t, int, const void*, int64_t, const int32_
 
 constexpr int kLlThreads = 256;
 constexpr int kLlWaves = kLlThreads / kWave;
+// Rows of the form without a route, one a lane. us so / by tiles with a kept route / and with the
+// sort, 2048 -> 1024 bf16: 64 rows of 64 leaves 36 / 45 / 49, of one 13 / 29 / 35; 4 rows 6 / 18 /
+// 24.
 constexpr int kLlSmallRows = 64;
 constexpr int kLlBigRows = 256;  // rows a leaf on average from which on 256-row tiles are taken
 
@@ -218,7 +222,9 @@ __device__ __forceinline__ V ll_load_or_zeros(bool there, const void* p) {
 
 // Blocks go to the 8 XCDs in turn, and each XCD has its own L2: runs of kLlXcdRun tiles stay on one
 // XCD, so that neighbours share the panels they read; runs go round, so that a stretch of tiles
-// without rows does not leave an XCD idle.
+// without rows does not leave an XCD idle. us with runs of 4 / 32 / 128, bf16: 32768 rows, 32
+// leaves, 2048 -> 4096 forward 656 / 656 / 776, dx 624 / 648 / 986, dW 702 / 717 / 826; 65536 rows,
+// 64 leaves, 2048 -> 2048 652 / 645 / 769, 654 / 647 / 807, 715 / 797 / 834.
 constexpr int kLlXcds = 8, kLlXcdRun = 32;
 __device__ __forceinline__ int64_t ll_xcd_order(int64_t blk) {
   const int64_t i = blk / kLlXcds;
@@ -350,7 +356,9 @@ __device__ __forceinline__ void ll_store_rows(const f32x4 (&acc)[SJ][SI], const 
 // kAligned: the next tile of depth goes from memory straight into the LDS buffer that is not read;
 // one barrier a tile. Otherwise chunks go through registers, whose loads wait until the tile's
 // products are issued. One tile of depth is on its way at a time, about 1.1 us each, which bounds
-// short depths: 10007 rows, 1000 -> 600 f16 28 us (430 TFLOP/s), 4096 -> 1280 136 us (770).
+// short depths: 10007 rows in 12 leaves, 1000 -> 600 f16 27 us (445 TFLOP/s), 4096 -> 1280 169 us
+// (620). f32 is bound by its products: 65536 rows in 64 leaves, 1024 -> 1024 forward 1209 us, dx
+// 1216 us (113 TFLOP/s; one library product of that size 142).
 template <typename T, bool kDx, int BJ, int BI, int WJ, int NW, bool kAligned>
 __global__ __launch_bounds__(NW* kWave) void ll_tile_kernel(LlTile a) {
   constexpr int E = Ll<T>::kEpc, KD = Ll<T>::kDepth, NT = NW * kWave;
@@ -497,8 +505,11 @@ __global__ __launch_bounds__(NW* kWave) void ll_tile_kernel(LlTile a) {
 // ---- short rows: at most 256 bytes of depth, so a wave holds its columns of the leaf's matrix
 // in registers and streams the leaf's rows past them, from memory straight into fragments, without
 // LDS or barriers. A wave takes up to kRowsTile rows of one leaf and SI * 16 columns. Bound by
-// memory latency and the f32 products: 1M rows, 64 -> 64 f32 in 4096 leaves 160 us (3.2 TB/s, 54 us
+// memory latency and the f32 products: 1M rows, 64 -> 64 f32 in 4096 leaves 152 us (3.4 TB/s, 54 us
 // of them products).
+// Rows of a wave's tile; us with 64 / 128 / 256: that forward pass 171 / 153 / 211, its dx 186 / 170
+// / 161; 100k rows in 1500 leaves, 32 -> 1 f32 7.6 / 8.4 / 11.7; 500k rows in 2000 leaves, 64 -> 64
+// bf16 38.5 / 37.8 / 42.5.
 constexpr int kRowsTile = 128, kRowsShift = 7;
 
 template <typename T, bool kDx, int STEPS, int SI, bool kAligned>
@@ -629,7 +640,8 @@ __global__ __launch_bounds__(kLlThreads) void ll_rows_kernel(LlTile a) {
 // descriptors: a lane's 32-bit offset is fixed and the depth is a scalar, so a fetch costs no
 // vector arithmetic; an operand has to lie within 4 GiB for that.
 // (Behind the last tile the same happens with zeros, which nothing uses.)
-// One leaf, 8192 x 8192 x 8192 bf16: forward 1231, row gradient 1354, weight gradient 1163 TFLOP/s;
+// One leaf, 8192 x 8192 x 8192 bf16: forward 1391, row gradient 1378, weight gradient 1157 TFLOP/s
+// (the library's products of the same operands 1611, 1396, 1211);
 // 1024 of depth take 23 us, a tile's start and end 12.
 //
 // A turned operand's depth rows lie in pairs, kPair bytes apart: 512 bytes a row and 32 to spare,
@@ -876,7 +888,9 @@ __device__ __forceinline__ void ll_store_sum(const LlGrad& a, int64_t unit, int 
     a.part_b[(unit - a.G) * a.N + c] = sum;
 }
 
-// zeros to dx of the rows without a leaf: 16 bytes a lane, block `part` of kLlZeroBlocks
+// zeros to dx of the rows without a leaf: 16 bytes a lane, block `part` of kLlZeroBlocks. us of a
+// gradient with 8 / 64 / 512 of them, 1M rows of 4096 leaves, 64 x 64 f32: a twentieth of the rows
+// without a leaf 406 / 304 / 303, half of them 2027 / 380 / 221.
 constexpr int kLlZeroBlocks = 64;
 template <typename T>
 __device__ __forceinline__ void ll_grad_zeros(const LlGrad& a, int64_t part) {
@@ -895,7 +909,7 @@ __device__ __forceinline__ void ll_grad_zeros(const LlGrad& a, int64_t part) {
 // kDx (one tile holds all of W): dx is made of the same tiles of dy, read once for both. Each wave
 // holds 16 columns of the leaf's W and multiplies all rows of a tile with them (B = 32: half of
 // them). Blocks behind the units' write the zeros of the rows without a leaf. 1M rows, 64 x 64 f32
-// in 4096 leaves: 294 us (2.6 TB/s), dW alone 176 (2.9 TB/s).
+// in 4096 leaves: 305 us (2.5 TB/s), dW alone 168 (3.05 TB/s), both with the join.
 template <typename T, int B, bool kAligned, bool kDx = false>
 __global__ __launch_bounds__(kLlThreads) void ll_grad_kernel(LlGrad a) {
   static_assert(!kDx || (B <= 64 && kAligned), "");
@@ -1178,7 +1192,7 @@ __global__ __launch_bounds__(kBigThreads, 2) void ll_big_grad_kernel(LlGrad a) {
 // leaves, or, if these are fewer, among the chunks in which they start: `per` blocks each, which
 // take a leaf's elements in turn, 4 a lane. The WAVES share a leaf's pieces and meet in LDS, so
 // that many pieces of a small matrix are not one chain of loads (1M rows of one leaf, 64 x 64 f32:
-// a weight gradient takes 218 us with 16 waves, 342 with none sharing).
+// a weight gradient takes 197 to 218 us with 16 waves, 342 with none sharing).
 template <typename T, int WAVES>
 __global__ __launch_bounds__(WAVES* kWave) void ll_join_kernel(LlGrad a, bool by_leaf, int per) {
   using A = std::conditional_t<sizeof(T) == 4, double, float>;
@@ -1447,6 +1461,8 @@ struct LlPacks {
 //   300000 rows, 100 leaves, 301 -> 199: 265 / 294, 325 / 428, 1026 / 806; 129 -> 127: 104 / 160,
 //     176 / 152, 459 / 298
 //   1500 rows, 2 leaves, 511 -> 513: 23 / 23, 35 / 26, 70 / 54
+//   below kLlPackRows, 2 leaves, 511 -> 513, a row gradient, all: 500 rows 39 / 22, 61 / 41; 1000
+//     rows 39 / 25, 69 / 46 (a lower bound would serve)
 // So gradients copy from widths of about 64 on, the row gradient alone from about 256 on, a forward
 // pass where the largest tiles follow; W, which a leaf's rows have to pay for, from 64 rows a leaf
 // on with dW and 192 without, 384 in a forward pass, and not in f32, whose products are slower.
