@@ -1,7 +1,7 @@
 // Products grouped by leaf: y[i] = W[g] x[i] + b[g] for the leaf g of row i, and the gradients
-//   dx[i] = W[g]^T dy[i],   dW[g] = sum over g's rows of dy[i] x[i]^T.
-// and db[g], the sum of dy over g's rows: of the same tiles of dy as dW, except the largest, where
-// it is the embedding's gradient (leaf_embed.hip), as it is without dW.
+//   dx[i] = W[g]^T dy[i],   dW[g] = sum over g's rows of dy[i] x[i]^T,
+// and db[g], the sum of dy over g's rows, which comes from the same tiles of dy as dW; without dW,
+// and beside its largest tiles, it is the embedding's gradient (leaf_embed.hip).
 //
 // x is [n, K], W is [G, N, K], rows of a leaf are found through the route's `order` and `offsets`
 // (leaf_route.hip). Rows are gathered while a tile is loaded and scattered when it is stored, so
@@ -507,9 +507,9 @@ __global__ __launch_bounds__(NW* kWave) void ll_tile_kernel(LlTile a) {
 // LDS or barriers. A wave takes up to kRowsTile rows of one leaf and SI * 16 columns. Bound by
 // memory latency and the f32 products: 1M rows, 64 -> 64 f32 in 4096 leaves 152 us (3.4 TB/s, 54 us
 // of them products).
-// Rows of a wave's tile; us with 64 / 128 / 256: that forward pass 171 / 153 / 211, its dx 186 / 170
-// / 161; 100k rows in 1500 leaves, 32 -> 1 f32 7.6 / 8.4 / 11.7; 500k rows in 2000 leaves, 64 -> 64
-// bf16 38.5 / 37.8 / 42.5.
+// Rows of a wave's tile; us with 64 / 128 / 256: that forward pass 171 / 153 / 211, its dx 186 /
+// 170 / 161; 100k rows in 1500 leaves, 32 -> 1 f32 7.6 / 8.4 / 11.7; 500k rows in 2000 leaves,
+// 64 -> 64 bf16 38.5 / 37.8 / 42.5.
 constexpr int kRowsTile = 128, kRowsShift = 7;
 
 template <typename T, bool kDx, int STEPS, int SI, bool kAligned>
