@@ -294,6 +294,7 @@ def _leaf_rows(buf, n: int, G: int):
             yield g, order[bounds[g] : bounds[g + 1]]
 
 
+@torch.autocast("cpu", enabled=False)  # (32-bit products, as the kernels')
 def _linear_plain(x, buf, w, b):
     y = torch.zeros((x.shape[0], w.shape[1]), dtype=torch.float32)
     for g, rows in _leaf_rows(buf, x.shape[0], w.shape[0]):
@@ -302,6 +303,7 @@ def _linear_plain(x, buf, w, b):
     return y.to(x.dtype)
 
 
+@torch.autocast("cpu", enabled=False)
 def _linear_plain_grad(dy, x, buf, w, need_x, need_w):
     dx = torch.zeros(x.shape, dtype=torch.float32) if need_x else None
     dw = torch.zeros(w.shape, dtype=torch.float32) if need_w else None

@@ -9,6 +9,7 @@ import torch
 import torch.autograd.forward_ad as fwad
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils.checkpoint import checkpoint
 from torch.utils.flop_counter import FlopCounterMode
 
 from mpitree_amd import (DecisionTreeClassifier, LeafRoute, leaf_embedding, leaf_linear,
@@ -445,3 +446,48 @@ def test_an_estimator_takes_rows_of_any_layout(device):
         assert torch.equal(est.leaf_linear(torch.from_numpy(X), w), want)
         # (numpy's own bytes the other way round)
         assert torch.equal(est.leaf_linear(X.astype(">f4"), w), want)
+
+
+# ------------------------------------------------------- inside torch's other machinery
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [9, 90])
+def test_recomputed_in_the_backward_pass(device, n):
+    ids, x, w, b = operands(device, n)
+    for leaves in (ids, leaf_route(ids, 3)):
+        args = [t.clone().requires_grad_() for t in (x, w, b)]
+
+        def step(x, w, b):
+            return leaf_linear(x, leaves, w, b) * leaf_embedding(leaves, b, scale=0.5)
+
+        want = torch.autograd.grad(step(*args).sum(), args)
+        y = checkpoint(step, *args, use_reentrant=False)
+        for p, q in zip(torch.autograd.grad(y.sum(), args), want):
+            assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_in_inference_mode_and_autocast(device):
+    for call, args in forward_calls(device):
+        want = call(*args)
+        with torch.inference_mode():
+            assert torch.equal(call(*args), want)
+        with torch.autocast(device, dtype=torch.bfloat16):  # the operands' types stay
+            got = call(*args)
+        assert got.dtype == want.dtype and torch.equal(got, want)
+        args = [a.clone().requires_grad_() for a in args]
+        want = torch.autograd.grad(call(*args).sum(), args)
+        with torch.autocast(device, dtype=torch.bfloat16):
+            for p, q in zip(torch.autograd.grad(call(*args).sum(), args), want):
+                assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradients_kept_for_a_second_backward(device):
+    for call, args in forward_calls(device):
+        args = [a.clone().requires_grad_() for a in args]
+        y = call(*args).square().sum()
+        first = torch.autograd.grad(y, args, retain_graph=True)
+        for p, q in zip(first, torch.autograd.grad(y, args)):
+            assert torch.equal(p, q)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y, args)
