@@ -294,7 +294,6 @@ def _leaf_rows(buf, n: int, G: int):
             yield g, order[bounds[g] : bounds[g + 1]]
 
 
-@torch.autocast("cpu", enabled=False)  # (32-bit products, as the kernels')
 def _linear_plain(x, buf, w, b):
     y = torch.zeros((x.shape[0], w.shape[1]), dtype=torch.float32)
     for g, rows in _leaf_rows(buf, x.shape[0], w.shape[0]):
@@ -303,7 +302,6 @@ def _linear_plain(x, buf, w, b):
     return y.to(x.dtype)
 
 
-@torch.autocast("cpu", enabled=False)
 def _linear_plain_grad(dy, x, buf, w, need_x, need_w):
     dx = torch.zeros(x.shape, dtype=torch.float32) if need_x else None
     dw = torch.zeros(w.shape, dtype=torch.float32) if need_w else None
@@ -321,7 +319,8 @@ def _linear_forward(x, ids, buf, w, b):
     (n, K), (G, N, _) = x.shape, w.shape
     if not x.is_cuda:
         buf = buf if buf is not None else _sort(ids, G)
-        return _linear_plain(x, buf, w, b), buf
+        with torch.autocast("cpu", enabled=False):  # (32-bit products, as the kernels')
+            return _linear_plain(x, buf, w, b), buf
     _check_launch(x, w, b, ids)
     hip, kind, dev, ids = native.hip(), _TYPES[x.dtype], x.get_device(), ids.contiguous()
     wide, bias = ids.dtype == torch.int64, 0 if b is None else b.data_ptr()
@@ -377,7 +376,8 @@ class _Linear(torch.autograd.Function):
         if dy.is_cuda:
             grads = _linear_grad(dy, x, buf, w, need_x, need_w, need_b)
         else:
-            grads = _linear_plain_grad(dy, x, buf, w, need_x, need_w)
+            with torch.autocast("cpu", enabled=False):
+                grads = _linear_plain_grad(dy, x, buf, w, need_x, need_w)
             grads += (_sum_by_leaf_plain(dy, buf, w.shape[0], 1.0) if need_b else None,)
         return (*grads, None, None)
 
