@@ -143,9 +143,10 @@ def test_float32_sums_are_held_in_64_bits(device, n, G, D):
 
 
 # ------------------------------------------------------------------------------ linear
-def linear_exact(dtype, ids, G, K, N, seed, shift=0, far=0):
+def linear_exact(dtype, ids, G, K, N, seed, shift=0, far=0, poison=None):
     """y, dx, dW and db for equality. shift: rows of x and dy start that many elements behind an
-    aligned address; far: elements between them, for x and dy in one buffer."""
+    aligned address; far: elements between them, for x and dy in one buffer. poison: NaN beside the
+    rows of x and dy (that many columns), in rows without a leaf and in matrices without rows."""
     g, n = gen(seed), ids.numel()
     if far:
         big = torch.empty(n * far, device="cuda", dtype=dtype)
@@ -157,6 +158,14 @@ def linear_exact(dtype, ids, G, K, N, seed, shift=0, far=0):
         x = whole(g, (n, K + shift), dtype)[:, shift:]
         dy = whole(g, (n, N + shift), dtype)[:, shift:]
     w, b = whole(g, (G, N, K), dtype), whole(g, (G, N), dtype, 9)
+    if poison is not None:
+        x, dy = (torch.cat([t, torch.full((n, poison), float("nan"), device="cuda", dtype=dtype)],
+                           1)[:, : t.shape[1]] for t in (x, dy))
+        gone = (ids < 0) | (ids >= G)
+        x[gone] = dy[gone] = float("nan")
+        met = torch.zeros(G, dtype=torch.bool, device="cuda")
+        met[ids[~gone].long()] = True
+        w[~met] = b[~met] = float("nan")
     for p in (x, w, b):
         p.requires_grad_()
     y = leaf_linear(x, ids, w, b)
@@ -260,3 +269,30 @@ def test_rows_that_are_one_row(dtype, n):
     want = torch.where((ids >= 0)[:, None],
                        ((W * X).sum(2) + b.detach().double())[ids.clamp(min=0).long()], 0.0)
     assert torch.equal(y, want.to(dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,G,K,N,poison", [
+    (50, 9, 40, 24, 8), (64, 100, 33, 17, 1), (3000, 7, 64, 64, 8), (3000, 2500, 64, 48, 8),
+    (3000, 90, 13, 21, 3), (5000, 12, 264, 136, 16), (5000, 12, 201, 199, 1), (9000, 3, 32, 1, 7),
+    (16_500, 20, 1024, 1032, 8), (16_500, 20, 1023, 1029, 3)])
+def test_nan_around_the_operands(dtype, n, G, K, N, poison):
+    # nothing that is no operand of a row reaches it, nor what a tile holds behind its end
+    linear_exact(dtype, skewed(n, G, 1.0, 0.1), G, K, N, n + K, poison=poison)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,G,D,pad", [(30, 9, 7, 1), (3000, 50, 63, 5), (20_000, 3, 64, 8),
+                                       (9000, 4000, 1024, 8)])
+def test_nan_around_a_table_and_its_gradient(dtype, n, G, D, pad):
+    g, ids = gen(n), skewed(n, G, 1.0, 0.1)
+    dy, t = whole(g, (n, D + pad), dtype), whole(g, (G, D + pad), dtype, 9)
+    dy[:, D:], t[:, D:] = float("nan"), float("nan")
+    dy[ids < 0] = float("nan")
+    want = sums64(ids, G, torch.where((ids < 0)[:, None], 0.0, dy[:, :D]).to(dtype))
+    assert torch.equal(table_gradient(ids, G, dy[:, :D]), want.to(dtype))
+    y = leaf_embedding(ids, t[:, :D], scale=2.0)
+    rows = t[:, :D].double()[ids.clamp(min=0)] * 2.0
+    assert torch.equal(y, torch.where((ids < 0)[:, None], 0.0, rows).to(dtype))
